@@ -721,6 +721,87 @@ int nmtg_multi_tensor_l2norm_scale(int n_tensors, const void* const* in, void* c
                                    void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Attention with a sliding window and a few first tokens that stay visible (sinks), forward and
+ * backward (no counterpart in the reference, whose attention is dense or masked by bytes). Query i
+ * of a sequence sees key j where j <= i and (j > i - window or j < sinks); window >= 1, sinks >= 0.
+ * lengths: int32 [batch] (values outside [0, len] are clamped) or null; positions at and behind a
+ * sequence's length see nothing and are seen by nobody, their outputs and gradients are zeros.
+ * q, out, dout, dq [len, batch, heads, head_dim]; k, v, dk, dv [len, batch, kv_heads, head_dim],
+ * heads a multiple of kv_heads: query head h reads key / value head h / (heads / kv_heads).
+ * strides: HOST array of three int64 per tensor (position, sequence, head; in elements, multiples of
+ * 8; head_dim contiguous), in the order of the tensor arguments: q, k, v, out for the forward and
+ * dout, q, k, v, out, dq, dk, dv for the backward. head_dim 64 or 128, fp16 or bf16, products and
+ * sums in fp32, probabilities and score gradients rounded to the 16-bit type for their products.
+ * softmax_lse: fp32 [batch, heads, len], natural logarithm (-inf where nothing is visible), written
+ * by the forward and read by the backward. workspace: nmtg_window_attn_bwd_workspace_bytes bytes,
+ * 256-byte aligned. An inf or NaN at a position that some query of the same 64 sees may reach the
+ * other queries of that tile (zero times it); positions behind a length are never read.
+ * ------------------------------------------------------------------------------------------ */
+int nmtg_window_attn_fwd(const void* q, const void* k, const void* v, void* out, float* softmax_lse,
+                         const int32_t* lengths, const int64_t* strides, int64_t len, int64_t batch,
+                         int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window,
+                         int64_t sinks, float softmax_scale, int dtype, void* stream);
+
+int64_t nmtg_window_attn_bwd_workspace_bytes(int64_t len, int64_t batch, int64_t heads,
+                                             int64_t kv_heads, int64_t head_dim, int64_t window,
+                                             int64_t sinks);
+
+int nmtg_window_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
+                         const void* out, const float* softmax_lse, void* dq, void* dk, void* dv,
+                         const int32_t* lengths, const int64_t* strides, int64_t len, int64_t batch,
+                         int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window,
+                         int64_t sinks, float softmax_scale, int dtype, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * A key / value cache in 4 or 8 bits for incremental decoding (no counterpart in the reference,
+ * whose caches hold the working dtype). Per sequence and key / value head, `capacity` positions of
+ *   codes  uint8 [batch, kv_heads, capacity, head_dim * bits / 8]   dense, 16-byte aligned
+ *   scales uint8 [batch, kv_heads, capacity, head_dim / 32]         dense
+ * for keys and for values. A block of 32 neighbouring elements has the scale 2^(byte - 127), the
+ * smallest under which its largest magnitude is at most 7 (4 bits) or 464 (8 bits), at least 2^-126;
+ * elements are E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6; the lower nibble is the lower index) or E4M3 (up to
+ * 448), rounded to nearest, ties to even. A block with an inf or NaN has scale byte 255 and reads
+ * back as NaN. head_dim 64 or 128; the 16-bit side is fp16 or bf16.
+ *
+ * nmtg_kv_cache_write: rows [count, batch, kv_heads, head_dim] (three strides each) to positions
+ *   starts[b] .. of sequence b (device int32), or start .. where starts is null. Rows that `starts`
+ *   puts outside [0, capacity) are dropped.
+ * nmtg_kv_cache_read: the mirror image, to dense k, v [count, batch, kv_heads, head_dim]; positions
+ *   outside the cache read as zeros.
+ * nmtg_kv_cache_attn: the newest tq positions of every sequence over its cache: query i of sequence b
+ *   stands at position lengths[b] - tq + i (lengths: device int32, the positions held, these included;
+ *   clamped to [0, capacity]) and sees positions up to its own, with window > 0 those of its window
+ *   and the first `sinks` only. A query that sees nothing gets zeros. longest: an upper bound of
+ *   lengths known to the host, which sizes the launch and the workspace; results do not depend on it
+ *   beyond the order of sums. q, out [tq, batch, heads, head_dim] by three strides. workspace:
+ *   nmtg_kv_cache_attn_workspace_bytes bytes, 16-byte aligned (none where that is 0).
+ * ------------------------------------------------------------------------------------------ */
+int nmtg_kv_cache_write(const void* k, int64_t k_stride_t, int64_t k_stride_b, int64_t k_stride_h,
+                        const void* v, int64_t v_stride_t, int64_t v_stride_b, int64_t v_stride_h,
+                        uint8_t* k_codes, uint8_t* k_scales, uint8_t* v_codes, uint8_t* v_scales,
+                        const int32_t* starts, int64_t start, int64_t count, int64_t batch,
+                        int64_t kv_heads, int64_t head_dim, int64_t capacity, int bits, int dtype,
+                        void* stream);
+
+int nmtg_kv_cache_read(const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
+                       const uint8_t* v_scales, void* k, void* v, const int32_t* starts, int64_t start,
+                       int64_t count, int64_t batch, int64_t kv_heads, int64_t head_dim,
+                       int64_t capacity, int bits, int dtype, void* stream);
+
+int64_t nmtg_kv_cache_attn_workspace_bytes(int64_t tq, int64_t batch, int64_t heads, int64_t kv_heads,
+                                           int64_t head_dim, int64_t longest, int64_t window,
+                                           int64_t sinks);
+
+int nmtg_kv_cache_attn(const void* q, int64_t q_stride_t, int64_t q_stride_b, int64_t q_stride_h,
+                       const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
+                       const uint8_t* v_scales, const int32_t* lengths, void* out,
+                       int64_t out_stride_t, int64_t out_stride_b, int64_t out_stride_h, int64_t tq,
+                       int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                       int64_t capacity, int64_t longest, int64_t window, int64_t sinks, float scale,
+                       int bits, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Per-kernel timing for benchmarks (no counterpart in the reference, whose tests time whole ops
  * with CUDA events, e.g. onmt/modules/test_layer_norm.py:14-31). Between nmtg_trace_begin() and
  * nmtg_trace_end() every kernel the library enqueues is bracketed by two HIP events on its

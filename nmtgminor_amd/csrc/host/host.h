@@ -1,7 +1,7 @@
 // Shared pieces of the native host layer (nmtgminor_amd/_host.so): the table of C entry points it calls, and the
 // operators as functions from tensors to tensors (allocate the results, enqueue the kernels). ops.cpp implements them,
 // autograd.cpp wraps them in autograd nodes, layers.cpp composes the transformer layers, attention.cpp the attention modules, loss.cpp the output
-// projection with its loss, optim.cpp prepares the optimizer's passes.
+// projection with its loss, optim.cpp prepares the optimizer's passes, long_context.cpp window attention and the quantised cache.
 //
 // Why it exists: interpreter, ctypes and autograd bookkeeping of a call through the Python functions take several times what
 // the kernels of a small batch take. Host time of a call on [64 x 512], LayerNorm / feed-forward block / dropout + add: forward
@@ -36,7 +36,8 @@ using std::optional;
   X(flash_attn_fwd) X(flash_attn_bwd) X(flash_attn_key_info_bytes) X(flash_attn_time_info_bytes)                      \
   X(flash_attn_batched_fwd) X(flash_attn_batched_bwd) X(multi_tensor_adam) X(multi_tensor_clip)                       \
   X(multi_tensor_l2norm) X(multi_tensor_l2norm_workspace_bytes) X(flash_attn_batched_fwd_probs) X(linear_step) X(step_linear) X(step_linear_ok) X(gemm_workspace_bytes) \
-  X(xentropy_bwd_colsum) X(xentropy_bwd_colsum_parts)
+  X(xentropy_bwd_colsum) X(xentropy_bwd_colsum_parts) X(window_attn_fwd) X(window_attn_bwd)                              \
+  X(window_attn_bwd_workspace_bytes) X(kv_cache_write) X(kv_cache_read) X(kv_cache_attn) X(kv_cache_attn_workspace_bytes)
 
 struct Api {
 #define X(name) decltype(&nmtg_##name) name = nullptr;
@@ -162,5 +163,6 @@ void define_layers(pybind11::module_& m);
 void define_optim(pybind11::module_& m);
 void define_attention(pybind11::module_& m);
 void define_loss(pybind11::module_& m);
+void define_long_context(pybind11::module_& m);
 
 }  // namespace nmtg_host

@@ -361,4 +361,5 @@ PYBIND11_MODULE(_host, m) {
   nmtg_host::define_optim(m);
   nmtg_host::define_attention(m);
   nmtg_host::define_loss(m);
+  nmtg_host::define_long_context(m);
 }

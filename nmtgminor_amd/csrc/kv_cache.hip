@@ -1,0 +1,588 @@
+// A key / value cache in 4 or 8 bits: its rows written (quantised), read back, and attended to by the newest positions.
+//
+// Format. Along the head dimension a row is cut into blocks of 32 elements. A block keeps a scale byte s and 32 elements of
+// 4 bits (E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6) or 8 bits (E4M3, up to 448); it stands for element * 2^(s - 127). The scale is
+// the smallest power of two under which the block's largest magnitude is at most 7 (464), the upper end of what rounds to
+// the largest element: nothing is further from its held value than half a step, and since a division by a power of two is
+// exact the codes do not depend on the precision they are computed in. A block that holds an inf or NaN gets scale byte
+// 255 and reads back as NaN throughout. Elements round to nearest, ties to even (the conversion instructions' own rule).
+//
+// Layout. codes [batch, kv_heads, capacity, head_dim * bits / 8], scales [batch, kv_heads, capacity, head_dim / 32]: the rows
+// of one head follow each other, so that a tile of 32 positions is one contiguous piece of memory for the kernel that is
+// bound by reading it (the decoding step).
+#include "gemm_ring.hip.h"
+#include <algorithm>
+
+namespace nmtg {
+namespace {
+
+constexpr int KV_BLOCK = 32;      // elements per scale
+constexpr int KV_TILE = 32;       // positions per step of a wavefront in the attention kernel
+constexpr int KV_WAVES = 4;
+constexpr int KV_ROWS = 16;       // query rows per block: the columns of the 16 x 16 x 32 products
+constexpr float KV_NEG = -1e30f;
+constexpr float KV_LAZY = 8.f;
+constexpr float KV_LOG2E = 1.4426950408889634f;
+
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
+__device__ __forceinline__ int64_t most(int64_t a, int64_t b) { return a > b ? a : b; }
+
+// 2^(byte - 127) as the conversion instructions take it: only the exponent field counts, 0 is 2^-127 and 255 gives NaN
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// Four (4 bits) or two (8 bits) times two elements of a word: pair P as two 16-bit elements of T in one register
+template <typename T, int BITS, int P>
+__device__ __forceinline__ uint32_t held_pair(uint32_t word, float scale) {
+  if constexpr (BITS == 4) {
+    if constexpr (elem<T>::dtype == NMTG_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, P));
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, P));
+  } else {
+    if constexpr (elem<T>::dtype == NMTG_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, P != 0));
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, scale, P != 0));
+  }
+}
+// all pairs of one word
+template <typename T, int BITS>
+__device__ __forceinline__ void held_word(uint32_t word, float scale, uint32_t* out) {
+  out[0] = held_pair<T, BITS, 0>(word, scale);
+  out[1] = held_pair<T, BITS, 1>(word, scale);
+  if constexpr (BITS == 4) {
+    out[2] = held_pair<T, BITS, 2>(word, scale);
+    out[3] = held_pair<T, BITS, 3>(word, scale);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------- write and read
+struct KvRows {
+  const void *k, *v;              // write: 16-bit rows [count, batch, kv_heads, head_dim] by three strides
+  void *k_out, *v_out;            // read: dense [count, batch, kv_heads, head_dim]
+  uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+  const int32_t* starts;          // first cache row of every sequence, or null: `start` for all
+  int64_t k_st, k_sb, k_sh, v_st, v_sb, v_sh;
+  int64_t start, count, capacity, total;   // total: count * batch * kv_heads * (head_dim / 8)
+  int batch, kv_heads;
+};
+
+// Item i of a call: 8 elements c of row (t, b, h), counted in the order of the 16-bit rows.
+struct KvItem { int64_t t; int b, h, c; int64_t row; bool live; };
+template <int D>
+__device__ __forceinline__ KvItem kv_item(const KvRows& a, int64_t i) {
+  constexpr int CH = D / 8;
+  KvItem r;
+  r.c = static_cast<int>(i % CH);
+  const int64_t rest = i / CH, bh = rest % (static_cast<int64_t>(a.batch) * a.kv_heads);
+  r.t = rest / (static_cast<int64_t>(a.batch) * a.kv_heads);
+  r.h = static_cast<int>(bh % a.kv_heads);
+  r.b = static_cast<int>(bh / a.kv_heads);
+  const int64_t at = (a.starts != nullptr ? a.starts[r.b] : a.start) + r.t;
+  r.live = at >= 0 && at < a.capacity;
+  r.row = (static_cast<int64_t>(r.b) * a.kv_heads + r.h) * a.capacity + at;
+  return r;
+}
+
+// One lane per 8 elements, four neighbouring lanes per block of 32; blockIdx.y: keys or values.
+template <typename T, int D, int BITS>
+__global__ __launch_bounds__(256) void kv_write_kernel(KvRows a) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= a.total) return;                   // total is a multiple of 8: whole blocks of four lanes leave together
+  const bool keys = blockIdx.y == 0;
+  const KvItem it = kv_item<D>(a, i);
+  if (!it.live) return;                       // the four lanes of a block share a row
+  const T* src = static_cast<const T*>(keys ? a.k : a.v) + it.t * (keys ? a.k_st : a.v_st) + it.b * (keys ? a.k_sb : a.v_sb) +
+                 it.h * (keys ? a.k_sh : a.v_sh) + 8 * it.c;
+  const pack<T, 8> raw = load_raw<T, 8>(src);
+  uint32_t w[4];
+  __builtin_memcpy(w, &raw, 16);
+  // magnitudes of 16-bit floats compare as integers
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
+  top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0xB1, 0xf, 0xf, true)));
+  top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x4E, 0xf, 0xf, true)));
+  const bool finite = top < (elem<T>::dtype == NMTG_BF16 ? 0x7f80u : 0x7c00u);
+  T largest;
+  largest.bits = static_cast<uint16_t>(top);
+  const uint32_t amax = __float_as_uint(elem<T>::to_float(largest));
+  constexpr int EMAX = BITS == 4 ? 2 : 8;
+  constexpr uint32_t UP = BITS == 4 ? 0x600000u : 0x680000u;      // fraction of 1.75 (7 / 4) and of 1.8125 (464 / 256)
+  const int byte = finite ? max(1, static_cast<int>(amax >> 23) - EMAX + ((amax & 0x7fffffu) > UP ? 1 : 0)) : 255;
+  const float scale = scale_of(static_cast<uint32_t>(finite ? byte : 127));
+  uint8_t* codes = (keys ? a.k_codes : a.v_codes) + it.row * (D * BITS / 8) + it.c * BITS;
+  if constexpr (BITS == 4) {
+    uint32_t out = 0;
+    if constexpr (elem<T>::dtype == NMTG_BF16) {
+      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(out, __builtin_bit_cast(bf16x2_t, w[0]), scale, 0);
+      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(out, __builtin_bit_cast(bf16x2_t, w[1]), scale, 1);
+      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(out, __builtin_bit_cast(bf16x2_t, w[2]), scale, 2);
+      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(out, __builtin_bit_cast(bf16x2_t, w[3]), scale, 3);
+    } else {
+      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[0]), scale, 0);
+      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[1]), scale, 1);
+      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[2]), scale, 2);
+      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[3]), scale, 3);
+    }
+    *reinterpret_cast<uint32_t*>(codes) = finite ? out : 0u;
+  } else {
+    s16x2_t out[2] = {{0, 0}, {0, 0}};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if constexpr (elem<T>::dtype == NMTG_BF16) {
+        out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(out[e], __builtin_bit_cast(bf16x2_t, w[2 * e]), scale, false);
+        out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(out[e], __builtin_bit_cast(bf16x2_t, w[2 * e + 1]), scale, true);
+      } else {
+        out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(out[e], __builtin_bit_cast(f16x2_t, w[2 * e]), scale, false);
+        out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(out[e], __builtin_bit_cast(f16x2_t, w[2 * e + 1]), scale, true);
+      }
+    }
+    uint2 two = make_uint2(__builtin_bit_cast(uint32_t, out[0]), __builtin_bit_cast(uint32_t, out[1]));
+    *reinterpret_cast<uint2*>(codes) = finite ? two : make_uint2(0, 0);
+  }
+  if ((it.c & 3) == 0) (keys ? a.k_scales : a.v_scales)[it.row * (D / KV_BLOCK) + it.c / 4] = static_cast<uint8_t>(byte);
+}
+
+template <typename T, int D, int BITS>
+__global__ __launch_bounds__(256) void kv_read_kernel(KvRows a) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= a.total) return;
+  const bool keys = blockIdx.y == 0;
+  const KvItem it = kv_item<D>(a, i);
+  uint4 out = make_uint4(0, 0, 0, 0);
+  if (it.live) {
+    const uint8_t* codes = (keys ? a.k_codes : a.v_codes) + it.row * (D * BITS / 8) + it.c * BITS;
+    const float scale = scale_of((keys ? a.k_scales : a.v_scales)[it.row * (D / KV_BLOCK) + it.c / 4]);
+    uint32_t w[4];
+    if constexpr (BITS == 4) {
+      held_word<T, 4>(*reinterpret_cast<const uint32_t*>(codes), scale, w);
+    } else {
+      const uint2 two = *reinterpret_cast<const uint2*>(codes);
+      held_word<T, 8>(two.x, scale, w);
+      held_word<T, 8>(two.y, scale, w + 2);
+    }
+    out = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static_cast<uint4*>(keys ? a.k_out : a.v_out)[i] = out;
+}
+
+// ------------------------------------------------------------------------------------------------------------ attention
+// One block per (split, key / value head and group of 16 query rows, sequence). The 16 rows are the newest positions of the
+// query heads that share the key / value head: row r is position r / g, head r % g of the group. A wavefront takes tiles of
+// 32 positions, each read once from memory into registers one tile ahead:
+//   S^T = K Q^T (16 x 16 x 32 products, twice 16 positions): lane (r = lane % 16, g = lane / 16) holds the codes of
+//   quarter g of position r, head_dim / 4 consecutive elements as they lie in memory; the products sum over the head
+//   dimension in whatever order both operands share, so the queries are read in the same order and no code is moved.
+//   The result has one query row per lane column and positions 4 g .. 4 g + 3 (+ 16) in a lane's registers, which is the
+//   operand layout of the second product, again with the tile's positions in an order both operands share:
+//   O^T = V^T P^T: lane (c, g) holds elements [c D / 16, (c + 1) D / 16) of those eight positions; converted to pairs of
+//   neighbouring elements and re-paired by position (one byte permutation per register) they are the operands of D / 16
+//   products.
+// The running maximum follows lazily (it moves when a score exceeds it by 2^8), the sums stay per lane until the end.
+struct KvAttn {
+  const void* q;
+  const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+  const int32_t* lengths;
+  void* out;
+  float *part, *part_ml;          // splits > 1: [splits][batch, kv_heads, rows][D] and [..][2] (maximum, sum)
+  int64_t q_st, q_sb, q_sh, o_st, o_sb, o_sh;
+  int64_t capacity;
+  int tq, heads, kv_heads, group, rows, splits;   // group: query heads per key / value head, rows: tq * group
+  int64_t window;                 // 0: none
+  int64_t sinks;
+  float scale_log2;
+};
+
+template <typename T> __device__ __forceinline__ f32x4_t mfma_16x16x32(const uint4& a, const uint4& b, f32x4_t c);
+template <> __device__ __forceinline__ f32x4_t mfma_16x16x32<bf16_t>(const uint4& a, const uint4& b, f32x4_t c) {
+  typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x4_t mfma_16x16x32<f16_t>(const uint4& a, const uint4& b, f32x4_t c) {
+  typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+
+template <typename T> struct pair16;
+template <> struct pair16<f16_t> { typedef f16x2_t type; };
+template <> struct pair16<bf16_t> { typedef bf16x2_t type; };
+template <typename T>
+__device__ __forceinline__ uint32_t round_pair(float lo, float hi) {
+  const f32x2_t v = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, typename pair16<T>::type));
+}
+
+// The codes and scales of one tile in a lane's registers.
+template <int D, int BITS>
+struct KvTile {
+  static constexpr int KW = D * BITS / 8 / 4 / 4;    // words of a quarter row
+  static constexpr int VW = D * BITS / 8 / 16 >= 4 ? D * BITS / 8 / 16 / 4 : 1;   // words of a sixteenth of a row
+  static constexpr int VB = D * BITS / 8 / 16;       // its bytes (2, 4 or 8)
+  uint32_t k[2][KW], ks[2], v[8][VW], vs[8];
+  // position: the tile's first; limit: the last row that may be read
+  __device__ __forceinline__ void load(const uint8_t* kc, const uint8_t* ksc, const uint8_t* vc, const uint8_t* vsc, int64_t position,
+                                       int64_t limit, int lane) {
+    constexpr int RB = D * BITS / 8, SB = D / KV_BLOCK;
+    const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int64_t row = least(position + 16 * m + r, limit);
+      __builtin_memcpy(k[m], __builtin_assume_aligned(kc + row * RB + g * (RB / 4), RB / 4 >= 16 ? 16 : RB / 4), 4 * KW);
+      ks[m] = ksc[row * SB + g * SB / 4];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t row = least(position + 16 * (e / 4) + 4 * g + (e & 3), limit);
+      const uint8_t* p = vc + row * RB + r * VB;
+      if constexpr (VB == 2) v[e][0] = *reinterpret_cast<const uint16_t*>(p);
+      else __builtin_memcpy(v[e], __builtin_assume_aligned(p, VB), VB);
+      vs[e] = vsc[row * SB + r * SB / 16];
+    }
+  }
+};
+
+template <typename T, int D, int BITS>
+__global__ __launch_bounds__(KV_WAVES * 64) void kv_attn_kernel(KvAttn a) {
+  constexpr int NK = D / 32, NV = D / 16;
+  constexpr int RB = D * BITS / 8, SB = D / KV_BLOCK;
+  __shared__ float lds_ml[KV_WAVES][KV_ROWS][2];
+  __shared__ float lds_o[KV_WAVES][KV_ROWS][D + 4];
+  const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
+  const int r = lane & 15, g = lane >> 4;
+  const int b = static_cast<int>(blockIdx.z), kvh = static_cast<int>(blockIdx.y) % a.kv_heads;
+  const int row0 = static_cast<int>(blockIdx.y) / a.kv_heads * KV_ROWS, split = static_cast<int>(blockIdx.x);
+  const int nrows = min(KV_ROWS, a.rows - row0);
+  const int64_t len = least(most(a.lengths[b], 0), a.capacity);
+  // this lane's query row, its position, and the positions of the block's first and last row
+  const int row = row0 + min(r, nrows - 1);
+  const int64_t qpos = len - a.tq + row / a.group;
+  const int64_t qfirst = len - a.tq + row0 / a.group, qlast = len - a.tq + (row0 + nrows - 1) / a.group;
+  const int64_t window = a.window > 0 ? a.window : a.capacity + 1;
+
+  // tiles of the sinks, then tiles from the first row's window on
+  const int64_t end = most(qlast + 1, 0), tiles_end = (end + KV_TILE - 1) / KV_TILE;
+  const int64_t lo = least(most(qfirst - window + 1, 0) / KV_TILE, tiles_end);
+  const int64_t ns = least((least(a.sinks, end) + KV_TILE - 1) / KV_TILE, lo);
+  const int64_t tiles = ns + tiles_end - lo;
+  const int64_t per = (tiles + a.splits - 1) / a.splits, t0 = least(split * per, tiles), t1 = least(t0 + per, tiles);
+
+  const int64_t bh = static_cast<int64_t>(b) * a.kv_heads + kvh;
+  const uint8_t *kc = a.k_codes + bh * a.capacity * RB, *ksc = a.k_scales + bh * a.capacity * SB;
+  const uint8_t *vc = a.v_codes + bh * a.capacity * RB, *vsc = a.v_scales + bh * a.capacity * SB;
+  uint4 qf[NK];
+  {
+    const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(row / a.group) * a.q_st + static_cast<int64_t>(b) * a.q_sb +
+                  static_cast<int64_t>(kvh * a.group + row % a.group) * a.q_sh + g * (D / 4);
+#pragma unroll
+    for (int s = 0; s < NK; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + 8 * s);
+  }
+  f32x4_t o[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m = KV_NEG, l = 0.f;
+
+  KvTile<D, BITS> next;
+  int64_t t = t0 + wave;
+  auto position_of = [&](int64_t i) { return (i < ns ? i : i - ns + lo) * KV_TILE; };
+  if (t < t1) next.load(kc, ksc, vc, vsc, position_of(t), a.capacity - 1, lane);
+  for (; t < t1; t += KV_WAVES) {
+    const int64_t position = position_of(t);
+    KvTile<D, BITS> tile = next;
+    if (t + KV_WAVES < t1) next.load(kc, ksc, vc, vsc, position_of(t + KV_WAVES), a.capacity - 1, lane);
+    f32x4_t s[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      const float scale = scale_of(tile.ks[h]);
+      uint32_t kw[4 * NK];
+#pragma unroll
+      for (int w = 0; w < KvTile<D, BITS>::KW; ++w) held_word<T, BITS>(tile.k[h][w], scale, kw + w * (BITS == 4 ? 4 : 2));
+#pragma unroll
+      for (int x = 0; x < NK; ++x) s[h] = mfma_16x16x32<T>(make_uint4(kw[4 * x], kw[4 * x + 1], kw[4 * x + 2], kw[4 * x + 3]), qf[x], s[h]);
+    }
+    // positions that some row does not see: only where the tile crosses the newest positions or an edge of a window
+    const bool inside = position + KV_TILE - 1 <= qfirst && (position > qlast - window || position + KV_TILE <= a.sinks);
+    float sc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sc[e] = s[e / 4][e & 3] * a.scale_log2;
+    uint32_t dead = 0;
+    if (!inside) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int64_t at = position + 16 * (e / 4) + 4 * g + (e & 3);
+        if (at > qpos || (at <= qpos - window && at >= a.sinks)) { dead |= 1u << e; sc[e] = KV_NEG; }
+        // What no row of the block sees (rows behind the newest, not written yet, among it) must not meet its probability of
+        // zero: an inf or NaN there would come through the product.
+        if (at > qlast || (at <= qfirst - window && at >= a.sinks)) {
+#pragma unroll
+          for (int w = 0; w < KvTile<D, BITS>::VW; ++w) tile.v[e][w] = 0;
+          tile.vs[e] = 127;
+        }
+      }
+    }
+    float top = sc[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[e]);
+    if (__builtin_amdgcn_ballot_w64(top > m + KV_LAZY) != 0) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float m_new = top > m + KV_LAZY ? top : m;      // the same in the four lanes of a query row
+      const float alpha = fast_exp2(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) o[j] *= alpha;
+    }
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      p[e] = fast_exp2(sc[e] - m);
+      if (!inside && ((dead >> e) & 1u) != 0) p[e] = 0.f;    // m may still be the initial one
+      l += p[e];
+    }
+    // probabilities rounded to the 16-bit type of the product (relative to a maximum at most 2^8 below the true one)
+    const uint4 pf = make_uint4(round_pair<T>(p[0], p[1]), round_pair<T>(p[2], p[3]), round_pair<T>(p[4], p[5]), round_pair<T>(p[6], p[7]));
+    // two positions at a time: pairs of neighbouring elements become pairs of neighbouring positions
+    uint32_t vw[NV][4];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      uint32_t x[NV / 2], y[NV / 2];
+      if constexpr (KvTile<D, BITS>::VB == 2) {
+        x[0] = held_pair<T, BITS, 0>(tile.v[e][0], scale_of(tile.vs[e]));
+        x[1] = held_pair<T, BITS, 1>(tile.v[e][0], scale_of(tile.vs[e]));
+        y[0] = held_pair<T, BITS, 0>(tile.v[e + 1][0], scale_of(tile.vs[e + 1]));
+        y[1] = held_pair<T, BITS, 1>(tile.v[e + 1][0], scale_of(tile.vs[e + 1]));
+      } else {
+#pragma unroll
+        for (int w = 0; w < KvTile<D, BITS>::VW; ++w) {
+          held_word<T, BITS>(tile.v[e][w], scale_of(tile.vs[e]), x + w * (BITS == 4 ? 4 : 2));
+          held_word<T, BITS>(tile.v[e + 1][w], scale_of(tile.vs[e + 1]), y + w * (BITS == 4 ? 4 : 2));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NV / 2; ++j) {
+        vw[2 * j][e / 2] = __builtin_amdgcn_perm(y[j], x[j], 0x05040100u);
+        vw[2 * j + 1][e / 2] = __builtin_amdgcn_perm(y[j], x[j], 0x07060302u);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) o[j] = mfma_16x16x32<T>(make_uint4(vw[j][0], vw[j][1], vw[j][2], vw[j][3]), pf, o[j]);
+  }
+
+  // the wavefronts' results: lane (r, g) holds elements (4 g + i) D / 16 + j of query row r in o[j][i]
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (g == 0) { lds_ml[wave][r][0] = m; lds_ml[wave][r][1] = l; }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) lds_o[wave][r][(4 * g + i) * NV + j] = o[j][i];
+  __syncthreads();
+  for (int i = static_cast<int>(threadIdx.x); i < nrows * D; i += KV_WAVES * 64) {
+    const int rr = i / D, d = i % D;
+    float top = lds_ml[0][rr][0];
+#pragma unroll
+    for (int w = 1; w < KV_WAVES; ++w) top = fmaxf(top, lds_ml[w][rr][0]);
+    float sum = 0.f, val = 0.f;
+#pragma unroll
+    for (int w = 0; w < KV_WAVES; ++w) {
+      const float f = fast_exp2(lds_ml[w][rr][0] - top);
+      sum += f * lds_ml[w][rr][1];
+      val += f * lds_o[w][rr][d];
+    }
+    const int qrow = row0 + rr;
+    if (a.splits == 1) {
+      T* op = static_cast<T*>(a.out) + static_cast<int64_t>(qrow / a.group) * a.o_st + static_cast<int64_t>(b) * a.o_sb +
+              static_cast<int64_t>(kvh * a.group + qrow % a.group) * a.o_sh;
+      op[d] = elem<T>::from_float(sum == 0.f ? 0.f : val / sum);      // (a NaN stays one)
+    } else {
+      const int64_t at = (split * (static_cast<int64_t>(gridDim.z) * a.kv_heads) + bh) * a.rows + qrow;
+      a.part[at * D + d] = val;
+      if (d == 0) { a.part_ml[2 * at] = top; a.part_ml[2 * at + 1] = sum; }
+    }
+  }
+}
+
+// The splits of every query row added up: one block of D threads per row.
+template <typename T, int D>
+__global__ __launch_bounds__(D) void kv_attn_join_kernel(KvAttn a, int64_t rows_all) {
+  const int64_t at = blockIdx.x;
+  const int d = static_cast<int>(threadIdx.x);
+  float top = KV_NEG;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[2 * (s * rows_all + at)]);
+  float sum = 0.f, val = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float f = fast_exp2(a.part_ml[2 * (s * rows_all + at)] - top);
+    sum += f * a.part_ml[2 * (s * rows_all + at) + 1];
+    val += f * a.part[(s * rows_all + at) * D + d];
+  }
+  const int qrow = static_cast<int>(at % a.rows);
+  const int64_t bh = at / a.rows, b = bh / a.kv_heads, kvh = bh % a.kv_heads;
+  T* op = static_cast<T*>(a.out) + static_cast<int64_t>(qrow / a.group) * a.o_st + b * a.o_sb + (kvh * a.group + qrow % a.group) * a.o_sh;
+  op[d] = elem<T>::from_float(sum == 0.f ? 0.f : val / sum);
+}
+
+int check_format(const char* what, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t capacity, int bits, int dtype) {
+  NMTG_REQUIRE(batch >= 0 && kv_heads >= 1 && capacity >= 0, "%s: bad shape batch=%lld kv_heads=%lld capacity=%lld", what, (long long)batch,
+               (long long)kv_heads, (long long)capacity);
+  NMTG_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head dimension %lld (64 and 128 are built)", what, (long long)head_dim);
+  NMTG_REQUIRE(bits == 4 || bits == 8, "%s: %d bits per element (4 and 8 are built)", what, bits);
+  NMTG_REQUIRE(dtype == NMTG_F16 || dtype == NMTG_BF16, "%s: fp16 or bf16 tensors required", what);
+  NMTG_REQUIRE(batch <= 65535 && kv_heads <= 65535 && capacity < (1ll << 31), "%s: more than 65535 sequences or heads, or 2^31 positions", what);
+  return 0;
+}
+bool rows_view_ok(const void* p, int64_t st, int64_t sb, int64_t sh) {
+  return aligned16(p) && st % 8 == 0 && sb % 8 == 0 && sh % 8 == 0 && st >= 0 && sb >= 0 && sh >= 0;
+}
+
+#define KV_DISPATCH(head_dim, bits, dtype, GO)                                                        \
+  if (dtype == NMTG_F16) {                                                                            \
+    if (head_dim == 64) { if (bits == 4) GO(f16_t, 64, 4); else GO(f16_t, 64, 8); }                   \
+    else { if (bits == 4) GO(f16_t, 128, 4); else GO(f16_t, 128, 8); }                                \
+  } else {                                                                                            \
+    if (head_dim == 64) { if (bits == 4) GO(bf16_t, 64, 4); else GO(bf16_t, 64, 8); }                 \
+    else { if (bits == 4) GO(bf16_t, 128, 4); else GO(bf16_t, 128, 8); }                              \
+  }
+
+// How many blocks share a sequence's positions: enough that the call has four blocks for every compute unit, each with at
+// least two tiles for every wavefront.
+int attn_splits(int64_t tq, int64_t batch, int64_t heads, int64_t kv_heads, int64_t longest, int64_t window, int64_t sinks) {
+  const int64_t rows = tq * (heads / kv_heads), blocks = batch * kv_heads * ((rows + KV_ROWS - 1) / KV_ROWS);
+  const int64_t reach = window > 0 ? std::min(longest, window + tq + sinks) : longest;
+  const int64_t tiles = (reach + KV_TILE - 1) / KV_TILE;
+  int64_t splits = (4 * num_cus() + blocks - 1) / std::max<int64_t>(blocks, 1);
+  splits = std::min(splits, tiles / (2 * KV_WAVES));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, 256)));
+}
+
+}  // namespace
+}  // namespace nmtg
+
+using namespace nmtg;
+
+extern "C" int nmtg_kv_cache_write(const void* k, int64_t k_stride_t, int64_t k_stride_b, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                                   int64_t v_stride_b, int64_t v_stride_h, uint8_t* k_codes, uint8_t* k_scales, uint8_t* v_codes,
+                                   uint8_t* v_scales, const int32_t* starts, int64_t start, int64_t count, int64_t batch, int64_t kv_heads,
+                                   int64_t head_dim, int64_t capacity, int bits, int dtype, void* stream) {
+  if (int rc = check_format("kv_cache_write", batch, kv_heads, head_dim, capacity, bits, dtype)) return rc;
+  NMTG_REQUIRE(count >= 0 && count < (1ll << 31), "kv_cache_write: %lld rows", (long long)count);
+  NMTG_REQUIRE(starts != nullptr || (start >= 0 && start + count <= capacity), "kv_cache_write: rows %lld .. %lld of a cache of %lld positions",
+               (long long)start, (long long)(start + count), (long long)capacity);
+  if (batch == 0 || count == 0 || capacity == 0) return 0;
+  NMTG_REQUIRE(k && v && k_codes && k_scales && v_codes && v_scales, "kv_cache_write: null pointer argument");
+  NMTG_REQUIRE(rows_view_ok(k, k_stride_t, k_stride_b, k_stride_h) && rows_view_ok(v, v_stride_t, v_stride_b, v_stride_h),
+               "kv_cache_write: k and v must be 16-byte aligned [count, batch, kv_heads, head_dim] views with a contiguous head_dim and "
+               "strides that are multiples of 8 elements");
+  NMTG_REQUIRE(aligned16(k_codes) && aligned16(v_codes), "kv_cache_write: 16-byte aligned codes required");
+  KvRows a = {};
+  a.k = k; a.v = v; a.k_codes = k_codes; a.k_scales = k_scales; a.v_codes = v_codes; a.v_scales = v_scales;
+  a.starts = starts; a.start = start; a.count = count; a.capacity = capacity;
+  a.k_st = k_stride_t; a.k_sb = k_stride_b; a.k_sh = k_stride_h; a.v_st = v_stride_t; a.v_sb = v_stride_b; a.v_sh = v_stride_h;
+  a.batch = static_cast<int>(batch); a.kv_heads = static_cast<int>(kv_heads);
+  a.total = count * batch * kv_heads * (head_dim / 8);
+  const int64_t blocks = (a.total + 255) / 256;
+  NMTG_REQUIRE(blocks <= 0x7fffffff, "kv_cache_write: too many rows in one call");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  TraceScope trace("kv_cache_write", st);
+#define GO(T, D, B) hipLaunchKernelGGL((kv_write_kernel<T, D, B>), dim3(static_cast<unsigned>(blocks), 2), dim3(256), 0, st, a)
+  KV_DISPATCH(head_dim, bits, dtype, GO)
+#undef GO
+  NMTG_CHECK_LAUNCH("kv_cache_write");
+  return 0;
+}
+
+extern "C" int nmtg_kv_cache_read(const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes, const uint8_t* v_scales, void* k,
+                                  void* v, const int32_t* starts, int64_t start, int64_t count, int64_t batch, int64_t kv_heads,
+                                  int64_t head_dim, int64_t capacity, int bits, int dtype, void* stream) {
+  if (int rc = check_format("kv_cache_read", batch, kv_heads, head_dim, capacity, bits, dtype)) return rc;
+  NMTG_REQUIRE(count >= 0 && count < (1ll << 31), "kv_cache_read: %lld rows", (long long)count);
+  NMTG_REQUIRE(starts != nullptr || (start >= 0 && start + count <= capacity), "kv_cache_read: rows %lld .. %lld of a cache of %lld positions",
+               (long long)start, (long long)(start + count), (long long)capacity);
+  if (batch == 0 || count == 0) return 0;
+  NMTG_REQUIRE(k && v && (capacity == 0 || (k_codes && k_scales && v_codes && v_scales)), "kv_cache_read: null pointer argument");
+  NMTG_REQUIRE(aligned16(k) && aligned16(v) && aligned16(k_codes) && aligned16(v_codes), "kv_cache_read: 16-byte aligned codes and results required");
+  KvRows a = {};
+  a.k_out = k; a.v_out = v;
+  a.k_codes = const_cast<uint8_t*>(k_codes); a.k_scales = const_cast<uint8_t*>(k_scales);
+  a.v_codes = const_cast<uint8_t*>(v_codes); a.v_scales = const_cast<uint8_t*>(v_scales);
+  a.starts = starts; a.start = start; a.count = count; a.capacity = capacity;
+  a.batch = static_cast<int>(batch); a.kv_heads = static_cast<int>(kv_heads);
+  a.total = count * batch * kv_heads * (head_dim / 8);
+  const int64_t blocks = (a.total + 255) / 256;
+  NMTG_REQUIRE(blocks <= 0x7fffffff, "kv_cache_read: too many rows in one call");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  TraceScope trace("kv_cache_read", st);
+#define GO(T, D, B) hipLaunchKernelGGL((kv_read_kernel<T, D, B>), dim3(static_cast<unsigned>(blocks), 2), dim3(256), 0, st, a)
+  KV_DISPATCH(head_dim, bits, dtype, GO)
+#undef GO
+  NMTG_CHECK_LAUNCH("kv_cache_read");
+  return 0;
+}
+
+extern "C" int64_t nmtg_kv_cache_attn_workspace_bytes(int64_t tq, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t longest,
+                                                      int64_t window, int64_t sinks) {
+  if (tq <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0) return 0;
+  const int splits = attn_splits(tq, batch, heads, kv_heads, longest, window, sinks);
+  return splits == 1 ? 0 : splits * tq * batch * heads * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+}
+
+extern "C" int nmtg_kv_cache_attn(const void* q, int64_t q_stride_t, int64_t q_stride_b, int64_t q_stride_h, const uint8_t* k_codes,
+                                  const uint8_t* k_scales, const uint8_t* v_codes, const uint8_t* v_scales, const int32_t* lengths, void* out,
+                                  int64_t out_stride_t, int64_t out_stride_b, int64_t out_stride_h, int64_t tq, int64_t batch, int64_t heads,
+                                  int64_t kv_heads, int64_t head_dim, int64_t capacity, int64_t longest, int64_t window, int64_t sinks,
+                                  float scale, int bits, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "kv_cache_attn";
+  if (int rc = check_format(what, batch, kv_heads, head_dim, capacity, bits, dtype)) return rc;
+  NMTG_REQUIRE(tq >= 0 && heads >= kv_heads && heads % kv_heads == 0, "%s: %lld query heads do not share %lld key / value heads evenly", what,
+               (long long)heads, (long long)kv_heads);
+  NMTG_REQUIRE(longest >= 0 && longest <= capacity, "%s: longest sequence %lld in a cache of %lld positions", what, (long long)longest, (long long)capacity);
+  NMTG_REQUIRE(window >= 0 && sinks >= 0 && window < (1ll << 40) && sinks < (1ll << 40), "%s: window %lld, sinks %lld", what, (long long)window, (long long)sinks);
+  NMTG_REQUIRE(scale >= -1e6f && scale <= 1e6f, "%s: scale %g", what, (double)scale);
+  if (batch == 0 || tq == 0) return 0;
+  NMTG_REQUIRE(q && lengths && out && (capacity == 0 || (k_codes && k_scales && v_codes && v_scales)), "%s: null pointer argument", what);
+  NMTG_REQUIRE(rows_view_ok(q, q_stride_t, q_stride_b, q_stride_h), "%s: q must be a 16-byte aligned [tq, batch, heads, head_dim] view with a contiguous "
+               "head_dim and strides that are multiples of 8 elements", what);
+  NMTG_REQUIRE(aligned16(k_codes) && aligned16(v_codes), "%s: 16-byte aligned codes required", what);
+  const int64_t group = heads / kv_heads, rows = tq * group, row_blocks = (rows + KV_ROWS - 1) / KV_ROWS;
+  NMTG_REQUIRE(rows < (1 << 24) && row_blocks * kv_heads <= 65535, "%s: too many query rows in one call", what);
+  KvAttn a = {};
+  a.q = q; a.k_codes = k_codes; a.k_scales = k_scales; a.v_codes = v_codes; a.v_scales = v_scales; a.lengths = lengths; a.out = out;
+  a.q_st = q_stride_t; a.q_sb = q_stride_b; a.q_sh = q_stride_h; a.o_st = out_stride_t; a.o_sb = out_stride_b; a.o_sh = out_stride_h;
+  a.capacity = capacity;
+  a.tq = static_cast<int>(tq); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads); a.group = static_cast<int>(group);
+  a.rows = static_cast<int>(rows); a.window = window; a.sinks = window > 0 ? sinks : 0; a.scale_log2 = scale * KV_LOG2E;
+  a.splits = attn_splits(tq, batch, heads, kv_heads, longest, window, sinks);
+  const int64_t rows_all = batch * kv_heads * rows;
+  if (a.splits > 1) {
+    const int64_t need = a.splits * rows_all * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+    NMTG_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= need,
+                 "%s: a 16-byte aligned workspace of %lld bytes required (nmtg_kv_cache_attn_workspace_bytes)", what, (long long)need);
+    NMTG_REQUIRE(rows_all <= 0x7fffffff, "%s: too many query rows in one call", what);
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = a.part + a.splits * rows_all * head_dim;
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(a.splits), static_cast<unsigned>(kv_heads * row_blocks), static_cast<unsigned>(batch));
+  {
+    TraceScope trace("kv_cache_attn", st);
+#define GO(T, D, B) hipLaunchKernelGGL((kv_attn_kernel<T, D, B>), grid, dim3(KV_WAVES * 64), 0, st, a)
+    KV_DISPATCH(head_dim, bits, dtype, GO)
+#undef GO
+  }
+  if (a.splits > 1) {
+    TraceScope trace("kv_cache_attn_join", st);
+    const dim3 rows_grid(static_cast<unsigned>(rows_all));
+    if (dtype == NMTG_F16) {
+      if (head_dim == 64) hipLaunchKernelGGL((kv_attn_join_kernel<f16_t, 64>), rows_grid, dim3(64), 0, st, a, rows_all);
+      else hipLaunchKernelGGL((kv_attn_join_kernel<f16_t, 128>), rows_grid, dim3(128), 0, st, a, rows_all);
+    } else {
+      if (head_dim == 64) hipLaunchKernelGGL((kv_attn_join_kernel<bf16_t, 64>), rows_grid, dim3(64), 0, st, a, rows_all);
+      else hipLaunchKernelGGL((kv_attn_join_kernel<bf16_t, 128>), rows_grid, dim3(128), 0, st, a, rows_all);
+    }
+  }
+  NMTG_CHECK_LAUNCH(what);
+  return 0;
+}

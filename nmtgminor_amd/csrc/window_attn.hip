@@ -1,0 +1,609 @@
+// Attention with a sliding window and a few first tokens that stay visible (sinks), forward and backward: query i of a
+// sequence sees key j where j <= i and (j > i - window or j < sinks). Work and memory grow with len * (window + sinks); there
+// is no mask tensor. Query heads may share a key / value head (heads = group * kv_heads), sequences may end early (lengths):
+// positions behind the end see nothing and are seen by nobody, their outputs and gradients are zeros.
+//
+//   forward     O_i = sum_j P_ij V_j,  P_ij = exp(s_ij - lse_i),  s_ij = scale Q_i . K_j
+//   backward    D_i = dO_i . O_i,  dS = P (dP - D),  dP_ij = dO_i . V_j
+//               dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO   (dK, dV summed over the heads of a group)
+//
+// The tiling is that of the other tiled attention kernels (flash_tile.hip.h): scores as S^T = K Q^T on 32 x 32 x 16 products,
+// one query per lane pair and 32 keys of a tile of 64 in a lane's registers, so that the softmax's maximum and sum are scalars
+// of a lane; probabilities go from accumulators into operands with two lane exchanges per 16 keys. A block visits the tiles
+// that hold sinks, then the tiles from its first query's window to its last query. What is different here:
+//   - Tiles go from memory straight into LDS (no registers in between), one tile ahead.
+//   - A tile lies in LDS once and is read both by rows and transposed: chunk c (16 bytes) of row r at position
+//     c ^ (2 (r & 3) | (r >> 2 & 1)). Eight neighbouring rows put one chunk into eight different bank groups (reads by rows),
+//     four neighbouring rows put a pair of chunks into four (transposed reads).
+//   - A wavefront that sees nothing of a tile skips it; masks are computed only where a tile crosses an edge.
+// No atomics and nothing added up across blocks: results do not depend on scheduling.
+#include "flash_tile.hip.h"
+#include <algorithm>
+
+namespace nmtg {
+namespace {
+
+constexpr int WA_WAVES = 4;
+
+struct WaView { const void* p; int64_t st, sb, sh; };   // [len, batch, heads, head_dim], head_dim contiguous
+
+struct WaArgs {
+  WaView q, k, v, o, d_o, dq, dk, dv;
+  float *lse, *delta;        // [batch, heads, len]
+  const int32_t* lengths;    // [batch] or null: every sequence fills `len`
+  int len, heads, kv_heads, group;
+  int64_t window, sinks;
+  float scale, scale_log2;
+};
+
+template <typename T>
+__device__ __forceinline__ const T* at_head(const WaView& x, int b, int h) {
+  return static_cast<const T*>(x.p) + static_cast<int64_t>(b) * x.sb + static_cast<int64_t>(h) * x.sh;
+}
+template <typename T>
+__device__ __forceinline__ T* out_head(const WaView& x, int b, int h) { return const_cast<T*>(at_head<T>(x, b, h)); }
+
+__device__ __forceinline__ int seq_len(const WaArgs& a, int b) {
+  return a.lengths != nullptr ? min(max(a.lengths[b], 0), a.len) : a.len;
+}
+
+// ---- the LDS image ----
+template <int D>
+__device__ __forceinline__ uint32_t img_at(int r, int c) {
+  return static_cast<uint32_t>(r * (2 * D) + ((c ^ (2 * (r & 3) | ((r >> 2) & 1))) * 16));
+}
+// A operand: rows 32 i + (lane & 31), columns 16 s + 8 (lane >> 5) .. + 7
+template <int D>
+__device__ __forceinline__ uint4 img_rows(const uint8_t* img, int i, int s, int lane) {
+  return *reinterpret_cast<const uint4*>(img + img_at<D>(32 * i + (lane & 31), 2 * s + (lane >> 5)));
+}
+// A operand of the transposed tile: columns 32 i + (lane & 31), rows 16 kk + 8 (lane >> 5) .. + 7
+template <int D>
+__device__ __forceinline__ uint4 img_columns(const uint8_t* img, int i, int kk, int lane) {
+  const int r = 16 * kk + 8 * (lane >> 5) + ((lane >> 2) & 3);
+  const int c = 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+  const uint8_t* p = img + (lane & 1) * 8;
+  const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p + img_at<D>(r, c)));
+  const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p + img_at<D>(r + 4, c)));
+  union { s16x4_t s[2]; uint4 u; } cv;
+  cv.s[0] = lo;
+  cv.s[1] = hi;
+  return cv.u;
+}
+
+// Transfers of one tile of 64 rows into an image, shared out over the block's wavefronts: lane l of transfer n fills chunk
+// 64 n + l. Rows behind `last` are read as row `last` (in bounds, finite where the sequence is; they are masked by the caller).
+template <typename T, int D>
+struct TileLoader {
+  static constexpr int CH = D / 8, N = FA_TILE * CH / 64 / WA_WAVES;
+  uint32_t voff[N];
+  int row[N], wave;
+  __device__ __forceinline__ TileLoader(int64_t stride_t, int wave_, int lane) : wave(wave_) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int id = 64 * (wave * N + n) + lane, r = id / CH, c = (id % CH) ^ (2 * (r & 3) | ((r >> 2) & 1));
+      row[n] = r;
+      voff[n] = static_cast<uint32_t>(r * stride_t * 2 + c * 16);
+    }
+  }
+  __device__ __forceinline__ void start(const T* head, int64_t stride_t, int first, int last, uint32_t img) const {
+    const T* base = head + static_cast<int64_t>(first) * stride_t;
+    const bool whole = first + FA_TILE - 1 <= last;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      uint32_t off = voff[n];
+      if (!whole) off -= static_cast<uint32_t>(max(first + row[n] - last, 0) * stride_t * 2);
+      dma16(off, base, img + static_cast<uint32_t>((wave * N + n) * 1024));
+    }
+  }
+};
+
+// the tiles of a block whose queries are first .. last: those of the sinks, then those from the first query's window on
+struct TileList {
+  int sinks, lo, count;
+  __device__ __forceinline__ TileList(const WaArgs& a, int first, int end) {
+    const int64_t from = static_cast<int64_t>(first) - a.window + 1;
+    const int tiles = (end + FA_TILE - 1) / FA_TILE;
+    lo = min(from > 0 ? static_cast<int>(from / FA_TILE) : 0, tiles);
+    sinks = min(static_cast<int>(((a.sinks < end ? a.sinks : end) + FA_TILE - 1) / FA_TILE), lo);
+    count = sinks + tiles - lo;
+  }
+  __device__ __forceinline__ int operator[](int i) const { return i < sinks ? i : i - sinks + lo; }
+};
+
+// ------------------------------------------------------------------------------------------------------------- forward
+template <typename T, int D, int NQ>
+__global__ __launch_bounds__(64 * WA_WAVES, 1) void window_fwd_kernel(WaArgs a) {
+  extern __shared__ __align__(16) uint8_t lds_raw[];
+  constexpr int IMG = FA_TILE * D * 2, ROWS = 32 * NQ * WA_WAVES;
+  const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y), q0 = static_cast<int>(blockIdx.x) * ROWS;
+  const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
+  const int n = seq_len(a, b), bh = b * a.heads + h;
+  T* ob = out_head<T>(a.o, b, h);
+  float* lse = a.lse + static_cast<int64_t>(bh) * a.len;
+  const int end = min(q0 + ROWS, n), qw = q0 + 32 * NQ * wave;
+  const T *kb = at_head<T>(a.k, b, h / a.group), *vb = at_head<T>(a.v, b, h / a.group);
+
+  uint4 qf[NQ][D / 16];
+  int qrow[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    qrow[x] = qw + 32 * x + (lane & 31);
+    load_resident<T, D>(qf[x], at_head<T>(a.q, b, h), a.q.st, qrow[x], n, lane);
+  }
+  acc16_t o[NQ][D / 32];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    m[x] = FA_NEG;
+    l[x] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[x][i][r] = 0.f;
+  }
+  const TileList tiles(a, q0, end > q0 ? end : 0);
+  const int count = end > q0 ? tiles.count : 0;
+  const TileLoader<T, D> ldk(a.k.st, wave, lane), ldv(a.v.st, wave, lane);
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw));
+  if (count > 0) {
+    ldk.start(kb, a.k.st, tiles[0] * FA_TILE, n - 1, lds0);
+    ldv.start(vb, a.v.st, tiles[0] * FA_TILE, n - 1, lds0 + IMG);
+  }
+  const int64_t first = qw, last = qw + 32 * NQ - 1;            // the wavefront's queries
+  for (int i = 0; i < count; ++i) {
+    const int t = tiles[i], k0 = t * FA_TILE;
+    wait_vmcnt<0>();
+    ring_barrier();
+    if (i + 1 < count) {
+      const uint32_t to = lds0 + ((i + 1) & 1) * 2 * IMG;
+      ldk.start(kb, a.k.st, tiles[i + 1] * FA_TILE, n - 1, to);
+      ldv.start(vb, a.v.st, tiles[i + 1] * FA_TILE, n - 1, to + IMG);
+    }
+    const uint8_t* kimg = lds_raw + (i & 1) * 2 * IMG;
+    const uint8_t* vimg = kimg + IMG;
+    // nothing of the tile is visible to the wavefront
+    if (k0 > last || first >= n || (k0 + FA_TILE - 1 <= first - a.window && k0 >= a.sinks)) continue;
+    acc16_t s[NQ][2];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x)
+#pragma unroll
+      for (int nn = 0; nn < 2; ++nn)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[x][nn][r] = 0.f;
+#pragma unroll
+    for (int ss = 0; ss < D / 16; ++ss)
+#pragma unroll
+      for (int nn = 0; nn < 2; ++nn) {
+        const uint4 kf = img_rows<D>(kimg, nn, ss, lane);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) mfma<T>::run(kf, qf[x][ss], s[x][nn]);
+      }
+    const bool edge = k0 + FA_TILE - 1 > first || last >= n || (k0 <= last - a.window && k0 + FA_TILE > a.sinks);
+    uint4 pf[NQ][FA_TILE / 16];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      uint32_t dead = 0;                                        // bit 16 nn + r: the key of that register is not visible
+      if (edge) {
+        const int64_t from = qrow[x] - a.window;
+#pragma unroll
+        for (int nn = 0; nn < 2; ++nn)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = k0 + 32 * nn + 8 * (r / 4) + 4 * half + r % 4;
+            if (key > qrow[x] || qrow[x] >= n || (key <= from && key >= a.sinks)) { dead |= 1u << (16 * nn + r); s[x][nn][r] = 0.f; }
+          }
+      }
+      float top = FA_NEG;
+#pragma unroll
+      for (int nn = 0; nn < 2; ++nn)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[x][nn][r] *= a.scale_log2;
+          if (edge && ((dead >> (16 * nn + r)) & 1u) != 0) s[x][nn][r] = FA_NEG;
+          top = fmaxf(top, s[x][nn][r]);
+        }
+      const float mx = pair_max(top);
+      // The reference point follows the maximum lazily: it moves when a row's maximum has grown by more than 2^8
+      const bool grow = mx > m[x] + FA_LAZY;
+      if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+        const float m_new = grow ? mx : m[x];
+        const float alpha = fast_exp2(m[x] - m_new);
+        m[x] = m_new;
+        l[x] *= alpha;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[x][j][r] *= alpha;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int nn = 0; nn < 2; ++nn)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float p = fast_exp2(s[x][nn][r] - m[x]);
+          if (edge && ((dead >> (16 * nn + r)) & 1u) != 0) p = 0.f;   // m may still be the initial one
+          s[x][nn][r] = p;
+          sum += p;
+        }
+      l[x] += sum;
+#pragma unroll
+      for (int kk = 0; kk < FA_TILE / 16; ++kk) {
+        float pv[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pv[e] = s[x][kk / 2][8 * (kk % 2) + e];
+        pf[x][kk] = acc_to_operand<T>(pv);
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < FA_TILE / 16; ++kk)
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const uint4 vf = img_columns<D>(vimg, j, kk, lane);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) mfma<T>::run(vf, pf[x][kk], o[x][j]);
+      }
+  }
+  __syncthreads();                                              // every wavefront is done with the images
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const float sum = pair_sum(l[x]);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (half == 0 && qrow[x] < a.len) lse[qrow[x]] = sum > 0.f ? (m[x] + log2f(sum)) * (1.0f / FA_LOG2E) : sum == 0.f ? -INFINITY : sum;
+    store_rows_out<T, D>(o[x], inv, lds_raw + wave * (32 * D * 2), ob, a.o.st, qw + 32 * x, a.len, lane);
+    if (x + 1 < NQ) __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------ backward: dQ, and D = rowsum(dO O)
+template <typename T, int D, int NQ>
+__global__ __launch_bounds__(64 * WA_WAVES, 1) void window_bwd_dq_kernel(WaArgs a) {
+  extern __shared__ __align__(16) uint8_t lds_raw[];
+  constexpr int IMG = FA_TILE * D * 2, ROWS = 32 * NQ * WA_WAVES;
+  const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y), q0 = static_cast<int>(blockIdx.x) * ROWS;
+  const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
+  const int n = seq_len(a, b), bh = b * a.heads + h;
+  const int end = min(q0 + ROWS, n), qw = q0 + 32 * NQ * wave;
+  const T *kb = at_head<T>(a.k, b, h / a.group), *vb = at_head<T>(a.v, b, h / a.group);
+
+  uint4 qf[NQ][D / 16], gf[NQ][D / 16];
+  int qrow[NQ];
+  float delta[NQ], lse2[NQ];
+  acc16_t dq[NQ][D / 32];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    qrow[x] = qw + 32 * x + (lane & 31);
+    load_resident<T, D>(qf[x], at_head<T>(a.q, b, h), a.q.st, qrow[x], n, lane);
+    load_resident<T, D>(gf[x], at_head<T>(a.d_o, b, h), a.d_o.st, qrow[x], n, lane);
+    uint4 of[D / 16];
+    load_resident<T, D>(of, at_head<T>(a.o, b, h), a.o.st, qrow[x], n, lane);
+    float d = 0.f;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      const T* u = reinterpret_cast<const T*>(&of[s]);
+      const T* w = reinterpret_cast<const T*>(&gf[x][s]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d += elem<T>::to_float(u[e]) * elem<T>::to_float(w[e]);
+    }
+    delta[x] = pair_sum(d);
+    lse2[x] = -FA_NEG;                                          // rows behind the end: probability 0
+    if (qrow[x] < n) {
+      const int64_t at = static_cast<int64_t>(bh) * a.len + qrow[x];
+      const float v = a.lse[at];
+      lse2[x] = v == -INFINITY ? -FA_NEG : v * FA_LOG2E;
+      if (half == 0) a.delta[at] = delta[x];
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[x][i][r] = 0.f;
+  }
+  const TileList tiles(a, q0, end > q0 ? end : 0);
+  const int count = end > q0 ? tiles.count : 0;
+  const TileLoader<T, D> ldk(a.k.st, wave, lane), ldv(a.v.st, wave, lane);
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw));
+  if (count > 0) {
+    ldk.start(kb, a.k.st, tiles[0] * FA_TILE, n - 1, lds0);
+    ldv.start(vb, a.v.st, tiles[0] * FA_TILE, n - 1, lds0 + IMG);
+  }
+  const int64_t first = qw, last = qw + 32 * NQ - 1;
+  for (int i = 0; i < count; ++i) {
+    const int t = tiles[i], k0 = t * FA_TILE;
+    wait_vmcnt<0>();
+    ring_barrier();
+    if (i + 1 < count) {
+      const uint32_t to = lds0 + ((i + 1) & 1) * 2 * IMG;
+      ldk.start(kb, a.k.st, tiles[i + 1] * FA_TILE, n - 1, to);
+      ldv.start(vb, a.v.st, tiles[i + 1] * FA_TILE, n - 1, to + IMG);
+    }
+    const uint8_t* kimg = lds_raw + (i & 1) * 2 * IMG;
+    const uint8_t* vimg = kimg + IMG;
+    if (k0 > last || first >= n || (k0 + FA_TILE - 1 <= first - a.window && k0 >= a.sinks)) continue;
+    const bool edge = k0 + FA_TILE - 1 > first || last >= n || (k0 <= last - a.window && k0 + FA_TILE > a.sinks);
+    uint4 df[NQ][FA_TILE / 16];
+#pragma unroll
+    for (int nn = 0; nn < 2; ++nn) {
+      acc16_t s[NQ], dp[NQ];
+#pragma unroll
+      for (int x = 0; x < NQ; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { s[x][r] = 0.f; dp[x][r] = 0.f; }
+#pragma unroll
+      for (int ss = 0; ss < D / 16; ++ss) {
+        const uint4 kf = img_rows<D>(kimg, nn, ss, lane), vf = img_rows<D>(vimg, nn, ss, lane);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+          mfma<T>::run(kf, qf[x][ss], s[x]);
+          mfma<T>::run(vf, gf[x][ss], dp[x]);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) {
+        const int64_t from = qrow[x] - a.window;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float p = fast_exp2(__builtin_fmaf(s[x][r], a.scale_log2, -lse2[x]));
+          if (edge) {
+            const int key = k0 + 32 * nn + 8 * (r / 4) + 4 * half + r % 4;
+            if (key > qrow[x] || qrow[x] >= n || (key <= from && key >= a.sinks)) p = 0.f;
+          }
+          s[x][r] = p * (dp[x][r] - delta[x]);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          float dsv[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dsv[e] = s[x][8 * kk + e];
+          df[x][2 * nn + kk] = acc_to_operand<T>(dsv);
+        }
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < FA_TILE / 16; ++kk)
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const uint4 kf = img_columns<D>(kimg, j, kk, lane);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) mfma<T>::run(kf, df[x][kk], dq[x][j]);
+      }
+  }
+  __syncthreads();
+  T* dqb = out_head<T>(a.dq, b, h);
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    store_rows_out<T, D>(dq[x], a.scale, lds_raw + wave * (32 * D * 2), dqb, a.dq.st, qw + 32 * x, a.len, lane);
+    if (x + 1 < NQ) __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------- backward: dK and dV
+// One key per lane pair: a block holds 128 keys of a key / value head, the queries of every head of its group come in tiles
+// of 64.
+template <typename T, int D>
+__global__ __launch_bounds__(64 * WA_WAVES, 1) void window_bwd_dkv_kernel(WaArgs a) {
+  extern __shared__ __align__(16) uint8_t lds_raw[];
+  constexpr int IMG = FA_TILE * D * 2, ROWS = 32 * WA_WAVES, BUF = 2 * IMG + 2 * FA_TILE * 4;   // Q, dO, lse2[64], D[64]
+  const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y), k0 = static_cast<int>(blockIdx.x) * ROWS;
+  const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
+  const int n = seq_len(a, b), kw = k0 + 32 * wave, krow = kw + (lane & 31);
+  uint4 kf[D / 16], vf[D / 16];
+  load_resident<T, D>(kf, at_head<T>(a.k, b, h), a.k.st, krow, n, lane);
+  load_resident<T, D>(vf, at_head<T>(a.v, b, h), a.v.st, krow, n, lane);
+  acc16_t dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) { dk[i][r] = 0.f; dv[i][r] = 0.f; }
+
+  // the query tiles that see some key of the block: to the end of the last key's window, or of the sequence where it holds sinks
+  const int64_t reach = k0 < a.sinks ? n : static_cast<int64_t>(k0) + ROWS - 1 + a.window;
+  const int t0 = k0 / FA_TILE, t1 = static_cast<int>(((reach < n ? reach : n) + FA_TILE - 1) / FA_TILE);
+  const int per = k0 < n ? t1 - t0 : 0, count = per * a.group;
+  const TileLoader<T, D> ldq(a.q.st, wave, lane), ldg(a.d_o.st, wave, lane);
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw));
+  float st_raw = 0.f;
+  const int tid = static_cast<int>(threadIdx.x);
+  // threads 0..63: the log-sum-exp of the tile's queries (-inf behind the end), 64..127: their D; asked for ahead of the tile's
+  // transfers and looked at behind them, at the end of the iteration
+  auto start = [&](int i, uint32_t to) {
+    const int hq = h * a.group + i / per, q0 = (t0 + i % per) * FA_TILE;
+    if (tid < 2 * FA_TILE) {
+      const int qi = q0 + (tid & (FA_TILE - 1));
+      const float* src = (tid < FA_TILE ? a.lse : a.delta) + (static_cast<int64_t>(b) * a.heads + hq) * a.len;
+      st_raw = tid < FA_TILE ? -INFINITY : 0.f;
+      if (qi < n) st_raw = src[qi];
+    }
+    ldq.start(at_head<T>(a.q, b, hq), a.q.st, q0, n - 1, to);
+    ldg.start(at_head<T>(a.d_o, b, hq), a.d_o.st, q0, n - 1, to + IMG);
+  };
+  auto store_stats = [&](uint8_t* buf) {
+    if (tid < 2 * FA_TILE) reinterpret_cast<float*>(buf + 2 * IMG)[tid] = tid < FA_TILE ? (st_raw == -INFINITY ? -FA_NEG : st_raw * FA_LOG2E) : st_raw;
+  };
+  if (count > 0) {
+    start(0, lds0);
+    store_stats(lds_raw);
+  }
+  for (int i = 0; i < count; ++i) {
+    const int q0 = (t0 + i % per) * FA_TILE;
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (i + 1 < count) start(i + 1, lds0 + ((i + 1) & 1) * BUF);
+    const uint8_t* qimg = lds_raw + (i & 1) * BUF;
+    const uint8_t* gimg = qimg + IMG;
+    const float* stats = reinterpret_cast<const float*>(qimg + 2 * IMG);
+    const int64_t klast = kw + 31;
+    const bool nothing = q0 + FA_TILE - 1 < kw || kw >= n || (q0 - a.window >= klast && kw >= a.sinks);
+    if (!nothing) {
+      const bool edge = q0 < klast || klast >= n || (q0 + FA_TILE - 1 - a.window >= kw && klast >= a.sinks);
+      uint4 pf[FA_TILE / 16], df[FA_TILE / 16];
+#pragma unroll
+      for (int nn = 0; nn < 2; ++nn) {
+        acc16_t s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+        for (int ss = 0; ss < D / 16; ++ss) {
+          mfma<T>::run(img_rows<D>(qimg, nn, ss, lane), kf[ss], s);
+          mfma<T>::run(img_rows<D>(gimg, nn, ss, lane), vf[ss], dp);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int ql = 32 * nn + 8 * g + 4 * half;            // first of four consecutive queries, within the tile
+          const float4 l4 = *reinterpret_cast<const float4*>(stats + ql);
+          const float4 d4 = *reinterpret_cast<const float4*>(stats + FA_TILE + ql);
+          const float lse2[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g + e;
+            float p = fast_exp2(__builtin_fmaf(s[r], a.scale_log2, -lse2[e]));
+            if (edge) {
+              const int64_t qi = q0 + ql + e;
+              if (krow > qi || krow >= n || (krow <= qi - a.window && krow >= a.sinks)) p = 0.f;
+            }
+            s[r] = p * (dp[r] - dl[e]);
+            dp[r] = p;
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          float pv[8], dsv[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) { pv[e] = dp[8 * kk + e]; dsv[e] = s[8 * kk + e]; }
+          pf[2 * nn + kk] = acc_to_operand<T>(pv);
+          df[2 * nn + kk] = acc_to_operand<T>(dsv);
+        }
+      }
+#pragma unroll
+      for (int kk = 0; kk < FA_TILE / 16; ++kk)
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          mfma<T>::run(img_columns<D>(gimg, j, kk, lane), pf[kk], dv[j]);
+          mfma<T>::run(img_columns<D>(qimg, j, kk, lane), df[kk], dk[j]);
+        }
+    }
+    if (i + 1 < count) store_stats(lds_raw + ((i + 1) & 1) * BUF);
+  }
+  __syncthreads();
+  uint8_t* patch = lds_raw + wave * (32 * D * 2);
+  store_rows_out<T, D>(dk, a.scale, patch, out_head<T>(a.dk, b, h), a.dk.st, kw, a.len, lane);
+  __syncthreads();
+  store_rows_out<T, D>(dv, 1.f, patch, out_head<T>(a.dv, b, h), a.dv.st, kw, a.len, lane);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+int check_call(const char* what, int64_t len, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window, int64_t sinks,
+               float scale, int dtype) {
+  NMTG_REQUIRE(len >= 0 && batch >= 0 && heads >= 1 && kv_heads >= 1, "%s: bad shape len=%lld batch=%lld heads=%lld kv_heads=%lld", what,
+               (long long)len, (long long)batch, (long long)heads, (long long)kv_heads);
+  NMTG_REQUIRE(heads % kv_heads == 0, "%s: %lld query heads do not share %lld key / value heads evenly", what, (long long)heads, (long long)kv_heads);
+  NMTG_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head dimension %lld (64 and 128 are built)", what, (long long)head_dim);
+  NMTG_REQUIRE(dtype == NMTG_F16 || dtype == NMTG_BF16, "%s: fp16 or bf16 tensors required (matrix-core kernel)", what);
+  NMTG_REQUIRE(window >= 1 && sinks >= 0 && window < (1ll << 40) && sinks < (1ll << 40), "%s: window %lld (at least 1), sinks %lld (at least 0)", what,
+               (long long)window, (long long)sinks);
+  NMTG_REQUIRE(scale >= -1e6f && scale <= 1e6f, "%s: scale %g", what, (double)scale);
+  NMTG_REQUIRE(heads <= 65535 && batch <= 65535 && len <= (1 << 24), "%s: more than 65535 heads or sequences, or 2^24 positions", what);
+  return 0;
+}
+// Views whose tile of 64 rows lies within 32-bit offsets of its first row
+int check_views(const char* what, WaView* views, const void* const* pointers, const int64_t* strides, int count) {
+  for (int i = 0; i < count; ++i) {
+    const int64_t* s = strides + 3 * i;
+    NMTG_REQUIRE(aligned16(pointers[i]) && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0 && s[0] >= 0 && s[1] >= 0 && s[2] >= 0 && s[0] < (1 << 24),
+                 "%s: every tensor must be a 16-byte aligned [len, batch, heads, head_dim] view with a contiguous head_dim and strides that are "
+                 "multiples of 8 elements (position stride below 2^24)", what);
+    views[i] = {pointers[i], s[0], s[1], s[2]};
+  }
+  return 0;
+}
+
+template <typename K>
+int launch_tiled(K kern, int lds, dim3 grid, const WaArgs& a, hipStream_t st, const char* what) {
+  if (lds > 64 * 1024) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return fail(NMTG_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS: %s", what, lds, hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL(kern, grid, dim3(64 * WA_WAVES), lds, st, a);
+  return 0;
+}
+template <int D> constexpr int fwd_lds() { return std::max(4 * FA_TILE * D * 2, WA_WAVES * 32 * D * 2); }
+template <int D> constexpr int dkv_lds() { return std::max(2 * (2 * FA_TILE * D * 2 + 2 * FA_TILE * 4), WA_WAVES * 32 * D * 2); }
+dim3 row_grid(const WaArgs& a, int rows, int64_t heads, int64_t batch) {
+  return dim3(static_cast<unsigned>((a.len + rows - 1) / rows), static_cast<unsigned>(heads), static_cast<unsigned>(batch));
+}
+
+template <typename T, int D>
+int fwd_launch(const WaArgs& a, int64_t batch, hipStream_t st) {
+  TraceScope trace("window_attn_fwd", st);
+  return launch_tiled(window_fwd_kernel<T, D, 1>, fwd_lds<D>(), row_grid(a, 32 * WA_WAVES, a.heads, batch), a, st, "window_attn_fwd");
+}
+template <typename T, int D>
+int bwd_launch(const WaArgs& a, int64_t batch, hipStream_t st) {
+  {
+    TraceScope trace("window_attn_bwd_dq", st);
+    if (int rc = launch_tiled(window_bwd_dq_kernel<T, D, 1>, fwd_lds<D>(), row_grid(a, 32 * WA_WAVES, a.heads, batch), a, st, "window_attn_bwd")) return rc;
+  }
+  TraceScope trace("window_attn_bwd_dkv", st);
+  return launch_tiled(window_bwd_dkv_kernel<T, D>, dkv_lds<D>(), row_grid(a, 32 * WA_WAVES, a.kv_heads, batch), a, st, "window_attn_bwd");
+}
+
+}  // namespace
+}  // namespace nmtg
+
+using namespace nmtg;
+
+extern "C" int nmtg_window_attn_fwd(const void* q, const void* k, const void* v, void* out, float* softmax_lse, const int32_t* lengths,
+                                    const int64_t* strides, int64_t len, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                    int64_t window, int64_t sinks, float softmax_scale, int dtype, void* stream) {
+  const char* what = "window_attn_fwd";
+  if (int rc = check_call(what, len, batch, heads, kv_heads, head_dim, window, sinks, softmax_scale, dtype)) return rc;
+  if (len == 0 || batch == 0) return 0;
+  NMTG_REQUIRE(q && k && v && out && softmax_lse && strides, "%s: null pointer argument", what);
+  WaView views[4];
+  const void* pointers[4] = {q, k, v, out};
+  if (int rc = check_views(what, views, pointers, strides, 4)) return rc;
+  WaArgs a = {};
+  a.q = views[0]; a.k = views[1]; a.v = views[2]; a.o = views[3];
+  a.lse = softmax_lse; a.lengths = lengths; a.len = static_cast<int>(len); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
+  a.group = static_cast<int>(heads / kv_heads); a.window = window; a.sinks = sinks; a.scale = softmax_scale; a.scale_log2 = softmax_scale * FA_LOG2E;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  int rc;
+  if (dtype == NMTG_F16) rc = head_dim == 64 ? fwd_launch<f16_t, 64>(a, batch, st) : fwd_launch<f16_t, 128>(a, batch, st);
+  else rc = head_dim == 64 ? fwd_launch<bf16_t, 64>(a, batch, st) : fwd_launch<bf16_t, 128>(a, batch, st);
+  if (rc) return rc;
+  NMTG_CHECK_LAUNCH(what);
+  return 0;
+}
+
+extern "C" int64_t nmtg_window_attn_bwd_workspace_bytes(int64_t len, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                                        int64_t window, int64_t sinks) {
+  if (len <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || window <= 0 || sinks < 0) return 0;
+  return batch * heads * len * static_cast<int64_t>(sizeof(float));
+}
+
+extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* softmax_lse,
+                                    void* dq, void* dk, void* dv, const int32_t* lengths, const int64_t* strides, int64_t len,
+                                    int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window, int64_t sinks,
+                                    float softmax_scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "window_attn_bwd";
+  if (int rc = check_call(what, len, batch, heads, kv_heads, head_dim, window, sinks, softmax_scale, dtype)) return rc;
+  if (len == 0 || batch == 0) return 0;
+  NMTG_REQUIRE(dout && q && k && v && out && softmax_lse && dq && dk && dv && strides, "%s: null pointer argument", what);
+  NMTG_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 &&
+                   workspace_bytes >= nmtg_window_attn_bwd_workspace_bytes(len, batch, heads, kv_heads, head_dim, window, sinks),
+               "%s: a 256-byte aligned workspace of nmtg_window_attn_bwd_workspace_bytes bytes required", what);
+  WaView views[8];
+  const void* pointers[8] = {dout, q, k, v, out, dq, dk, dv};
+  if (int rc = check_views(what, views, pointers, strides, 8)) return rc;
+  WaArgs a = {};
+  a.d_o = views[0]; a.q = views[1]; a.k = views[2]; a.v = views[3]; a.o = views[4]; a.dq = views[5]; a.dk = views[6]; a.dv = views[7];
+  a.lse = const_cast<float*>(softmax_lse); a.delta = static_cast<float*>(workspace); a.lengths = lengths; a.len = static_cast<int>(len);
+  a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads); a.group = static_cast<int>(heads / kv_heads);
+  a.window = window; a.sinks = sinks; a.scale = softmax_scale; a.scale_log2 = softmax_scale * FA_LOG2E;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  int rc;
+  if (dtype == NMTG_F16) rc = head_dim == 64 ? bwd_launch<f16_t, 64>(a, batch, st) : bwd_launch<f16_t, 128>(a, batch, st);
+  else rc = head_dim == 64 ? bwd_launch<bf16_t, 64>(a, batch, st) : bwd_launch<bf16_t, 128>(a, batch, st);
+  if (rc) return rc;
+  NMTG_CHECK_LAUNCH(what);
+  return 0;
+}
