@@ -34,6 +34,10 @@ struct WaArgs {
   int len, heads, kv_heads, group;
   int64_t window, sinks;
   float scale, scale_log2;
+  // backward, dK and dV in parts (see DkvPlan): fp32 [parts][batch, kv_heads, part_rows][2][head_dim] of the key blocks, then
+  // [chunks][batch, kv_heads, sink_rows][2][head_dim] of the blocks that hold sinks
+  float *part, *sink_part;
+  int key_blocks, sink_blocks, parts, chunks, part_rows, sink_rows;
 };
 
 template <typename T>
@@ -378,12 +382,33 @@ __global__ __launch_bounds__(64 * WA_WAVES, 1) void window_bwd_dq_kernel(WaArgs 
 
 // ------------------------------------------------------------------------------------------------- backward: dK and dV
 // One key per lane pair: a block holds 128 keys of a key / value head, the queries of every head of its group come in tiles
-// of 64.
+// of 64. The work is laid out so that blocks are alike (DkvPlan): the queries behind the windows of a block that holds sinks, up to
+// the sequence's end, are shared out over `chunks` more blocks, and where the key blocks would not fill the chip each is
+// shared out over `parts`. Such blocks leave fp32 sums that a last kernel adds in a fixed order.
+constexpr int WA_KEYS = 32 * WA_WAVES;
+
+// accumulators of the wavefront's 32 rows as fp32 rows of D elements, `pitch` floats apart
+template <int D>
+__device__ __forceinline__ void store_part(const acc16_t (&acc)[D / 32], float mul, float* base, int64_t pitch, int row0, int rows, int lane) {
+  const int half = lane >> 5, row = row0 + (lane & 31);
+  if (row >= rows) return;
+  float* p = base + static_cast<int64_t>(row) * pitch + 4 * half;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(p + 32 * i + 8 * g) = make_float4(acc[i][4 * g] * mul, acc[i][4 * g + 1] * mul, acc[i][4 * g + 2] * mul, acc[i][4 * g + 3] * mul);
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(64 * WA_WAVES, 1) void window_bwd_dkv_kernel(WaArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
-  constexpr int IMG = FA_TILE * D * 2, ROWS = 32 * WA_WAVES, BUF = 2 * IMG + 2 * FA_TILE * 4;   // Q, dO, lse2[64], D[64]
-  const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y), k0 = static_cast<int>(blockIdx.x) * ROWS;
+  constexpr int IMG = FA_TILE * D * 2, BUF = 2 * IMG + 2 * FA_TILE * 4;   // Q, dO, lse2[64], D[64]
+  const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y);
+  // blocks behind the key blocks' parts: chunk of the queries that see a block's keys as sinks only
+  const int x = static_cast<int>(blockIdx.x), own = a.key_blocks * a.parts;
+  const bool sink_chunk = x >= own;
+  const int k0 = (sink_chunk ? (x - own) / a.chunks : x / a.parts) * WA_KEYS, share = sink_chunk ? (x - own) % a.chunks : x % a.parts;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const int n = seq_len(a, b), kw = k0 + 32 * wave, krow = kw + (lane & 31);
   uint4 kf[D / 16], vf[D / 16];
@@ -395,10 +420,13 @@ __global__ __launch_bounds__(64 * WA_WAVES, 1) void window_bwd_dkv_kernel(WaArgs
 #pragma unroll
     for (int r = 0; r < 16; ++r) { dk[i][r] = 0.f; dv[i][r] = 0.f; }
 
-  // the query tiles that see some key of the block: to the end of the last key's window, or of the sequence where it holds sinks
-  const int64_t reach = k0 < a.sinks ? n : static_cast<int64_t>(k0) + ROWS - 1 + a.window;
-  const int t0 = k0 / FA_TILE, t1 = static_cast<int>(((reach < n ? reach : n) + FA_TILE - 1) / FA_TILE);
-  const int per = k0 < n ? t1 - t0 : 0, count = per * a.group;
+  // the query tiles up to the end of the last key's window, and those behind it
+  const int64_t reach = static_cast<int64_t>(k0) + WA_KEYS - 1 + a.window;
+  const int tw = static_cast<int>(((reach < n ? reach : n) + FA_TILE - 1) / FA_TILE), tn = (n + FA_TILE - 1) / FA_TILE;
+  const int t0 = sink_chunk ? tw : k0 / FA_TILE, t1 = sink_chunk ? tn : tw;
+  const int per = k0 < n ? t1 - t0 : 0, all = per * a.group, shares = sink_chunk ? a.chunks : a.parts;
+  // this block's share of the (head, tile) pairs
+  const int i0 = static_cast<int>(static_cast<int64_t>(all) * share / shares), i1 = static_cast<int>(static_cast<int64_t>(all) * (share + 1) / shares);
   const TileLoader<T, D> ldq(a.q.st, wave, lane), ldg(a.d_o.st, wave, lane);
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw));
   float st_raw = 0.f;
@@ -419,15 +447,15 @@ __global__ __launch_bounds__(64 * WA_WAVES, 1) void window_bwd_dkv_kernel(WaArgs
   auto store_stats = [&](uint8_t* buf) {
     if (tid < 2 * FA_TILE) reinterpret_cast<float*>(buf + 2 * IMG)[tid] = tid < FA_TILE ? (st_raw == -INFINITY ? -FA_NEG : st_raw * FA_LOG2E) : st_raw;
   };
-  if (count > 0) {
-    start(0, lds0);
-    store_stats(lds_raw);
+  if (i0 < i1) {
+    start(i0, lds0 + (i0 & 1) * BUF);
+    store_stats(lds_raw + (i0 & 1) * BUF);
   }
-  for (int i = 0; i < count; ++i) {
+  for (int i = i0; i < i1; ++i) {
     const int q0 = (t0 + i % per) * FA_TILE;
     wait_vmcnt<0>();
     __syncthreads();
-    if (i + 1 < count) start(i + 1, lds0 + ((i + 1) & 1) * BUF);
+    if (i + 1 < i1) start(i + 1, lds0 + ((i + 1) & 1) * BUF);
     const uint8_t* qimg = lds_raw + (i & 1) * BUF;
     const uint8_t* gimg = qimg + IMG;
     const float* stats = reinterpret_cast<const float*>(qimg + 2 * IMG);
@@ -481,13 +509,45 @@ __global__ __launch_bounds__(64 * WA_WAVES, 1) void window_bwd_dkv_kernel(WaArgs
           mfma<T>::run(img_columns<D>(qimg, j, kk, lane), df[kk], dk[j]);
         }
     }
-    if (i + 1 < count) store_stats(lds_raw + ((i + 1) & 1) * BUF);
+    if (i + 1 < i1) store_stats(lds_raw + ((i + 1) & 1) * BUF);
+  }
+  const bool in_parts = sink_chunk || a.parts > 1 || k0 < a.sink_blocks * WA_KEYS;
+  if (in_parts) {
+    const int rows = sink_chunk ? a.sink_rows : a.part_rows;
+    float* base = (sink_chunk ? a.sink_part : a.part) +
+                  ((static_cast<int64_t>(share) * gridDim.z + b) * a.kv_heads + h) * rows * (2 * D);
+    store_part<D>(dk, a.scale, base, 2 * D, kw, rows, lane);
+    store_part<D>(dv, 1.f, base + D, 2 * D, kw, rows, lane);
+    return;
   }
   __syncthreads();
   uint8_t* patch = lds_raw + wave * (32 * D * 2);
   store_rows_out<T, D>(dk, a.scale, patch, out_head<T>(a.dk, b, h), a.dk.st, kw, a.len, lane);
   __syncthreads();
   store_rows_out<T, D>(dv, 1.f, patch, out_head<T>(a.dv, b, h), a.dv.st, kw, a.len, lane);
+}
+
+// The sums of the parts, rounded: D / 4 threads per row of keys and as many for its row of values.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void window_dkv_join_kernel(WaArgs a, int64_t total) {
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (id >= total) return;
+  constexpr int CH = 2 * D / 4;
+  const int c = static_cast<int>(id % CH), h = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z);
+  const int row = static_cast<int>(id / CH);
+  const int64_t bh = static_cast<int64_t>(b) * a.kv_heads + h, bhs = static_cast<int64_t>(gridDim.z) * a.kv_heads;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](const float* base, int count, int pitch) {
+    for (int i = 0; i < count; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(base + ((i * bhs + bh) * pitch + row) * (2 * D) + 4 * c);
+      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    }
+  };
+  add(a.part, a.parts, a.part_rows);
+  if (row < a.sink_rows) add(a.sink_part, a.chunks, a.sink_rows);
+  T* out = c < CH / 2 ? out_head<T>(a.dk, b, h) + static_cast<int64_t>(row) * a.dk.st + 4 * c
+                      : out_head<T>(a.dv, b, h) + static_cast<int64_t>(row) * a.dv.st + 4 * (c - CH / 2);
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(sum.x, sum.y), pack2<T>(sum.z, sum.w));
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -536,14 +596,46 @@ int fwd_launch(const WaArgs& a, int64_t batch, hipStream_t st) {
   TraceScope trace("window_attn_fwd", st);
   return launch_tiled(window_fwd_kernel<T, D, 1>, fwd_lds<D>(), row_grid(a, 32 * WA_WAVES, a.heads, batch), a, st, "window_attn_fwd");
 }
+// How the blocks of dK and dV are laid out, and the floats they leave behind.
+struct DkvPlan {
+  int key_blocks, sink_blocks, parts, chunks, part_rows, sink_rows;
+  int64_t part_floats, sink_floats;
+  DkvPlan(int64_t len, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window, int64_t sinks) {
+    const int64_t blocks = (len + WA_KEYS - 1) / WA_KEYS, group = heads / kv_heads;
+    const int64_t tiles = (std::min(len, window + WA_KEYS) + FA_TILE - 1) / FA_TILE;      // query tiles of a key block, per head
+    key_blocks = static_cast<int>(blocks);
+    // some query stands behind the window of a block's first sinks
+    sink_blocks = len > WA_KEYS - 1 + window ? static_cast<int>(std::min(blocks, (std::min(sinks, len) + WA_KEYS - 1) / WA_KEYS)) : 0;
+    const int64_t behind = (len - std::min(len, window) + FA_TILE - 1) / FA_TILE;
+    chunks = sink_blocks > 0 ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((behind + tiles - 1) / tiles, 128))) : 0;
+    // two blocks for every compute unit, each with at least four tiles
+    parts = static_cast<int>(std::max<int64_t>(1, std::min({(2 * num_cus() + blocks * batch * kv_heads - 1) / (blocks * batch * kv_heads), tiles * group / 4, int64_t(16)})));
+    sink_rows = static_cast<int>(std::min<int64_t>(len, static_cast<int64_t>(sink_blocks) * WA_KEYS));
+    part_rows = parts > 1 ? static_cast<int>(len) : sink_rows;
+    part_floats = batch * kv_heads * parts * part_rows * 2 * head_dim;
+    sink_floats = batch * kv_heads * chunks * sink_rows * 2 * head_dim;
+  }
+};
+int64_t delta_floats(int64_t len, int64_t batch, int64_t heads) { return (batch * heads * len + 63) / 64 * 64; }
+
 template <typename T, int D>
 int bwd_launch(const WaArgs& a, int64_t batch, hipStream_t st) {
   {
     TraceScope trace("window_attn_bwd_dq", st);
     if (int rc = launch_tiled(window_bwd_dq_kernel<T, D, 1>, fwd_lds<D>(), row_grid(a, 32 * WA_WAVES, a.heads, batch), a, st, "window_attn_bwd")) return rc;
   }
-  TraceScope trace("window_attn_bwd_dkv", st);
-  return launch_tiled(window_bwd_dkv_kernel<T, D>, dkv_lds<D>(), row_grid(a, 32 * WA_WAVES, a.kv_heads, batch), a, st, "window_attn_bwd");
+  {
+    TraceScope trace("window_attn_bwd_dkv", st);
+    const dim3 grid(static_cast<unsigned>(a.key_blocks * a.parts + a.sink_blocks * a.chunks), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch));
+    if (int rc = launch_tiled(window_bwd_dkv_kernel<T, D>, dkv_lds<D>(), grid, a, st, "window_attn_bwd")) return rc;
+  }
+  if (a.part_rows > 0) {
+    TraceScope trace("window_attn_bwd_join", st);
+    const int64_t total = static_cast<int64_t>(a.part_rows) * (2 * D / 4);
+    hipLaunchKernelGGL((window_dkv_join_kernel<T, D>), dim3(static_cast<unsigned>((total + 255) / 256), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch)),
+                       dim3(256), 0, st, a, total);
+  }
+  return 0;
 }
 
 }  // namespace
@@ -577,7 +669,9 @@ extern "C" int nmtg_window_attn_fwd(const void* q, const void* k, const void* v,
 extern "C" int64_t nmtg_window_attn_bwd_workspace_bytes(int64_t len, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                                         int64_t window, int64_t sinks) {
   if (len <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || window <= 0 || sinks < 0) return 0;
-  return batch * heads * len * static_cast<int64_t>(sizeof(float));
+  if (heads % kv_heads != 0) return 0;
+  const DkvPlan plan(len, batch, heads, kv_heads, head_dim, window, sinks);
+  return (delta_floats(len, batch, heads) + plan.part_floats + plan.sink_floats) * static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* softmax_lse,
@@ -596,7 +690,13 @@ extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void*
   if (int rc = check_views(what, views, pointers, strides, 8)) return rc;
   WaArgs a = {};
   a.d_o = views[0]; a.q = views[1]; a.k = views[2]; a.v = views[3]; a.o = views[4]; a.dq = views[5]; a.dk = views[6]; a.dv = views[7];
-  a.lse = const_cast<float*>(softmax_lse); a.delta = static_cast<float*>(workspace); a.lengths = lengths; a.len = static_cast<int>(len);
+  a.lse = const_cast<float*>(softmax_lse); a.delta = static_cast<float*>(workspace);
+  const DkvPlan plan(len, batch, heads, kv_heads, head_dim, window, sinks);
+  a.part = a.delta + delta_floats(len, batch, heads);
+  a.sink_part = a.part + plan.part_floats;
+  a.key_blocks = plan.key_blocks; a.sink_blocks = plan.sink_blocks; a.parts = plan.parts; a.chunks = plan.chunks;
+  a.part_rows = plan.part_rows; a.sink_rows = plan.sink_rows;
+  a.lengths = lengths; a.len = static_cast<int>(len);
   a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads); a.group = static_cast<int>(heads / kv_heads);
   a.window = window; a.sinks = sinks; a.scale = softmax_scale; a.scale_log2 = softmax_scale * FA_LOG2E;
   hipStream_t st = static_cast<hipStream_t>(stream);
