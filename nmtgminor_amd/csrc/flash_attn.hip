@@ -69,18 +69,6 @@ struct FaArgs {
 // accumulator register holds in the two halves of a wavefront (j and j + 4) lie side by side as one 64-bit lane mask.
 __device__ __forceinline__ int bit_slot(int key) { return (key & ~7) | ((key & 3) << 1) | ((key >> 2) & 1); }
 
-// Touches the rows that stay in registers for a whole tile loop (the queries of the inference kernel), in front of the
-// loop and outside any branch. They are loaded under conditions, and without a use that the compiler sees on every path
-// it repeats the wait for them inside the loop, behind the loads of the next tile: every tile then waits for its own
-// prefetch. Not for the training kernels: behind a statement like this one (or a wait instruction of our own) the
-// compiler no longer reads wave-uniform values (tile classes, dropout bits) through the scalar cache but with vector
-// loads, each waited for on the spot.
-template <int N>
-__device__ __forceinline__ void registers_landed(const uint4 (&f)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" ::"v"(f[i].x), "v"(f[i].y), "v"(f[i].z), "v"(f[i].w));
-}
-
 // Where sequence b lies and how long it is. Packed calls read the cumulative lengths. Batch-strided calls (no cumulative
 // lengths) give every sequence max_q queries and max_k keys, b * *_sb elements into each tensor; a key padding mask cuts
 // the keys at the last live one, and masked keys below that are handled tile by tile (pad_tile()).

@@ -124,6 +124,18 @@ __device__ __forceinline__ void load_resident(uint4 (&f)[D / 16], const T* base,
   for (int s = 0; s < D / 16; ++s) f[s] = row < len ? *reinterpret_cast<const uint4*>(p + 16 * s) : make_uint4(0, 0, 0, 0);
 }
 
+// Touches the rows that stay in registers for a whole tile loop (the queries of the inference kernel), in front of the
+// loop and outside any branch. They are loaded under conditions, and without a use that the compiler sees on every path
+// it repeats the wait for them inside the loop, behind the loads of the next tile: every tile then waits for its own
+// prefetch. Not for the training kernels: behind a statement like this one (or a wait instruction of our own) the
+// compiler no longer reads wave-uniform values (tile classes, dropout bits) through the scalar cache but with vector
+// loads, each waited for on the spot.
+template <int N>
+__device__ __forceinline__ void registers_landed(const uint4 (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" ::"v"(f[i].x), "v"(f[i].y), "v"(f[i].z), "v"(f[i].w));
+}
+
 // Writes the wavefront's 32 rows x D accumulators (acc[i][r]: column 32 i + 8 (r / 4) + 4 half + r % 4 of row lane & 31)
 // through its own LDS patch as whole 16-byte chunks, rows past `len` skipped.
 template <typename T, int D>

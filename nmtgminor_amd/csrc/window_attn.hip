@@ -23,7 +23,7 @@
 namespace nmtg {
 namespace {
 
-constexpr int WA_WAVES = 4;
+constexpr int WA_WAVES = 4, WA_ROWS = 32 * WA_WAVES;   // of a block: 128 queries (forward, dQ) or keys (dK, dV), 32 per wavefront
 
 struct WaView { const void* p; int64_t st, sb, sh; };   // [len, batch, heads, head_dim], head_dim contiguous
 
@@ -75,11 +75,11 @@ __device__ __forceinline__ uint4 img_columns(const uint8_t* img, int i, int kk, 
   return cv.u;
 }
 
-// Transfers of one tile of 64 rows into an image, shared out over the block's wavefronts: lane l of transfer n fills chunk
+// Transfers of one tile of ROWS rows into an image, shared out over the block's wavefronts: lane l of transfer n fills chunk
 // 64 n + l. Rows behind `last` are read as row `last` (in bounds, finite where the sequence is; they are masked by the caller).
-template <typename T, int D>
+template <typename T, int D, int ROWS = FA_TILE>
 struct TileLoader {
-  static constexpr int CH = D / 8, N = FA_TILE * CH / 64 / WA_WAVES;
+  static constexpr int CH = D / 8, N = ROWS * CH / 64 / WA_WAVES;
   uint32_t voff[N];
   int row[N], wave;
   __device__ __forceinline__ TileLoader(int64_t stride_t, int wave_, int lane) : wave(wave_) {
@@ -92,7 +92,7 @@ struct TileLoader {
   }
   __device__ __forceinline__ void start(const T* head, int64_t stride_t, int first, int last, uint32_t img) const {
     const T* base = head + static_cast<int64_t>(first) * stride_t;
-    const bool whole = first + FA_TILE - 1 <= last;
+    const bool whole = first + ROWS - 1 <= last;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       uint32_t off = voff[n];
@@ -101,6 +101,12 @@ struct TileLoader {
     }
   }
 };
+
+// The transfers of the next tile have landed for the whole block, and its reads of the tile before are done.
+__device__ __forceinline__ void next_tile() {
+  wait_vmcnt<0>();
+  ring_barrier();
+}
 
 // the tiles of a block whose queries are first .. last: those of the sinks, then those from the first query's window on
 struct TileList {
@@ -115,277 +121,226 @@ struct TileList {
   __device__ __forceinline__ int operator[](int i) const { return i < sinks ? i : i - sinks + lo; }
 };
 
+// Whether queries first .. last of a sequence of n see nothing, or do not see everything, of the tile of keys from k0 on.
+__device__ __forceinline__ bool nothing_seen(const WaArgs& a, int n, int first, int last, int k0) {
+  return k0 > last || first >= n || (k0 + FA_TILE - 1 <= first - a.window && k0 >= a.sinks);
+}
+__device__ __forceinline__ bool some_hidden(const WaArgs& a, int n, int first, int last, int k0) {
+  return k0 + FA_TILE - 1 > first || last >= n || (k0 <= last - a.window && k0 + FA_TILE > a.sinks);
+}
+
+// Scores of one query against keys key0 + 8 (r / 4) + r % 4 (register r): those it does not see become `hidden`, the infinity
+// that the scale turns negative, whose probability is zero.
+__device__ __forceinline__ void hide_keys(acc16_t& s, const WaArgs& a, int n, int qrow, int key0, float hidden) {
+  const int64_t front = qrow - a.window;                        // keys up to here are in front of the window
+  const int from = static_cast<int>(front > -1 ? front : -1) - key0, to = (qrow < n ? qrow : -1) - key0;
+  const int sinks = static_cast<int>(a.sinks < n ? a.sinks : n) - key0;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int key = 8 * (r / 4) + r % 4;
+    s[r] = (key > to) | ((key <= from) & (key >= sinks)) ? hidden : s[r];   // (selects: short-circuit tests became branches per element)
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------- forward
-template <typename T, int D, int NQ>
-__global__ __launch_bounds__(64 * WA_WAVES, 1) void window_fwd_kernel(WaArgs a) {
+constexpr float WA_FLOOR = -5e29f;   // a running maximum before the first visible key: finite, and far above the -inf of hidden ones
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_kernel(WaArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
-  constexpr int IMG = FA_TILE * D * 2, ROWS = 32 * NQ * WA_WAVES;
-  const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y), q0 = static_cast<int>(blockIdx.x) * ROWS;
+  constexpr int IMG = FA_TILE * D * 2;
+  const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y), q0 = static_cast<int>(blockIdx.x) * WA_ROWS;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const int n = seq_len(a, b), bh = b * a.heads + h;
-  T* ob = out_head<T>(a.o, b, h);
-  float* lse = a.lse + static_cast<int64_t>(bh) * a.len;
-  const int end = min(q0 + ROWS, n), qw = q0 + 32 * NQ * wave;
+  const int end = min(q0 + WA_ROWS, n), qw = q0 + 32 * wave, qrow = qw + (lane & 31);
   const T *kb = at_head<T>(a.k, b, h / a.group), *vb = at_head<T>(a.v, b, h / a.group);
 
-  uint4 qf[NQ][D / 16];
-  int qrow[NQ];
+  uint4 qf[D / 16];
+  load_resident<T, D>(qf, at_head<T>(a.q, b, h), a.q.st, qrow, n, lane);
+  acc16_t o[D / 32];
+  float m = WA_FLOOR, l = 0.f;
 #pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    qrow[x] = qw + 32 * x + (lane & 31);
-    load_resident<T, D>(qf[x], at_head<T>(a.q, b, h), a.q.st, qrow[x], n, lane);
-  }
-  acc16_t o[NQ][D / 32];
-  float m[NQ], l[NQ];
+  for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    m[x] = FA_NEG;
-    l[x] = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[x][i][r] = 0.f;
-  }
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+  registers_landed(qf);
   const TileList tiles(a, q0, end > q0 ? end : 0);
   const int count = end > q0 ? tiles.count : 0;
   const TileLoader<T, D> ldk(a.k.st, wave, lane), ldv(a.v.st, wave, lane);
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw));
-  if (count > 0) {
-    ldk.start(kb, a.k.st, tiles[0] * FA_TILE, n - 1, lds0);
-    ldv.start(vb, a.v.st, tiles[0] * FA_TILE, n - 1, lds0 + IMG);
-  }
-  const int64_t first = qw, last = qw + 32 * NQ - 1;            // the wavefront's queries
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw)));
+  auto start = [&](int i) {
+    const int row = tiles[i] * FA_TILE;
+    const uint32_t to = lds0 + static_cast<uint32_t>(i & 1) * 2 * IMG;
+    ldk.start(kb, a.k.st, row, n - 1, to);
+    ldv.start(vb, a.v.st, row, n - 1, to + IMG);
+  };
+  if (count > 0) start(0);
+  const int first = qw, last = qw + 31;                         // the wavefront's queries
+  const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
+  constexpr uint32_t ONES = elem<T>::dtype == NMTG_BF16 ? 0x3f803f80u : 0x3c003c00u;
   for (int i = 0; i < count; ++i) {
-    const int t = tiles[i], k0 = t * FA_TILE;
-    wait_vmcnt<0>();
-    ring_barrier();
-    if (i + 1 < count) {
-      const uint32_t to = lds0 + ((i + 1) & 1) * 2 * IMG;
-      ldk.start(kb, a.k.st, tiles[i + 1] * FA_TILE, n - 1, to);
-      ldv.start(vb, a.v.st, tiles[i + 1] * FA_TILE, n - 1, to + IMG);
-    }
+    const int k0 = tiles[i] * FA_TILE;
+    next_tile();
+    if (i + 1 < count) start(i + 1);
     const uint8_t* kimg = lds_raw + (i & 1) * 2 * IMG;
     const uint8_t* vimg = kimg + IMG;
-    // nothing of the tile is visible to the wavefront
-    if (k0 > last || first >= n || (k0 + FA_TILE - 1 <= first - a.window && k0 >= a.sinks)) continue;
-    acc16_t s[NQ][2];
+    if (nothing_seen(a, n, first, last, k0)) continue;
+    acc16_t s[2];
 #pragma unroll
-    for (int x = 0; x < NQ; ++x)
+    for (int nn = 0; nn < 2; ++nn)
 #pragma unroll
-      for (int nn = 0; nn < 2; ++nn)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[x][nn][r] = 0.f;
+      for (int r = 0; r < 16; ++r) s[nn][r] = 0.f;
 #pragma unroll
     for (int ss = 0; ss < D / 16; ++ss)
 #pragma unroll
-      for (int nn = 0; nn < 2; ++nn) {
-        const uint4 kf = img_rows<D>(kimg, nn, ss, lane);
+      for (int nn = 0; nn < 2; ++nn) mfma<T>::run(img_rows<D>(kimg, nn, ss, lane), qf[ss], s[nn]);
+    if (some_hidden(a, n, first, last, k0)) {
 #pragma unroll
-        for (int x = 0; x < NQ; ++x) mfma<T>::run(kf, qf[x][ss], s[x][nn]);
-      }
-    const bool edge = k0 + FA_TILE - 1 > first || last >= n || (k0 <= last - a.window && k0 + FA_TILE > a.sinks);
-    uint4 pf[NQ][FA_TILE / 16];
-#pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-      uint32_t dead = 0;                                        // bit 16 nn + r: the key of that register is not visible
-      if (edge) {
-        const int64_t from = qrow[x] - a.window;
-#pragma unroll
-        for (int nn = 0; nn < 2; ++nn)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = k0 + 32 * nn + 8 * (r / 4) + 4 * half + r % 4;
-            if (key > qrow[x] || qrow[x] >= n || (key <= from && key >= a.sinks)) { dead |= 1u << (16 * nn + r); s[x][nn][r] = 0.f; }
-          }
-      }
-      float top = FA_NEG;
+      for (int nn = 0; nn < 2; ++nn) hide_keys(s[nn], a, n, qrow, k0 + 32 * nn + 4 * half, hidden);
+    }
+    // the tile's maximum from the extreme raw score
+    float top = s[0][0];
+    if (a.scale_log2 >= 0.f) {
 #pragma unroll
       for (int nn = 0; nn < 2; ++nn)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[x][nn][r] *= a.scale_log2;
-          if (edge && ((dead >> (16 * nn + r)) & 1u) != 0) s[x][nn][r] = FA_NEG;
-          top = fmaxf(top, s[x][nn][r]);
-        }
-      const float mx = pair_max(top);
-      // The reference point follows the maximum lazily: it moves when a row's maximum has grown by more than 2^8
-      const bool grow = mx > m[x] + FA_LAZY;
-      if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-        const float m_new = grow ? mx : m[x];
-        const float alpha = fast_exp2(m[x] - m_new);
-        m[x] = m_new;
-        l[x] *= alpha;
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[x][j][r] *= alpha;
-      }
-      float sum = 0.f;
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[nn][r]);
+    } else {
 #pragma unroll
       for (int nn = 0; nn < 2; ++nn)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float p = fast_exp2(s[x][nn][r] - m[x]);
-          if (edge && ((dead >> (16 * nn + r)) & 1u) != 0) p = 0.f;   // m may still be the initial one
-          s[x][nn][r] = p;
-          sum += p;
-        }
-      l[x] += sum;
+        for (int r = 0; r < 16; ++r) top = fminf(top, s[nn][r]);
+    }
+    const float mx = pair_max(top * a.scale_log2);
+    // The reference point follows the maximum lazily: it moves when a row's maximum has grown by more than 2^8, so that
+    // probabilities relative to it stay below 256 and most tiles rescale nothing.
+    const bool grow = mx > m + FA_LAZY;
+    if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+      const float m_new = grow ? mx : m;
+      const float alpha = fast_exp2(m - m_new);
+      m = m_new;
+      l *= alpha;
 #pragma unroll
-      for (int kk = 0; kk < FA_TILE / 16; ++kk) {
-        float pv[8];
+      for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) pv[e] = s[x][kk / 2][8 * (kk % 2) + e];
-        pf[x][kk] = acc_to_operand<T>(pv);
-      }
+        for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
+    }
+    uint4 pf[FA_TILE / 16];
+#pragma unroll
+    for (int kk = 0; kk < FA_TILE / 16; ++kk) {
+      float pv[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pv[e] = fast_exp2(__builtin_fmaf(s[kk / 2][8 * (kk % 2) + e], a.scale_log2, -m));
+      pf[kk] = acc_to_operand<T>(pv);
+      // The sum is that of the rounded probabilities: the weights that the values get add up to one, and two of them cost
+      // one instruction.
+      l = dot2<T>(pf[kk].x, ONES, dot2<T>(pf[kk].y, ONES, dot2<T>(pf[kk].z, ONES, dot2<T>(pf[kk].w, ONES, l))));
     }
 #pragma unroll
     for (int kk = 0; kk < FA_TILE / 16; ++kk)
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const uint4 vf = img_columns<D>(vimg, j, kk, lane);
-#pragma unroll
-        for (int x = 0; x < NQ; ++x) mfma<T>::run(vf, pf[x][kk], o[x][j]);
-      }
+      for (int j = 0; j < D / 32; ++j) mfma<T>::run(img_columns<D>(vimg, j, kk, lane), pf[kk], o[j]);
   }
   __syncthreads();                                              // every wavefront is done with the images
-#pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    const float sum = pair_sum(l[x]);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (half == 0 && qrow[x] < a.len) lse[qrow[x]] = sum > 0.f ? (m[x] + log2f(sum)) * (1.0f / FA_LOG2E) : sum == 0.f ? -INFINITY : sum;
-    store_rows_out<T, D>(o[x], inv, lds_raw + wave * (32 * D * 2), ob, a.o.st, qw + 32 * x, a.len, lane);
-    if (x + 1 < NQ) __syncthreads();
-  }
+  const float sum = pair_sum(l);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (half == 0 && qrow < a.len)
+    a.lse[static_cast<int64_t>(bh) * a.len + qrow] = sum > 0.f ? (m + log2f(sum)) * (1.0f / FA_LOG2E) : sum == 0.f ? -INFINITY : sum;
+  store_rows_out<T, D>(o, inv, lds_raw + wave * (32 * D * 2), out_head<T>(a.o, b, h), a.o.st, qw, a.len, lane);
 }
 
 // ------------------------------------------------------------------------------------ backward: dQ, and D = rowsum(dO O)
-template <typename T, int D, int NQ>
-__global__ __launch_bounds__(64 * WA_WAVES, 1) void window_bwd_dq_kernel(WaArgs a) {
+template <typename T, int D>
+__global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_kernel(WaArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
-  constexpr int IMG = FA_TILE * D * 2, ROWS = 32 * NQ * WA_WAVES;
-  const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y), q0 = static_cast<int>(blockIdx.x) * ROWS;
+  constexpr int IMG = FA_TILE * D * 2;
+  const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y), q0 = static_cast<int>(blockIdx.x) * WA_ROWS;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const int n = seq_len(a, b), bh = b * a.heads + h;
-  const int end = min(q0 + ROWS, n), qw = q0 + 32 * NQ * wave;
+  const int end = min(q0 + WA_ROWS, n), qw = q0 + 32 * wave, qrow = qw + (lane & 31);
   const T *kb = at_head<T>(a.k, b, h / a.group), *vb = at_head<T>(a.v, b, h / a.group);
 
-  uint4 qf[NQ][D / 16], gf[NQ][D / 16];
-  int qrow[NQ];
-  float delta[NQ], lse2[NQ];
-  acc16_t dq[NQ][D / 32];
-#pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    qrow[x] = qw + 32 * x + (lane & 31);
-    load_resident<T, D>(qf[x], at_head<T>(a.q, b, h), a.q.st, qrow[x], n, lane);
-    load_resident<T, D>(gf[x], at_head<T>(a.d_o, b, h), a.d_o.st, qrow[x], n, lane);
-    uint4 of[D / 16];
-    load_resident<T, D>(of, at_head<T>(a.o, b, h), a.o.st, qrow[x], n, lane);
-    float d = 0.f;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      const T* u = reinterpret_cast<const T*>(&of[s]);
-      const T* w = reinterpret_cast<const T*>(&gf[x][s]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) d += elem<T>::to_float(u[e]) * elem<T>::to_float(w[e]);
-    }
-    delta[x] = pair_sum(d);
-    lse2[x] = -FA_NEG;                                          // rows behind the end: probability 0
-    if (qrow[x] < n) {
-      const int64_t at = static_cast<int64_t>(bh) * a.len + qrow[x];
-      const float v = a.lse[at];
-      lse2[x] = v == -INFINITY ? -FA_NEG : v * FA_LOG2E;
-      if (half == 0) a.delta[at] = delta[x];
-    }
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dq[x][i][r] = 0.f;
-  }
   const TileList tiles(a, q0, end > q0 ? end : 0);
   const int count = end > q0 ? tiles.count : 0;
   const TileLoader<T, D> ldk(a.k.st, wave, lane), ldv(a.v.st, wave, lane);
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw));
-  if (count > 0) {
-    ldk.start(kb, a.k.st, tiles[0] * FA_TILE, n - 1, lds0);
-    ldv.start(vb, a.v.st, tiles[0] * FA_TILE, n - 1, lds0 + IMG);
-  }
-  const int64_t first = qw, last = qw + 32 * NQ - 1;
-  for (int i = 0; i < count; ++i) {
-    const int t = tiles[i], k0 = t * FA_TILE;
-    wait_vmcnt<0>();
-    ring_barrier();
-    if (i + 1 < count) {
-      const uint32_t to = lds0 + ((i + 1) & 1) * 2 * IMG;
-      ldk.start(kb, a.k.st, tiles[i + 1] * FA_TILE, n - 1, to);
-      ldv.start(vb, a.v.st, tiles[i + 1] * FA_TILE, n - 1, to + IMG);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw)));
+  auto start = [&](int i) {
+    const int row = tiles[i] * FA_TILE;
+    const uint32_t to = lds0 + static_cast<uint32_t>(i & 1) * 2 * IMG;
+    ldk.start(kb, a.k.st, row, n - 1, to);
+    ldv.start(vb, a.v.st, row, n - 1, to + IMG);
+  };
+  uint4 qf[D / 16], gf[D / 16];
+  load_resident<T, D>(qf, at_head<T>(a.q, b, h), a.q.st, qrow, n, lane);
+  load_resident<T, D>(gf, at_head<T>(a.d_o, b, h), a.d_o.st, qrow, n, lane);
+  float delta = 0.f, lse2 = -FA_NEG;                            // rows behind the end: probability 0
+  {
+    uint4 of[D / 16];
+    load_resident<T, D>(of, at_head<T>(a.o, b, h), a.o.st, qrow, n, lane);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      delta = dot2<T>(of[s].x, gf[s].x, dot2<T>(of[s].y, gf[s].y, delta));
+      delta = dot2<T>(of[s].z, gf[s].z, dot2<T>(of[s].w, gf[s].w, delta));
     }
+    delta = pair_sum(delta);
+    if (qrow < n) {
+      const int64_t at = static_cast<int64_t>(bh) * a.len + qrow;
+      const float v = a.lse[at];
+      lse2 = v == -INFINITY ? -FA_NEG : v * FA_LOG2E;
+      if (half == 0) a.delta[at] = delta;
+    }
+  }
+  acc16_t dq[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
+  registers_landed(qf);
+  if (count > 0) start(0);
+  const int first = qw, last = qw + 31;
+  const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
+  for (int i = 0; i < count; ++i) {
+    const int k0 = tiles[i] * FA_TILE;
+    next_tile();
+    if (i + 1 < count) start(i + 1);
     const uint8_t* kimg = lds_raw + (i & 1) * 2 * IMG;
     const uint8_t* vimg = kimg + IMG;
-    if (k0 > last || first >= n || (k0 + FA_TILE - 1 <= first - a.window && k0 >= a.sinks)) continue;
-    const bool edge = k0 + FA_TILE - 1 > first || last >= n || (k0 <= last - a.window && k0 + FA_TILE > a.sinks);
-    uint4 df[NQ][FA_TILE / 16];
+    if (nothing_seen(a, n, first, last, k0)) continue;
+    const bool edge = some_hidden(a, n, first, last, k0);
+    // 32 keys at a time, so that scores, score gradients and their operands need half the registers
 #pragma unroll
     for (int nn = 0; nn < 2; ++nn) {
-      acc16_t s[NQ], dp[NQ];
+      acc16_t s, dp;
 #pragma unroll
-      for (int x = 0; x < NQ; ++x)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) { s[x][r] = 0.f; dp[x][r] = 0.f; }
+      for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
 #pragma unroll
       for (int ss = 0; ss < D / 16; ++ss) {
-        const uint4 kf = img_rows<D>(kimg, nn, ss, lane), vf = img_rows<D>(vimg, nn, ss, lane);
-#pragma unroll
-        for (int x = 0; x < NQ; ++x) {
-          mfma<T>::run(kf, qf[x][ss], s[x]);
-          mfma<T>::run(vf, gf[x][ss], dp[x]);
-        }
+        mfma<T>::run(img_rows<D>(kimg, nn, ss, lane), qf[ss], s);
+        mfma<T>::run(img_rows<D>(vimg, nn, ss, lane), gf[ss], dp);
       }
+      if (edge) hide_keys(s, a, n, qrow, k0 + 32 * nn + 4 * half, hidden);
 #pragma unroll
-      for (int x = 0; x < NQ; ++x) {
-        const int64_t from = qrow[x] - a.window;
+      for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], a.scale_log2, -lse2)) * (dp[r] - delta);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float p = fast_exp2(__builtin_fmaf(s[x][r], a.scale_log2, -lse2[x]));
-          if (edge) {
-            const int key = k0 + 32 * nn + 8 * (r / 4) + 4 * half + r % 4;
-            if (key > qrow[x] || qrow[x] >= n || (key <= from && key >= a.sinks)) p = 0.f;
-          }
-          s[x][r] = p * (dp[x][r] - delta[x]);
-        }
+      for (int kk = 0; kk < 2; ++kk) {
+        float dsv[8];
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          float dsv[8];
+        for (int e = 0; e < 8; ++e) dsv[e] = s[8 * kk + e];
+        const uint4 df = acc_to_operand<T>(dsv);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dsv[e] = s[x][8 * kk + e];
-          df[x][2 * nn + kk] = acc_to_operand<T>(dsv);
-        }
+        for (int j = 0; j < D / 32; ++j) mfma<T>::run(img_columns<D>(kimg, j, 2 * nn + kk, lane), df, dq[j]);
       }
     }
-#pragma unroll
-    for (int kk = 0; kk < FA_TILE / 16; ++kk)
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const uint4 kf = img_columns<D>(kimg, j, kk, lane);
-#pragma unroll
-        for (int x = 0; x < NQ; ++x) mfma<T>::run(kf, df[x][kk], dq[x][j]);
-      }
   }
   __syncthreads();
-  T* dqb = out_head<T>(a.dq, b, h);
-#pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    store_rows_out<T, D>(dq[x], a.scale, lds_raw + wave * (32 * D * 2), dqb, a.dq.st, qw + 32 * x, a.len, lane);
-    if (x + 1 < NQ) __syncthreads();
-  }
+  store_rows_out<T, D>(dq, a.scale, lds_raw + wave * (32 * D * 2), out_head<T>(a.dq, b, h), a.dq.st, qw, a.len, lane);
 }
 
 // ------------------------------------------------------------------------------------------------- backward: dK and dV
-// One key per lane pair: a block holds 128 keys of a key / value head, the queries of every head of its group come in tiles
-// of 64. The work is laid out so that blocks are alike (DkvPlan): the queries behind the windows of a block that holds sinks, up to
+// One key per lane pair: a block holds 128 keys of a key / value head, the queries of every head of its group come in tiles.
+// The work is laid out so that blocks are alike (DkvPlan): the queries behind the windows of a block that holds sinks, up to
 // the sequence's end, are shared out over `chunks` more blocks, and where the key blocks would not fill the chip each is
 // shared out over `parts`. Such blocks leave fp32 sums that a last kernel adds in a fixed order.
-constexpr int WA_KEYS = 32 * WA_WAVES;
 
 // accumulators of the wavefront's 32 rows as fp32 rows of D elements, `pitch` floats apart
 template <int D>
@@ -400,19 +355,34 @@ __device__ __forceinline__ void store_part(const acc16_t (&acc)[D / 32], float m
       *reinterpret_cast<float4*>(p + 32 * i + 8 * g) = make_float4(acc[i][4 * g] * mul, acc[i][4 * g + 1] * mul, acc[i][4 * g + 2] * mul, acc[i][4 * g + 3] * mul);
 }
 
+// Query tiles of 64, or of 32 for head_dim 128: two wavefronts of that size on a SIMD leave 256 registers each, which the
+// accumulators of 32 keys half fill, so the keys of a block are read from LDS (32 KB, which the smaller tiles make room for)
+// and only the values stay in registers. With both in registers there was one wavefront on a SIMD, and nothing ran
+// under the waits of the other: 8192 positions, window 1024, 32 heads of 128: 1178 us against 784.
+template <int D> constexpr int dkv_tile() { return D == 64 ? 64 : 32; }
+template <int D> constexpr int dkv_buf() { return 2 * dkv_tile<D>() * D * 2 + 2 * dkv_tile<D>() * 4; }   // Q, dO, lse2, D
+template <int D> constexpr int dkv_keys() { return D == 64 ? 0 : WA_ROWS * D * 2; }
+
 template <typename T, int D>
-__global__ __launch_bounds__(64 * WA_WAVES, 1) void window_bwd_dkv_kernel(WaArgs a) {
+__global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
-  constexpr int IMG = FA_TILE * D * 2, BUF = 2 * IMG + 2 * FA_TILE * 4;   // Q, dO, lse2[64], D[64]
+  constexpr int TILE = dkv_tile<D>(), IMG = TILE * D * 2, BUF = dkv_buf<D>();
+  constexpr bool KEYS_IN_LDS = dkv_keys<D>() > 0;
   const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y);
   // blocks behind the key blocks' parts: chunk of the queries that see a block's keys as sinks only
   const int x = static_cast<int>(blockIdx.x), own = a.key_blocks * a.parts;
   const bool sink_chunk = x >= own;
-  const int k0 = (sink_chunk ? (x - own) / a.chunks : x / a.parts) * WA_KEYS, share = sink_chunk ? (x - own) % a.chunks : x % a.parts;
+  const int k0 = (sink_chunk ? (x - own) / a.chunks : x / a.parts) * WA_ROWS, share = sink_chunk ? (x - own) % a.chunks : x % a.parts;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const int n = seq_len(a, b), kw = k0 + 32 * wave, krow = kw + (lane & 31);
-  uint4 kf[D / 16], vf[D / 16];
-  load_resident<T, D>(kf, at_head<T>(a.k, b, h), a.k.st, krow, n, lane);
+  uint4 kf[KEYS_IN_LDS ? 1 : D / 16], vf[D / 16];
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw)));
+  const uint8_t* keys = lds_raw + 2 * BUF + wave * (32 * D * 2);
+  if constexpr (KEYS_IN_LDS) {
+    if (k0 < n) TileLoader<T, D, WA_ROWS>(a.k.st, wave, lane).start(at_head<T>(a.k, b, h), a.k.st, k0, n - 1, lds0 + 2 * BUF);
+  } else {
+    load_resident<T, D>(kf, at_head<T>(a.k, b, h), a.k.st, krow, n, lane);
+  }
   load_resident<T, D>(vf, at_head<T>(a.v, b, h), a.v.st, krow, n, lane);
   acc16_t dk[D / 32], dv[D / 32];
 #pragma unroll
@@ -421,38 +391,38 @@ __global__ __launch_bounds__(64 * WA_WAVES, 1) void window_bwd_dkv_kernel(WaArgs
     for (int r = 0; r < 16; ++r) { dk[i][r] = 0.f; dv[i][r] = 0.f; }
 
   // the query tiles up to the end of the last key's window, and those behind it
-  const int64_t reach = static_cast<int64_t>(k0) + WA_KEYS - 1 + a.window;
-  const int tw = static_cast<int>(((reach < n ? reach : n) + FA_TILE - 1) / FA_TILE), tn = (n + FA_TILE - 1) / FA_TILE;
-  const int t0 = sink_chunk ? tw : k0 / FA_TILE, t1 = sink_chunk ? tn : tw;
+  const int64_t reach = static_cast<int64_t>(k0) + WA_ROWS - 1 + a.window;
+  const int tw = static_cast<int>(((reach < n ? reach : n) + TILE - 1) / TILE), tn = (n + TILE - 1) / TILE;
+  const int t0 = sink_chunk ? tw : k0 / TILE, t1 = sink_chunk ? tn : tw;
   const int per = k0 < n ? t1 - t0 : 0, all = per * a.group, shares = sink_chunk ? a.chunks : a.parts;
   // this block's share of the (head, tile) pairs
   const int i0 = static_cast<int>(static_cast<int64_t>(all) * share / shares), i1 = static_cast<int>(static_cast<int64_t>(all) * (share + 1) / shares);
-  const TileLoader<T, D> ldq(a.q.st, wave, lane), ldg(a.d_o.st, wave, lane);
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw));
+  const TileLoader<T, D, TILE> ldq(a.q.st, wave, lane), ldg(a.d_o.st, wave, lane);
+  const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
   float st_raw = 0.f;
   const int tid = static_cast<int>(threadIdx.x);
   // threads 0..63: the log-sum-exp of the tile's queries (-inf behind the end), 64..127: their D; asked for ahead of the tile's
   // transfers and looked at behind them, at the end of the iteration
   auto start = [&](int i, uint32_t to) {
-    const int hq = h * a.group + i / per, q0 = (t0 + i % per) * FA_TILE;
-    if (tid < 2 * FA_TILE) {
-      const int qi = q0 + (tid & (FA_TILE - 1));
-      const float* src = (tid < FA_TILE ? a.lse : a.delta) + (static_cast<int64_t>(b) * a.heads + hq) * a.len;
-      st_raw = tid < FA_TILE ? -INFINITY : 0.f;
+    const int hq = h * a.group + i / per, q0 = (t0 + i % per) * TILE;
+    if (tid < 2 * TILE) {
+      const int qi = q0 + (tid & (TILE - 1));
+      const float* src = (tid < TILE ? a.lse : a.delta) + (static_cast<int64_t>(b) * a.heads + hq) * a.len;
+      st_raw = tid < TILE ? -INFINITY : 0.f;
       if (qi < n) st_raw = src[qi];
     }
     ldq.start(at_head<T>(a.q, b, hq), a.q.st, q0, n - 1, to);
     ldg.start(at_head<T>(a.d_o, b, hq), a.d_o.st, q0, n - 1, to + IMG);
   };
   auto store_stats = [&](uint8_t* buf) {
-    if (tid < 2 * FA_TILE) reinterpret_cast<float*>(buf + 2 * IMG)[tid] = tid < FA_TILE ? (st_raw == -INFINITY ? -FA_NEG : st_raw * FA_LOG2E) : st_raw;
+    if (tid < 2 * TILE) reinterpret_cast<float*>(buf + 2 * IMG)[tid] = tid < TILE ? (st_raw == -INFINITY ? -FA_NEG : st_raw * FA_LOG2E) : st_raw;
   };
   if (i0 < i1) {
     start(i0, lds0 + (i0 & 1) * BUF);
     store_stats(lds_raw + (i0 & 1) * BUF);
   }
   for (int i = i0; i < i1; ++i) {
-    const int q0 = (t0 + i % per) * FA_TILE;
+    const int q0 = (t0 + i % per) * TILE;
     wait_vmcnt<0>();
     __syncthreads();
     if (i + 1 < i1) start(i + 1, lds0 + ((i + 1) & 1) * BUF);
@@ -460,34 +430,45 @@ __global__ __launch_bounds__(64 * WA_WAVES, 1) void window_bwd_dkv_kernel(WaArgs
     const uint8_t* gimg = qimg + IMG;
     const float* stats = reinterpret_cast<const float*>(qimg + 2 * IMG);
     const int64_t klast = kw + 31;
-    const bool nothing = q0 + FA_TILE - 1 < kw || kw >= n || (q0 - a.window >= klast && kw >= a.sinks);
+    const bool nothing = q0 + TILE - 1 < kw || kw >= n || (q0 - a.window >= klast && kw >= a.sinks);
     if (!nothing) {
-      const bool edge = q0 < klast || klast >= n || (q0 + FA_TILE - 1 - a.window >= kw && klast >= a.sinks);
-      uint4 pf[FA_TILE / 16], df[FA_TILE / 16];
+      const bool edge = q0 < klast || klast >= n || (q0 + TILE - 1 - a.window >= kw && klast >= a.sinks);
+      // 32 queries at a time, so that scores, their gradients and their operands need half the registers
 #pragma unroll
-      for (int nn = 0; nn < 2; ++nn) {
+      for (int nn = 0; nn < TILE / 32; ++nn) {
+        uint4 pf[2], df[2];
         acc16_t s, dp;
 #pragma unroll
         for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
 #pragma unroll
         for (int ss = 0; ss < D / 16; ++ss) {
-          mfma<T>::run(img_rows<D>(qimg, nn, ss, lane), kf[ss], s);
+          uint4 key;
+          if constexpr (KEYS_IN_LDS) key = img_rows<D>(keys, 0, ss, lane);
+          else key = kf[ss];
+          mfma<T>::run(img_rows<D>(qimg, nn, ss, lane), key, s);
           mfma<T>::run(img_rows<D>(gimg, nn, ss, lane), vf[ss], dp);
+        }
+        if (edge) {
+          // queries that do not see this lane's key: in front of it, or behind its window (a sink has none)
+          const int at = q0 + 32 * nn + 4 * half;
+          const int64_t behind = krow < a.sinks ? n : krow + a.window;
+          const int from = krow < n ? krow - at : n, to = static_cast<int>(behind < n ? behind : n) - at;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int qi = 8 * (r / 4) + r % 4;
+            s[r] = (qi < from) | (qi >= to) ? hidden : s[r];
+          }
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int ql = 32 * nn + 8 * g + 4 * half;            // first of four consecutive queries, within the tile
           const float4 l4 = *reinterpret_cast<const float4*>(stats + ql);
-          const float4 d4 = *reinterpret_cast<const float4*>(stats + FA_TILE + ql);
+          const float4 d4 = *reinterpret_cast<const float4*>(stats + TILE + ql);
           const float lse2[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int r = 4 * g + e;
-            float p = fast_exp2(__builtin_fmaf(s[r], a.scale_log2, -lse2[e]));
-            if (edge) {
-              const int64_t qi = q0 + ql + e;
-              if (krow > qi || krow >= n || (krow <= qi - a.window && krow >= a.sinks)) p = 0.f;
-            }
+            const float p = fast_exp2(__builtin_fmaf(s[r], a.scale_log2, -lse2[e]));
             s[r] = p * (dp[r] - dl[e]);
             dp[r] = p;
           }
@@ -497,21 +478,22 @@ __global__ __launch_bounds__(64 * WA_WAVES, 1) void window_bwd_dkv_kernel(WaArgs
           float pv[8], dsv[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) { pv[e] = dp[8 * kk + e]; dsv[e] = s[8 * kk + e]; }
-          pf[2 * nn + kk] = acc_to_operand<T>(pv);
-          df[2 * nn + kk] = acc_to_operand<T>(dsv);
+          pf[kk] = acc_to_operand<T>(pv);
+          df[kk] = acc_to_operand<T>(dsv);
         }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            mfma<T>::run(img_columns<D>(gimg, j, 2 * nn + kk, lane), pf[kk], dv[j]);
+            mfma<T>::run(img_columns<D>(qimg, j, 2 * nn + kk, lane), df[kk], dk[j]);
+          }
       }
-#pragma unroll
-      for (int kk = 0; kk < FA_TILE / 16; ++kk)
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          mfma<T>::run(img_columns<D>(gimg, j, kk, lane), pf[kk], dv[j]);
-          mfma<T>::run(img_columns<D>(qimg, j, kk, lane), df[kk], dk[j]);
-        }
     }
     if (i + 1 < i1) store_stats(lds_raw + ((i + 1) & 1) * BUF);
   }
-  const bool in_parts = sink_chunk || a.parts > 1 || k0 < a.sink_blocks * WA_KEYS;
+  wait_vmcnt<0>();                                              // of a share without a tile: the keys' transfers
+  const bool in_parts = sink_chunk || a.parts > 1 || k0 < a.sink_blocks * WA_ROWS;
   if (in_parts) {
     const int rows = sink_chunk ? a.sink_rows : a.part_rows;
     float* base = (sink_chunk ? a.sink_part : a.part) +
@@ -576,6 +558,9 @@ int check_views(const char* what, WaView* views, const void* const* pointers, co
   return 0;
 }
 
+// a scale of zero as one so small that every score is: hidden scores are infinite, and infinity times it stays so
+float log2_scale(float scale) { return scale == 0.f ? 1e-30f : scale * FA_LOG2E; }
+
 template <typename K>
 int launch_tiled(K kern, int lds, dim3 grid, const WaArgs& a, hipStream_t st, const char* what) {
   if (lds > 64 * 1024) {
@@ -585,8 +570,8 @@ int launch_tiled(K kern, int lds, dim3 grid, const WaArgs& a, hipStream_t st, co
   hipLaunchKernelGGL(kern, grid, dim3(64 * WA_WAVES), lds, st, a);
   return 0;
 }
-template <int D> constexpr int fwd_lds() { return std::max(4 * FA_TILE * D * 2, WA_WAVES * 32 * D * 2); }
-template <int D> constexpr int dkv_lds() { return std::max(2 * (2 * FA_TILE * D * 2 + 2 * FA_TILE * 4), WA_WAVES * 32 * D * 2); }
+template <int D> constexpr int tiles_lds() { return std::max(4 * FA_TILE * D * 2, WA_WAVES * 32 * D * 2); }
+template <int D> constexpr int dkv_lds() { return std::max(2 * dkv_buf<D>() + dkv_keys<D>(), WA_WAVES * 32 * D * 2); }
 dim3 row_grid(const WaArgs& a, int rows, int64_t heads, int64_t batch) {
   return dim3(static_cast<unsigned>((a.len + rows - 1) / rows), static_cast<unsigned>(heads), static_cast<unsigned>(batch));
 }
@@ -594,23 +579,23 @@ dim3 row_grid(const WaArgs& a, int rows, int64_t heads, int64_t batch) {
 template <typename T, int D>
 int fwd_launch(const WaArgs& a, int64_t batch, hipStream_t st) {
   TraceScope trace("window_attn_fwd", st);
-  return launch_tiled(window_fwd_kernel<T, D, 1>, fwd_lds<D>(), row_grid(a, 32 * WA_WAVES, a.heads, batch), a, st, "window_attn_fwd");
+  return launch_tiled(window_fwd_kernel<T, D>, tiles_lds<D>(), row_grid(a, WA_ROWS, a.heads, batch), a, st, "window_attn_fwd");
 }
 // How the blocks of dK and dV are laid out, and the floats they leave behind.
 struct DkvPlan {
   int key_blocks, sink_blocks, parts, chunks, part_rows, sink_rows;
   int64_t part_floats, sink_floats;
   DkvPlan(int64_t len, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window, int64_t sinks) {
-    const int64_t blocks = (len + WA_KEYS - 1) / WA_KEYS, group = heads / kv_heads;
-    const int64_t tiles = (std::min(len, window + WA_KEYS) + FA_TILE - 1) / FA_TILE;      // query tiles of a key block, per head
+    const int64_t blocks = (len + WA_ROWS - 1) / WA_ROWS, group = heads / kv_heads;
+    const int64_t tiles = (std::min(len, window + WA_ROWS) + FA_TILE - 1) / FA_TILE;      // query tiles of a key block, per head
     key_blocks = static_cast<int>(blocks);
     // some query stands behind the window of a block's first sinks
-    sink_blocks = len > WA_KEYS - 1 + window ? static_cast<int>(std::min(blocks, (std::min(sinks, len) + WA_KEYS - 1) / WA_KEYS)) : 0;
+    sink_blocks = len > WA_ROWS - 1 + window ? static_cast<int>(std::min(blocks, (std::min(sinks, len) + WA_ROWS - 1) / WA_ROWS)) : 0;
     const int64_t behind = (len - std::min(len, window) + FA_TILE - 1) / FA_TILE;
     chunks = sink_blocks > 0 ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((behind + tiles - 1) / tiles, 128))) : 0;
     // two blocks for every compute unit, each with at least four tiles
     parts = static_cast<int>(std::max<int64_t>(1, std::min({(2 * num_cus() + blocks * batch * kv_heads - 1) / (blocks * batch * kv_heads), tiles * group / 4, int64_t(16)})));
-    sink_rows = static_cast<int>(std::min<int64_t>(len, static_cast<int64_t>(sink_blocks) * WA_KEYS));
+    sink_rows = static_cast<int>(std::min<int64_t>(len, static_cast<int64_t>(sink_blocks) * WA_ROWS));
     part_rows = parts > 1 ? static_cast<int>(len) : sink_rows;
     part_floats = batch * kv_heads * parts * part_rows * 2 * head_dim;
     sink_floats = batch * kv_heads * chunks * sink_rows * 2 * head_dim;
@@ -622,7 +607,7 @@ template <typename T, int D>
 int bwd_launch(const WaArgs& a, int64_t batch, hipStream_t st) {
   {
     TraceScope trace("window_attn_bwd_dq", st);
-    if (int rc = launch_tiled(window_bwd_dq_kernel<T, D, 1>, fwd_lds<D>(), row_grid(a, 32 * WA_WAVES, a.heads, batch), a, st, "window_attn_bwd")) return rc;
+    if (int rc = launch_tiled(window_bwd_dq_kernel<T, D>, tiles_lds<D>(), row_grid(a, WA_ROWS, a.heads, batch), a, st, "window_attn_bwd")) return rc;
   }
   {
     TraceScope trace("window_attn_bwd_dkv", st);
@@ -656,7 +641,7 @@ extern "C" int nmtg_window_attn_fwd(const void* q, const void* k, const void* v,
   WaArgs a = {};
   a.q = views[0]; a.k = views[1]; a.v = views[2]; a.o = views[3];
   a.lse = softmax_lse; a.lengths = lengths; a.len = static_cast<int>(len); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
-  a.group = static_cast<int>(heads / kv_heads); a.window = window; a.sinks = sinks; a.scale = softmax_scale; a.scale_log2 = softmax_scale * FA_LOG2E;
+  a.group = static_cast<int>(heads / kv_heads); a.window = window; a.sinks = sinks; a.scale = softmax_scale; a.scale_log2 = log2_scale(softmax_scale);
   hipStream_t st = static_cast<hipStream_t>(stream);
   int rc;
   if (dtype == NMTG_F16) rc = head_dim == 64 ? fwd_launch<f16_t, 64>(a, batch, st) : fwd_launch<f16_t, 128>(a, batch, st);
@@ -698,7 +683,7 @@ extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void*
   a.part_rows = plan.part_rows; a.sink_rows = plan.sink_rows;
   a.lengths = lengths; a.len = static_cast<int>(len);
   a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads); a.group = static_cast<int>(heads / kv_heads);
-  a.window = window; a.sinks = sinks; a.scale = softmax_scale; a.scale_log2 = softmax_scale * FA_LOG2E;
+  a.window = window; a.sinks = sinks; a.scale = softmax_scale; a.scale_log2 = log2_scale(softmax_scale);
   hipStream_t st = static_cast<hipStream_t>(stream);
   int rc;
   if (dtype == NMTG_F16) rc = head_dim == 64 ? bwd_launch<f16_t, 64>(a, batch, st) : bwd_launch<f16_t, 128>(a, batch, st);
