@@ -25,13 +25,26 @@ namespace {
 
 constexpr int WA_WAVES = 4, WA_ROWS = 32 * WA_WAVES;   // of a block: 128 queries (forward, dQ) or keys (dK, dV), 32 per wavefront
 
+// Consecutive blocks of a launch go round the eight XCDs, each with an L2 of its own: item i of `total` in launch order, re-counted so
+// that every XCD gets a contiguous piece, in which blocks that read the same keys and values are neighbours.
+__device__ __forceinline__ uint32_t xcd_item(uint32_t i, uint32_t total) {
+  const uint32_t xcd = i & 7, share = total >> 3, more = total & 7;
+  return xcd * share + min(xcd, more) + (i >> 3);
+}
+// Query block x of head h, sequence b: the heads of a group first, then the blocks of the sequence.
+struct WaBlock { int x, h, b; };
+__device__ __forceinline__ WaBlock query_block(int blocks, int group, int kv_heads) {
+  const uint32_t id = xcd_item(blockIdx.x, gridDim.x), rest = id / group, kv = rest / blocks;
+  return {static_cast<int>(rest % blocks), static_cast<int>(kv % kv_heads * group + id % group), static_cast<int>(kv / kv_heads)};
+}
+
 struct WaView { const void* p; int64_t st, sb, sh; };   // [len, batch, heads, head_dim], head_dim contiguous
 
 struct WaArgs {
   WaView q, k, v, o, d_o, dq, dk, dv;
   float *lse, *delta;        // [batch, heads, len]
   const int32_t* lengths;    // [batch] or null: every sequence fills `len`
-  int len, heads, kv_heads, group;
+  int len, batch, heads, kv_heads, group;
   int64_t window, sinks;
   float scale, scale_log2;
   // backward, dK and dV in parts (see DkvPlan): fp32 [parts][batch, kv_heads, part_rows][2][head_dim] of the key blocks, then
@@ -149,7 +162,8 @@ template <typename T, int D>
 __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_kernel(WaArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
   constexpr int IMG = FA_TILE * D * 2;
-  const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y), q0 = static_cast<int>(blockIdx.x) * WA_ROWS;
+  const WaBlock block = query_block((a.len + WA_ROWS - 1) / WA_ROWS, a.group, a.kv_heads);
+  const int b = block.b, h = block.h, q0 = block.x * WA_ROWS;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const int n = seq_len(a, b), bh = b * a.heads + h;
   const int end = min(q0 + WA_ROWS, n), qw = q0 + 32 * wave, qrow = qw + (lane & 31);
@@ -254,7 +268,8 @@ template <typename T, int D>
 __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_kernel(WaArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
   constexpr int IMG = FA_TILE * D * 2;
-  const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y), q0 = static_cast<int>(blockIdx.x) * WA_ROWS;
+  const WaBlock block = query_block((a.len + WA_ROWS - 1) / WA_ROWS, a.group, a.kv_heads);
+  const int b = block.b, h = block.h, q0 = block.x * WA_ROWS;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const int n = seq_len(a, b), bh = b * a.heads + h;
   const int end = min(q0 + WA_ROWS, n), qw = q0 + 32 * wave, qrow = qw + (lane & 31);
@@ -368,11 +383,13 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
   extern __shared__ __align__(16) uint8_t lds_raw[];
   constexpr int TILE = dkv_tile<D>(), IMG = TILE * D * 2, BUF = dkv_buf<D>();
   constexpr bool KEYS_IN_LDS = dkv_keys<D>() > 0;
-  const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y);
-  // blocks behind the key blocks' parts: chunk of the queries that see a block's keys as sinks only
-  const int x = static_cast<int>(blockIdx.x), own = a.key_blocks * a.parts;
-  const bool sink_chunk = x >= own;
-  const int k0 = (sink_chunk ? (x - own) / a.chunks : x / a.parts) * WA_ROWS, share = sink_chunk ? (x - own) % a.chunks : x % a.parts;
+  // the key blocks' parts first, then, shorter and so the ones to end with, the chunks of queries that see a block's keys as sinks only
+  const uint32_t own = static_cast<uint32_t>(a.key_blocks * a.parts), heads = static_cast<uint32_t>(a.kv_heads) * a.batch;
+  const bool sink_chunk = blockIdx.x >= own * heads;
+  const uint32_t id = sink_chunk ? xcd_item(blockIdx.x - own * heads, gridDim.x - own * heads) : xcd_item(blockIdx.x, own * heads);
+  const uint32_t per_head = sink_chunk ? static_cast<uint32_t>(a.sink_blocks * a.chunks) : own, shares = sink_chunk ? a.chunks : a.parts;
+  const int h = static_cast<int>(id / per_head % a.kv_heads), b = static_cast<int>(id / per_head / a.kv_heads);
+  const int k0 = static_cast<int>(id % per_head / shares) * WA_ROWS, share = static_cast<int>(id % per_head % shares);
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const int n = seq_len(a, b), kw = k0 + 32 * wave, krow = kw + (lane & 31);
   uint4 kf[KEYS_IN_LDS ? 1 : D / 16], vf[D / 16];
@@ -394,9 +411,9 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
   const int64_t reach = static_cast<int64_t>(k0) + WA_ROWS - 1 + a.window;
   const int tw = static_cast<int>(((reach < n ? reach : n) + TILE - 1) / TILE), tn = (n + TILE - 1) / TILE;
   const int t0 = sink_chunk ? tw : k0 / TILE, t1 = sink_chunk ? tn : tw;
-  const int per = k0 < n ? t1 - t0 : 0, all = per * a.group, shares = sink_chunk ? a.chunks : a.parts;
+  const int per = k0 < n ? t1 - t0 : 0, all = per * a.group;
   // this block's share of the (head, tile) pairs
-  const int i0 = static_cast<int>(static_cast<int64_t>(all) * share / shares), i1 = static_cast<int>(static_cast<int64_t>(all) * (share + 1) / shares);
+  const int i0 = static_cast<int>(static_cast<int64_t>(all) * share / static_cast<int>(shares)), i1 = static_cast<int>(static_cast<int64_t>(all) * (share + 1) / static_cast<int>(shares));
   const TileLoader<T, D, TILE> ldq(a.q.st, wave, lane), ldg(a.d_o.st, wave, lane);
   const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
   float st_raw = 0.f;
@@ -497,7 +514,7 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
   if (in_parts) {
     const int rows = sink_chunk ? a.sink_rows : a.part_rows;
     float* base = (sink_chunk ? a.sink_part : a.part) +
-                  ((static_cast<int64_t>(share) * gridDim.z + b) * a.kv_heads + h) * rows * (2 * D);
+                  ((static_cast<int64_t>(share) * a.batch + b) * a.kv_heads + h) * rows * (2 * D);
     store_part<D>(dk, a.scale, base, 2 * D, kw, rows, lane);
     store_part<D>(dv, 1.f, base + D, 2 * D, kw, rows, lane);
     return;
@@ -544,6 +561,7 @@ int check_call(const char* what, int64_t len, int64_t batch, int64_t heads, int6
                (long long)window, (long long)sinks);
   NMTG_REQUIRE(scale >= -1e6f && scale <= 1e6f, "%s: scale %g", what, (double)scale);
   NMTG_REQUIRE(heads <= 65535 && batch <= 65535 && len <= (1 << 24), "%s: more than 65535 heads or sequences, or 2^24 positions", what);
+  NMTG_REQUIRE((len / 128 + 1) * 32 * heads * batch <= 0x7fffffff, "%s: too many blocks in one launch", what);
   return 0;
 }
 // Views whose tile of 64 rows lies within 32-bit offsets of its first row
@@ -572,14 +590,13 @@ int launch_tiled(K kern, int lds, dim3 grid, const WaArgs& a, hipStream_t st, co
 }
 template <int D> constexpr int tiles_lds() { return std::max(4 * FA_TILE * D * 2, WA_WAVES * 32 * D * 2); }
 template <int D> constexpr int dkv_lds() { return std::max(2 * dkv_buf<D>() + dkv_keys<D>(), WA_WAVES * 32 * D * 2); }
-dim3 row_grid(const WaArgs& a, int rows, int64_t heads, int64_t batch) {
-  return dim3(static_cast<unsigned>((a.len + rows - 1) / rows), static_cast<unsigned>(heads), static_cast<unsigned>(batch));
-}
+dim3 linear_grid(const WaArgs& a, int64_t blocks, int64_t heads) { return dim3(static_cast<unsigned>(blocks * heads * a.batch)); }
+int64_t row_blocks(const WaArgs& a) { return (a.len + WA_ROWS - 1) / WA_ROWS; }
 
 template <typename T, int D>
-int fwd_launch(const WaArgs& a, int64_t batch, hipStream_t st) {
+int fwd_launch(const WaArgs& a, hipStream_t st) {
   TraceScope trace("window_attn_fwd", st);
-  return launch_tiled(window_fwd_kernel<T, D>, tiles_lds<D>(), row_grid(a, WA_ROWS, a.heads, batch), a, st, "window_attn_fwd");
+  return launch_tiled(window_fwd_kernel<T, D>, tiles_lds<D>(), linear_grid(a, row_blocks(a), a.heads), a, st, "window_attn_fwd");
 }
 // How the blocks of dK and dV are laid out, and the floats they leave behind.
 struct DkvPlan {
@@ -604,20 +621,20 @@ struct DkvPlan {
 int64_t delta_floats(int64_t len, int64_t batch, int64_t heads) { return (batch * heads * len + 63) / 64 * 64; }
 
 template <typename T, int D>
-int bwd_launch(const WaArgs& a, int64_t batch, hipStream_t st) {
+int bwd_launch(const WaArgs& a, hipStream_t st) {
   {
     TraceScope trace("window_attn_bwd_dq", st);
-    if (int rc = launch_tiled(window_bwd_dq_kernel<T, D>, tiles_lds<D>(), row_grid(a, WA_ROWS, a.heads, batch), a, st, "window_attn_bwd")) return rc;
+    if (int rc = launch_tiled(window_bwd_dq_kernel<T, D>, tiles_lds<D>(), linear_grid(a, row_blocks(a), a.heads), a, st, "window_attn_bwd")) return rc;
   }
   {
     TraceScope trace("window_attn_bwd_dkv", st);
-    const dim3 grid(static_cast<unsigned>(a.key_blocks * a.parts + a.sink_blocks * a.chunks), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch));
+    const dim3 grid = linear_grid(a, a.key_blocks * a.parts + a.sink_blocks * a.chunks, a.kv_heads);
     if (int rc = launch_tiled(window_bwd_dkv_kernel<T, D>, dkv_lds<D>(), grid, a, st, "window_attn_bwd")) return rc;
   }
   if (a.part_rows > 0) {
     TraceScope trace("window_attn_bwd_join", st);
     const int64_t total = static_cast<int64_t>(a.part_rows) * (2 * D / 4);
-    hipLaunchKernelGGL((window_dkv_join_kernel<T, D>), dim3(static_cast<unsigned>((total + 255) / 256), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch)),
+    hipLaunchKernelGGL((window_dkv_join_kernel<T, D>), dim3(static_cast<unsigned>((total + 255) / 256), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(a.batch)),
                        dim3(256), 0, st, a, total);
   }
   return 0;
@@ -640,12 +657,12 @@ extern "C" int nmtg_window_attn_fwd(const void* q, const void* k, const void* v,
   if (int rc = check_views(what, views, pointers, strides, 4)) return rc;
   WaArgs a = {};
   a.q = views[0]; a.k = views[1]; a.v = views[2]; a.o = views[3];
-  a.lse = softmax_lse; a.lengths = lengths; a.len = static_cast<int>(len); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
+  a.lse = softmax_lse; a.lengths = lengths; a.len = static_cast<int>(len); a.batch = static_cast<int>(batch); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
   a.group = static_cast<int>(heads / kv_heads); a.window = window; a.sinks = sinks; a.scale = softmax_scale; a.scale_log2 = log2_scale(softmax_scale);
   hipStream_t st = static_cast<hipStream_t>(stream);
   int rc;
-  if (dtype == NMTG_F16) rc = head_dim == 64 ? fwd_launch<f16_t, 64>(a, batch, st) : fwd_launch<f16_t, 128>(a, batch, st);
-  else rc = head_dim == 64 ? fwd_launch<bf16_t, 64>(a, batch, st) : fwd_launch<bf16_t, 128>(a, batch, st);
+  if (dtype == NMTG_F16) rc = head_dim == 64 ? fwd_launch<f16_t, 64>(a, st) : fwd_launch<f16_t, 128>(a, st);
+  else rc = head_dim == 64 ? fwd_launch<bf16_t, 64>(a, st) : fwd_launch<bf16_t, 128>(a, st);
   if (rc) return rc;
   NMTG_CHECK_LAUNCH(what);
   return 0;
@@ -682,12 +699,12 @@ extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void*
   a.key_blocks = plan.key_blocks; a.sink_blocks = plan.sink_blocks; a.parts = plan.parts; a.chunks = plan.chunks;
   a.part_rows = plan.part_rows; a.sink_rows = plan.sink_rows;
   a.lengths = lengths; a.len = static_cast<int>(len);
-  a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads); a.group = static_cast<int>(heads / kv_heads);
+  a.batch = static_cast<int>(batch); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads); a.group = static_cast<int>(heads / kv_heads);
   a.window = window; a.sinks = sinks; a.scale = softmax_scale; a.scale_log2 = log2_scale(softmax_scale);
   hipStream_t st = static_cast<hipStream_t>(stream);
   int rc;
-  if (dtype == NMTG_F16) rc = head_dim == 64 ? bwd_launch<f16_t, 64>(a, batch, st) : bwd_launch<f16_t, 128>(a, batch, st);
-  else rc = head_dim == 64 ? bwd_launch<bf16_t, 64>(a, batch, st) : bwd_launch<bf16_t, 128>(a, batch, st);
+  if (dtype == NMTG_F16) rc = head_dim == 64 ? bwd_launch<f16_t, 64>(a, st) : bwd_launch<f16_t, 128>(a, st);
+  else rc = head_dim == 64 ? bwd_launch<bf16_t, 64>(a, st) : bwd_launch<bf16_t, 128>(a, st);
   if (rc) return rc;
   NMTG_CHECK_LAUNCH(what);
   return 0;
