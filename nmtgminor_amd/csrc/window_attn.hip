@@ -66,9 +66,9 @@ __device__ __forceinline__ int seq_len(const WaArgs& a, int b) {
 
 // ---- the LDS image ----
 template <int D>
-__device__ __forceinline__ uint32_t img_at(int r, int c) {
-  return static_cast<uint32_t>(r * (2 * D) + ((c ^ (2 * (r & 3) | ((r >> 2) & 1))) * 16));
-}
+__device__ __forceinline__ int img_swizzle(int r) { return D == 64 ? (4 * ((r >> 1) & 1) | ((r >> 2) & 3)) : (4 * (r & 3) | ((r >> 2) & 3)); }
+template <int D>
+__device__ __forceinline__ uint32_t img_at(int r, int c) { return static_cast<uint32_t>(r * (2 * D) + (c ^ img_swizzle<D>(r)) * 16); }
 // A operand: rows 32 i + (lane & 31), columns 16 s + 8 (lane >> 5) .. + 7
 template <int D>
 __device__ __forceinline__ uint4 img_rows(const uint8_t* img, int i, int s, int lane) {
@@ -98,7 +98,7 @@ struct TileLoader {
   __device__ __forceinline__ TileLoader(int64_t stride_t, int wave_, int lane) : wave(wave_) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int id = 64 * (wave * N + n) + lane, r = id / CH, c = (id % CH) ^ (2 * (r & 3) | ((r >> 2) & 1));
+      const int id = 64 * (wave * N + n) + lane, r = id / CH, c = (id % CH) ^ img_swizzle<D>(r);
       row[n] = r;
       voff[n] = static_cast<uint32_t>(r * stride_t * 2 + c * 16);
     }
