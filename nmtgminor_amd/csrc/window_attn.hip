@@ -94,26 +94,38 @@ template <typename T, int D, int ROWS = FA_TILE>
 struct TileLoader {
   static constexpr int CH = D / 8, N = ROWS * CH / 64 / WA_WAVES;
   uint32_t voff[N];
-  int row[N], wave;
-  __device__ __forceinline__ TileLoader(int64_t stride_t, int wave_, int lane) : wave(wave_) {
+  int wave, lane;
+  __device__ __forceinline__ TileLoader(int64_t stride_t, int wave_, int lane_) : wave(wave_), lane(lane_) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int id = 64 * (wave * N + n) + lane, r = id / CH, c = (id % CH) ^ img_swizzle<D>(r);
-      row[n] = r;
       voff[n] = static_cast<uint32_t>(r * stride_t * 2 + c * 16);
     }
   }
   __device__ __forceinline__ void start(const T* head, int64_t stride_t, int first, int last, uint32_t img) const {
     const T* base = head + static_cast<int64_t>(first) * stride_t;
-    const bool whole = first + ROWS - 1 <= last;
+    const uint32_t to = img + static_cast<uint32_t>(wave * N * 1024);
+    if (first + ROWS - 1 <= last) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      uint32_t off = voff[n];
-      if (!whole) off -= static_cast<uint32_t>(max(first + row[n] - last, 0) * stride_t * 2);
-      dma16(off, base, img + static_cast<uint32_t>((wave * N + n) * 1024));
+      for (int n = 0; n < N; ++n) dma16(voff[n], base, to + 1024 * n);
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int id = 64 * (wave * N + n) + lane, behind = first + id / CH - last;
+        dma16(voff[n] - static_cast<uint32_t>(max(behind, 0) * stride_t * 2), base, to + 1024 * n);
+      }
     }
   }
 };
+
+// visit(i, buffer) for i from i0 to i1, the two buffers in turn: constants, so that LDS addresses need no arithmetic per tile.
+template <typename F>
+__device__ __forceinline__ void in_turn(int i0, int i1, const F& visit) {
+  for (int i = i0; i < i1; i += 2) {
+    visit(i, std::integral_constant<int, 0>{});
+    if (i + 1 < i1) visit(i + 1, std::integral_constant<int, 1>{});
+  }
+}
 
 // The transfers of the next tile have landed for the whole block, and its reads of the tile before are done.
 __device__ __forceinline__ void next_tile() {
@@ -182,23 +194,23 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_ker
   const int count = end > q0 ? tiles.count : 0;
   const TileLoader<T, D> ldk(a.k.st, wave, lane), ldv(a.v.st, wave, lane);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw)));
-  auto start = [&](int i) {
+  auto start = [&](int i, int buffer) {
     const int row = tiles[i] * FA_TILE;
-    const uint32_t to = lds0 + static_cast<uint32_t>(i & 1) * 2 * IMG;
+    const uint32_t to = lds0 + static_cast<uint32_t>(buffer) * 2 * IMG;
     ldk.start(kb, a.k.st, row, n - 1, to);
     ldv.start(vb, a.v.st, row, n - 1, to + IMG);
   };
-  if (count > 0) start(0);
+  if (count > 0) start(0, 0);
   const int first = qw, last = qw + 31;                         // the wavefront's queries
   const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
   constexpr uint32_t ONES = elem<T>::dtype == NMTG_BF16 ? 0x3f803f80u : 0x3c003c00u;
-  for (int i = 0; i < count; ++i) {
+  const auto visit = [&](int i, auto buffer) __attribute__((always_inline)) {
     const int k0 = tiles[i] * FA_TILE;
     next_tile();
-    if (i + 1 < count) start(i + 1);
-    const uint8_t* kimg = lds_raw + (i & 1) * 2 * IMG;
+    if (i + 1 < count) start(i + 1, 1 - buffer);
+    const uint8_t* kimg = lds_raw + buffer * (2 * IMG);
     const uint8_t* vimg = kimg + IMG;
-    if (nothing_seen(a, n, first, last, k0)) continue;
+    if (nothing_seen(a, n, first, last, k0)) return;
     acc16_t s[2];
 #pragma unroll
     for (int nn = 0; nn < 2; ++nn)
@@ -254,7 +266,8 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_ker
     for (int kk = 0; kk < FA_TILE / 16; ++kk)
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) mfma<T>::run(img_columns<D>(vimg, j, kk, lane), pf[kk], o[j]);
-  }
+  };
+  in_turn(0, count, visit);
   __syncthreads();                                              // every wavefront is done with the images
   const float sum = pair_sum(l);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -279,9 +292,9 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_
   const int count = end > q0 ? tiles.count : 0;
   const TileLoader<T, D> ldk(a.k.st, wave, lane), ldv(a.v.st, wave, lane);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw)));
-  auto start = [&](int i) {
+  auto start = [&](int i, int buffer) {
     const int row = tiles[i] * FA_TILE;
-    const uint32_t to = lds0 + static_cast<uint32_t>(i & 1) * 2 * IMG;
+    const uint32_t to = lds0 + static_cast<uint32_t>(buffer) * 2 * IMG;
     ldk.start(kb, a.k.st, row, n - 1, to);
     ldv.start(vb, a.v.st, row, n - 1, to + IMG);
   };
@@ -311,16 +324,16 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
   registers_landed(qf);
-  if (count > 0) start(0);
+  if (count > 0) start(0, 0);
   const int first = qw, last = qw + 31;
   const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
-  for (int i = 0; i < count; ++i) {
+  const auto visit = [&](int i, auto buffer) __attribute__((always_inline)) {
     const int k0 = tiles[i] * FA_TILE;
     next_tile();
-    if (i + 1 < count) start(i + 1);
-    const uint8_t* kimg = lds_raw + (i & 1) * 2 * IMG;
+    if (i + 1 < count) start(i + 1, 1 - buffer);
+    const uint8_t* kimg = lds_raw + buffer * (2 * IMG);
     const uint8_t* vimg = kimg + IMG;
-    if (nothing_seen(a, n, first, last, k0)) continue;
+    if (nothing_seen(a, n, first, last, k0)) return;
     const bool edge = some_hidden(a, n, first, last, k0);
     // 32 keys at a time, so that scores, score gradients and their operands need half the registers
 #pragma unroll
@@ -346,7 +359,8 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_
         for (int j = 0; j < D / 32; ++j) mfma<T>::run(img_columns<D>(kimg, j, 2 * nn + kk, lane), df, dq[j]);
       }
     }
-  }
+  };
+  in_turn(0, count, visit);
   __syncthreads();
   store_rows_out<T, D>(dq, a.scale, lds_raw + wave * (32 * D * 2), out_head<T>(a.dq, b, h), a.dq.st, qw, a.len, lane);
 }
@@ -435,15 +449,15 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
     if (tid < 2 * TILE) reinterpret_cast<float*>(buf + 2 * IMG)[tid] = tid < TILE ? (st_raw == -INFINITY ? -FA_NEG : st_raw * FA_LOG2E) : st_raw;
   };
   if (i0 < i1) {
-    start(i0, lds0 + (i0 & 1) * BUF);
-    store_stats(lds_raw + (i0 & 1) * BUF);
+    start(i0, lds0);
+    store_stats(lds_raw);
   }
-  for (int i = i0; i < i1; ++i) {
+  const auto visit = [&](int i, auto buffer) __attribute__((always_inline)) {
     const int q0 = (t0 + i % per) * TILE;
     wait_vmcnt<0>();
     __syncthreads();
-    if (i + 1 < i1) start(i + 1, lds0 + ((i + 1) & 1) * BUF);
-    const uint8_t* qimg = lds_raw + (i & 1) * BUF;
+    if (i + 1 < i1) start(i + 1, lds0 + (1 - buffer) * BUF);
+    const uint8_t* qimg = lds_raw + buffer * BUF;
     const uint8_t* gimg = qimg + IMG;
     const float* stats = reinterpret_cast<const float*>(qimg + 2 * IMG);
     const int64_t klast = kw + 31;
@@ -507,8 +521,9 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
           }
       }
     }
-    if (i + 1 < i1) store_stats(lds_raw + ((i + 1) & 1) * BUF);
-  }
+    if (i + 1 < i1) store_stats(lds_raw + (1 - buffer) * BUF);
+  };
+  in_turn(i0, i1, visit);
   wait_vmcnt<0>();                                              // of a share without a tile: the keys' transfers
   const bool in_parts = sink_chunk || a.parts > 1 || k0 < a.sink_blocks * WA_ROWS;
   if (in_parts) {
