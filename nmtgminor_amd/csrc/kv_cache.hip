@@ -18,9 +18,8 @@ namespace {
 
 constexpr int KV_BLOCK = 32;      // elements per scale
 constexpr int KV_TILE = 32;       // positions per step of a wavefront in the attention kernel
-constexpr int KV_WAVES = 4;
 constexpr int KV_ROWS = 16;       // query rows per block: the columns of the 16 x 16 x 32 products
-constexpr float KV_NEG = -1e30f;
+constexpr float KV_FLOOR = -5e29f;  // a running maximum before the first visible position: finite, far above the -inf of hidden ones
 constexpr float KV_LAZY = 8.f;
 constexpr float KV_LOG2E = 1.4426950408889634f;
 
@@ -59,114 +58,137 @@ __device__ __forceinline__ void held_word(uint32_t word, float scale, uint32_t* 
 }
 
 // ------------------------------------------------------------------------------------------------------- write and read
+// A block takes a tile of 16-bit rows: 2^tshift neighbouring positions of as many (sequence, head) pairs as 128 (head_dim 64) or
+// 64 rows make. In the 16-bit tensors neighbouring pairs lie side by side, in the cache neighbouring positions do: with 8 or 16
+// positions a tile is read and written in pieces of at least 256 bytes on both sides. (One row after the other in the order of the
+// 16-bit tensors left the cache side with pieces of 32 or 64 bytes, half of a line, and took half of the time for 64-bit divisions: ROWTIME)
 struct KvRows {
   const void *k, *v;              // write: 16-bit rows [count, batch, kv_heads, head_dim] by three strides
   void *k_out, *v_out;            // read: dense [count, batch, kv_heads, head_dim]
   uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
   const int32_t* starts;          // first cache row of every sequence, or null: `start` for all
   int64_t k_st, k_sb, k_sh, v_st, v_sb, v_sh;
-  int64_t start, count, capacity, total;   // total: count * batch * kv_heads * (head_dim / 8)
-  int batch, kv_heads;
+  int64_t start, capacity;
+  int count, batch, kv_heads, tshift, pair_tiles;
 };
 
-// Item i of a call: 8 elements c of row (t, b, h), counted in the order of the 16-bit rows.
-struct KvItem { int64_t t; int b, h, c; int64_t row; bool live; };
-template <int D>
-__device__ __forceinline__ KvItem kv_item(const KvRows& a, int64_t i) {
-  constexpr int CH = D / 8;
-  KvItem r;
-  r.c = static_cast<int>(i % CH);
-  const int64_t rest = i / CH, bh = rest % (static_cast<int64_t>(a.batch) * a.kv_heads);
-  r.t = rest / (static_cast<int64_t>(a.batch) * a.kv_heads);
-  r.h = static_cast<int>(bh % a.kv_heads);
-  r.b = static_cast<int>(bh / a.kv_heads);
-  const int64_t at = (a.starts != nullptr ? a.starts[r.b] : a.start) + r.t;
-  r.live = at >= 0 && at < a.capacity;
-  r.row = (static_cast<int64_t>(r.b) * a.kv_heads + r.h) * a.capacity + at;
+template <int D> struct RowTile {
+  static constexpr int CH = D / 8, STEP = 256 / CH, PASSES = 4, ROWS = STEP * PASSES;   // rows per pass of the block, rows per tile
+};
+// Row `row` of the block's tile. held: its cache row, or -1 where `starts` puts it outside.
+struct KvRow { int t, b, h; int64_t held; bool live; };
+__device__ __forceinline__ KvRow kv_row(const KvRows& a, uint32_t tile, int rows, int row) {
+  KvRow r;
+  const int t_tile = static_cast<int>(tile / static_cast<uint32_t>(a.pair_tiles)), p_tile = static_cast<int>(tile % static_cast<uint32_t>(a.pair_tiles));
+  r.t = (t_tile << a.tshift) + (row & ((1 << a.tshift) - 1));
+  const uint32_t pair = static_cast<uint32_t>(p_tile) * static_cast<uint32_t>(rows >> a.tshift) + static_cast<uint32_t>(row >> a.tshift);
+  r.live = r.t < a.count && pair < static_cast<uint32_t>(a.batch) * static_cast<uint32_t>(a.kv_heads);
+  r.b = static_cast<int>(pair / static_cast<uint32_t>(a.kv_heads));
+  r.h = static_cast<int>(pair) - r.b * a.kv_heads;
+  const int64_t at = (a.starts != nullptr && r.live ? a.starts[r.b] : a.start) + r.t;
+  r.held = at >= 0 && at < a.capacity ? static_cast<int64_t>(pair) * a.capacity + at : -1;
   return r;
 }
 
 // One lane per 8 elements, four neighbouring lanes per block of 32; blockIdx.y: keys or values.
 template <typename T, int D, int BITS>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvRows a) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= a.total) return;                   // total is a multiple of 8: whole blocks of four lanes leave together
+  using R = RowTile<D>;
   const bool keys = blockIdx.y == 0;
-  const KvItem it = kv_item<D>(a, i);
-  if (!it.live) return;                       // the four lanes of a block share a row
-  const T* src = static_cast<const T*>(keys ? a.k : a.v) + it.t * (keys ? a.k_st : a.v_st) + it.b * (keys ? a.k_sb : a.v_sb) +
-                 it.h * (keys ? a.k_sh : a.v_sh) + 8 * it.c;
-  const pack<T, 8> raw = load_raw<T, 8>(src);
-  uint32_t w[4];
-  __builtin_memcpy(w, &raw, 16);
-  // magnitudes of 16-bit floats compare as integers
-  uint32_t top = 0;
+  const T* src = static_cast<const T*>(keys ? a.k : a.v);
+  const int64_t st = keys ? a.k_st : a.v_st, sb = keys ? a.k_sb : a.v_sb, sh = keys ? a.k_sh : a.v_sh;
+  const int c = static_cast<int>(threadIdx.x) % R::CH;
+  int64_t held[R::PASSES];
+  uint32_t w[R::PASSES][4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
-  top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0xB1, 0xf, 0xf, true)));
-  top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x4E, 0xf, 0xf, true)));
-  const bool finite = top < (elem<T>::dtype == NMTG_BF16 ? 0x7f80u : 0x7c00u);
-  T largest;
-  largest.bits = static_cast<uint16_t>(top);
-  const uint32_t amax = __float_as_uint(elem<T>::to_float(largest));
-  constexpr int EMAX = BITS == 4 ? 2 : 8;
-  constexpr uint32_t UP = BITS == 4 ? 0x600000u : 0x680000u;      // fraction of 1.75 (7 / 4) and of 1.8125 (464 / 256)
-  const int byte = finite ? max(1, static_cast<int>(amax >> 23) - EMAX + ((amax & 0x7fffffu) > UP ? 1 : 0)) : 255;
-  const float scale = scale_of(static_cast<uint32_t>(finite ? byte : 127));
-  uint8_t* codes = (keys ? a.k_codes : a.v_codes) + it.row * (D * BITS / 8) + it.c * BITS;
-  if constexpr (BITS == 4) {
-    uint32_t out = 0;
-    if constexpr (elem<T>::dtype == NMTG_BF16) {
-      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(out, __builtin_bit_cast(bf16x2_t, w[0]), scale, 0);
-      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(out, __builtin_bit_cast(bf16x2_t, w[1]), scale, 1);
-      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(out, __builtin_bit_cast(bf16x2_t, w[2]), scale, 2);
-      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(out, __builtin_bit_cast(bf16x2_t, w[3]), scale, 3);
-    } else {
-      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[0]), scale, 0);
-      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[1]), scale, 1);
-      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[2]), scale, 2);
-      out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[3]), scale, 3);
-    }
-    *reinterpret_cast<uint32_t*>(codes) = finite ? out : 0u;
-  } else {
-    s16x2_t out[2] = {{0, 0}, {0, 0}};
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if constexpr (elem<T>::dtype == NMTG_BF16) {
-        out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(out[e], __builtin_bit_cast(bf16x2_t, w[2 * e]), scale, false);
-        out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(out[e], __builtin_bit_cast(bf16x2_t, w[2 * e + 1]), scale, true);
-      } else {
-        out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(out[e], __builtin_bit_cast(f16x2_t, w[2 * e]), scale, false);
-        out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(out[e], __builtin_bit_cast(f16x2_t, w[2 * e + 1]), scale, true);
-      }
-    }
-    uint2 two = make_uint2(__builtin_bit_cast(uint32_t, out[0]), __builtin_bit_cast(uint32_t, out[1]));
-    *reinterpret_cast<uint2*>(codes) = finite ? two : make_uint2(0, 0);
+  for (int i = 0; i < R::PASSES; ++i) {            // all loads on their way before the first is looked at
+    const KvRow r = kv_row(a, blockIdx.x, R::ROWS, i * R::STEP + static_cast<int>(threadIdx.x) / R::CH);
+    held[i] = r.live ? r.held : -1;
+    pack<T, 8> raw = {};
+    if (held[i] >= 0) raw = load_raw<T, 8>(src + r.t * st + r.b * sb + r.h * sh + 8 * c);
+    __builtin_memcpy(w[i], &raw, 16);
   }
-  if ((it.c & 3) == 0) (keys ? a.k_scales : a.v_scales)[it.row * (D / KV_BLOCK) + it.c / 4] = static_cast<uint8_t>(byte);
+#pragma unroll
+  for (int i = 0; i < R::PASSES; ++i) {
+    // magnitudes of 16-bit floats compare as integers
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max(top, max(w[i][e] & 0x7fffu, (w[i][e] >> 16) & 0x7fffu));
+    top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0xB1, 0xf, 0xf, true)));
+    top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x4E, 0xf, 0xf, true)));
+    if (held[i] < 0) continue;                     // the four lanes of a block share a row
+    const bool finite = top < (elem<T>::dtype == NMTG_BF16 ? 0x7f80u : 0x7c00u);
+    T largest;
+    largest.bits = static_cast<uint16_t>(top);
+    const uint32_t amax = __float_as_uint(elem<T>::to_float(largest));
+    constexpr int EMAX = BITS == 4 ? 2 : 8;
+    constexpr uint32_t UP = BITS == 4 ? 0x600000u : 0x680000u;      // fraction of 1.75 (7 / 4) and of 1.8125 (464 / 256)
+    const int byte = finite ? max(1, static_cast<int>(amax >> 23) - EMAX + ((amax & 0x7fffffu) > UP ? 1 : 0)) : 255;
+    const float scale = scale_of(static_cast<uint32_t>(finite ? byte : 127));
+    uint8_t* codes = (keys ? a.k_codes : a.v_codes) + held[i] * (D * BITS / 8) + c * BITS;
+    if constexpr (BITS == 4) {
+      uint32_t out = 0;
+      if constexpr (elem<T>::dtype == NMTG_BF16) {
+        out = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(out, __builtin_bit_cast(bf16x2_t, w[i][0]), scale, 0);
+        out = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(out, __builtin_bit_cast(bf16x2_t, w[i][1]), scale, 1);
+        out = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(out, __builtin_bit_cast(bf16x2_t, w[i][2]), scale, 2);
+        out = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(out, __builtin_bit_cast(bf16x2_t, w[i][3]), scale, 3);
+      } else {
+        out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[i][0]), scale, 0);
+        out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[i][1]), scale, 1);
+        out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[i][2]), scale, 2);
+        out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[i][3]), scale, 3);
+      }
+      *reinterpret_cast<uint32_t*>(codes) = finite ? out : 0u;
+    } else {
+      s16x2_t out[2] = {{0, 0}, {0, 0}};
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if constexpr (elem<T>::dtype == NMTG_BF16) {
+          out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(out[e], __builtin_bit_cast(bf16x2_t, w[i][2 * e]), scale, false);
+          out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(out[e], __builtin_bit_cast(bf16x2_t, w[i][2 * e + 1]), scale, true);
+        } else {
+          out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(out[e], __builtin_bit_cast(f16x2_t, w[i][2 * e]), scale, false);
+          out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(out[e], __builtin_bit_cast(f16x2_t, w[i][2 * e + 1]), scale, true);
+        }
+      }
+      uint2 two = make_uint2(__builtin_bit_cast(uint32_t, out[0]), __builtin_bit_cast(uint32_t, out[1]));
+      *reinterpret_cast<uint2*>(codes) = finite ? two : make_uint2(0, 0);
+    }
+    if ((c & 3) == 0) (keys ? a.k_scales : a.v_scales)[held[i] * (D / KV_BLOCK) + c / 4] = static_cast<uint8_t>(byte);
+  }
 }
 
 template <typename T, int D, int BITS>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvRows a) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= a.total) return;
+  using R = RowTile<D>;
   const bool keys = blockIdx.y == 0;
-  const KvItem it = kv_item<D>(a, i);
-  uint4 out = make_uint4(0, 0, 0, 0);
-  if (it.live) {
-    const uint8_t* codes = (keys ? a.k_codes : a.v_codes) + it.row * (D * BITS / 8) + it.c * BITS;
-    const float scale = scale_of((keys ? a.k_scales : a.v_scales)[it.row * (D / KV_BLOCK) + it.c / 4]);
-    uint32_t w[4];
-    if constexpr (BITS == 4) {
-      held_word<T, 4>(*reinterpret_cast<const uint32_t*>(codes), scale, w);
-    } else {
-      const uint2 two = *reinterpret_cast<const uint2*>(codes);
-      held_word<T, 8>(two.x, scale, w);
-      held_word<T, 8>(two.y, scale, w + 2);
+  const uint8_t *kc = keys ? a.k_codes : a.v_codes, *ksc = keys ? a.k_scales : a.v_scales;
+  const int c = static_cast<int>(threadIdx.x) % R::CH;
+  int64_t to[R::PASSES];
+  uint2 raw[R::PASSES];
+  uint32_t byte[R::PASSES];
+#pragma unroll
+  for (int i = 0; i < R::PASSES; ++i) {
+    const KvRow r = kv_row(a, blockIdx.x, R::ROWS, i * R::STEP + static_cast<int>(threadIdx.x) / R::CH);
+    to[i] = r.live ? (static_cast<int64_t>(r.t) * a.batch + r.b) * a.kv_heads + r.h : -1;
+    raw[i] = make_uint2(0, 0);                     // positions outside the cache: zeros
+    byte[i] = 127;
+    if (r.live && r.held >= 0) {
+      const uint8_t* codes = kc + r.held * (D * BITS / 8) + c * BITS;
+      if constexpr (BITS == 4) raw[i].x = *reinterpret_cast<const uint32_t*>(codes);
+      else raw[i] = *reinterpret_cast<const uint2*>(codes);
+      byte[i] = ksc[r.held * (D / KV_BLOCK) + c / 4];
     }
-    out = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  static_cast<uint4*>(keys ? a.k_out : a.v_out)[i] = out;
+#pragma unroll
+  for (int i = 0; i < R::PASSES; ++i) {
+    if (to[i] < 0) continue;
+    uint32_t w[4];
+    held_word<T, BITS>(raw[i].x, scale_of(byte[i]), w);
+    if constexpr (BITS == 8) held_word<T, BITS>(raw[i].y, scale_of(byte[i]), w + 2);
+    static_cast<uint4*>(keys ? a.k_out : a.v_out)[to[i] * R::CH + c] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------ attention
@@ -191,8 +213,7 @@ struct KvAttn {
   int64_t q_st, q_sb, q_sh, o_st, o_sb, o_sh;
   int64_t capacity;
   int tq, heads, kv_heads, group, rows, splits;   // group: query heads per key / value head, rows: tq * group
-  int64_t window;                 // 0: none
-  int64_t sinks;
+  int window, sinks;              // window beyond every position: none
   float scale_log2;
 };
 
@@ -218,60 +239,90 @@ __device__ __forceinline__ uint32_t round_pair(float lo, float hi) {
 // The codes and scales of one tile in a lane's registers.
 template <int D, int BITS>
 struct KvTile {
-  static constexpr int KW = D * BITS / 8 / 4 / 4;    // words of a quarter row
-  static constexpr int VW = D * BITS / 8 / 16 >= 4 ? D * BITS / 8 / 16 / 4 : 1;   // words of a sixteenth of a row
-  static constexpr int VB = D * BITS / 8 / 16;       // its bytes (2, 4 or 8)
+  static constexpr int RB = D * BITS / 8, SB = D / KV_BLOCK;        // bytes of a row's codes and scales
+  static constexpr int KW = RB / 16;                                // words of a quarter row
+  static constexpr int VB = RB / 16, VW = VB >= 4 ? VB / 4 : 1;     // bytes of a sixteenth of a row, words to hold them
   uint32_t k[2][KW], ks[2], v[8][VW], vs[8];
-  // position: the tile's first; limit: the last row that may be read
+  // the tile's rows start at row `position` of the head's rows; `rows` of its 32 may be read, the others repeat the last of them
   __device__ __forceinline__ void load(const uint8_t* kc, const uint8_t* ksc, const uint8_t* vc, const uint8_t* vsc, int64_t position,
-                                       int64_t limit, int lane) {
-    constexpr int RB = D * BITS / 8, SB = D / KV_BLOCK;
+                                       int64_t rows, int lane) {
+    const uint8_t *kp = kc + position * RB, *ksp = ksc + position * SB, *vp = vc + position * RB, *vsp = vsc + position * SB;
     const int r = lane & 15, g = lane >> 4;
+    if (rows >= KV_TILE) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const int64_t row = least(position + 16 * m + r, limit);
-      __builtin_memcpy(k[m], __builtin_assume_aligned(kc + row * RB + g * (RB / 4), RB / 4 >= 16 ? 16 : RB / 4), 4 * KW);
-      ks[m] = ksc[row * SB + g * SB / 4];
-    }
+      for (int m = 0; m < 2; ++m) load_k(m, kp, ksp, static_cast<uint32_t>(16 * m + r), g);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int64_t row = least(position + 16 * (e / 4) + 4 * g + (e & 3), limit);
-      const uint8_t* p = vc + row * RB + r * VB;
-      if constexpr (VB == 2) v[e][0] = *reinterpret_cast<const uint16_t*>(p);
-      else __builtin_memcpy(v[e], __builtin_assume_aligned(p, VB), VB);
-      vs[e] = vsc[row * SB + r * SB / 16];
+      for (int e = 0; e < 8; ++e) load_v(e, vp, static_cast<uint32_t>(16 * (e / 4) + 4 * g + (e & 3)), r);
+      // the scales of four neighbouring positions in one load, the lane's block shifted down
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const uint8_t* p = vsp + static_cast<uint32_t>((16 * m + 4 * g) * SB);
+        if constexpr (SB == 4) {
+          typedef uint32_t words __attribute__((ext_vector_type(4), aligned(4)));
+          const words w = *reinterpret_cast<const words*>(p);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vs[4 * m + e] = w[e];
+        } else {
+          typedef uint32_t words __attribute__((ext_vector_type(2), aligned(2)));
+          const words w = *reinterpret_cast<const words*>(p);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vs[4 * m + e] = w[e / 2] >> (16 * (e & 1));   // (its lower half counts)
+        }
+      }
+    } else {
+      const uint32_t last = static_cast<uint32_t>(rows - 1);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) load_k(m, kp, ksp, min(static_cast<uint32_t>(16 * m + r), last), g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t row = min(static_cast<uint32_t>(16 * (e / 4) + 4 * g + (e & 3)), last);
+        load_v(e, vp, row, r);
+        if constexpr (SB == 4) vs[e] = *reinterpret_cast<const uint32_t*>(vsp + row * SB);
+        else vs[e] = *reinterpret_cast<const uint16_t*>(vsp + row * SB);
+      }
     }
   }
+  __device__ __forceinline__ void load_k(int m, const uint8_t* kp, const uint8_t* ksp, uint32_t row, int g) {
+    __builtin_memcpy(k[m], __builtin_assume_aligned(kp + (row * RB + g * (RB / 4)), RB / 4 >= 16 ? 16 : RB / 4), 4 * KW);
+    ks[m] = ksp[row * SB + static_cast<uint32_t>(g) * SB / 4];
+  }
+  __device__ __forceinline__ void load_v(int e, const uint8_t* vp, uint32_t row, int r) {
+    const uint8_t* p = vp + (row * RB + r * VB);
+    if constexpr (VB == 2) v[e][0] = *reinterpret_cast<const uint16_t*>(p);
+    else __builtin_memcpy(v[e], __builtin_assume_aligned(p, VB), VB);
+  }
+  // scale of the lane's elements of position e: byte r SB / 16 of its scales
+  __device__ __forceinline__ float v_scale(int e, int r) const { return scale_of((vs[e] >> (8 * (r * SB / 16))) & 0xffu); }
 };
 
+// Wavefronts per block: 4 or 8, see attn_plan().
 template <typename T, int D, int BITS>
-__global__ __launch_bounds__(KV_WAVES * 64) void kv_attn_kernel(KvAttn a) {
+__global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
   constexpr int NK = D / 32, NV = D / 16;
-  constexpr int RB = D * BITS / 8, SB = D / KV_BLOCK;
-  __shared__ float lds_ml[KV_WAVES][KV_ROWS][2];
-  __shared__ float lds_o[KV_WAVES][KV_ROWS][D + 4];
-  const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
+  using Tile = KvTile<D, BITS>;
+  extern __shared__ __align__(16) float lds_attn[];                 // [waves][KV_ROWS][2] maximum and sum, [waves][rows][D + 4]
+  const int waves = static_cast<int>(blockDim.x) >> 6;
+  const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int r = lane & 15, g = lane >> 4;
   const int b = static_cast<int>(blockIdx.z), kvh = static_cast<int>(blockIdx.y) % a.kv_heads;
   const int row0 = static_cast<int>(blockIdx.y) / a.kv_heads * KV_ROWS, split = static_cast<int>(blockIdx.x);
   const int nrows = min(KV_ROWS, a.rows - row0);
-  const int64_t len = least(most(a.lengths[b], 0), a.capacity);
+  const int len = static_cast<int>(least(most(a.lengths[b], 0), a.capacity));
   // this lane's query row, its position, and the positions of the block's first and last row
   const int row = row0 + min(r, nrows - 1);
-  const int64_t qpos = len - a.tq + row / a.group;
-  const int64_t qfirst = len - a.tq + row0 / a.group, qlast = len - a.tq + (row0 + nrows - 1) / a.group;
-  const int64_t window = a.window > 0 ? a.window : a.capacity + 1;
+  const int qpos = len - a.tq + row / a.group;
+  const int qfirst = len - a.tq + row0 / a.group, qlast = len - a.tq + (row0 + nrows - 1) / a.group;
 
   // tiles of the sinks, then tiles from the first row's window on
-  const int64_t end = most(qlast + 1, 0), tiles_end = (end + KV_TILE - 1) / KV_TILE;
-  const int64_t lo = least(most(qfirst - window + 1, 0) / KV_TILE, tiles_end);
-  const int64_t ns = least((least(a.sinks, end) + KV_TILE - 1) / KV_TILE, lo);
-  const int64_t tiles = ns + tiles_end - lo;
-  const int64_t per = (tiles + a.splits - 1) / a.splits, t0 = least(split * per, tiles), t1 = least(t0 + per, tiles);
+  const int end = max(qlast + 1, 0), tiles_end = (end + KV_TILE - 1) / KV_TILE;
+  const int lo = min(max(qfirst - a.window + 1, 0) / KV_TILE, tiles_end);
+  const int ns = min((min(a.sinks, end) + KV_TILE - 1) / KV_TILE, lo);
+  const int tiles = ns + tiles_end - lo;
+  const int per = (tiles + a.splits - 1) / a.splits, t0 = min(split * per, tiles), t1 = min(t0 + per, tiles);
 
   const int64_t bh = static_cast<int64_t>(b) * a.kv_heads + kvh;
-  const uint8_t *kc = a.k_codes + bh * a.capacity * RB, *ksc = a.k_scales + bh * a.capacity * SB;
-  const uint8_t *vc = a.v_codes + bh * a.capacity * RB, *vsc = a.v_scales + bh * a.capacity * SB;
+  const uint8_t *kc = a.k_codes + bh * a.capacity * Tile::RB, *ksc = a.k_scales + bh * a.capacity * Tile::SB;
+  const uint8_t *vc = a.v_codes + bh * a.capacity * Tile::RB, *vsc = a.v_scales + bh * a.capacity * Tile::SB;
   uint4 qf[NK];
   {
     const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(row / a.group) * a.q_st + static_cast<int64_t>(b) * a.q_sb +
@@ -282,45 +333,44 @@ __global__ __launch_bounds__(KV_WAVES * 64) void kv_attn_kernel(KvAttn a) {
   f32x4_t o[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m = KV_NEG, l = 0.f;
+  float m = KV_FLOOR, l = 0.f;
 
-  KvTile<D, BITS> next;
-  int64_t t = t0 + wave;
-  auto position_of = [&](int64_t i) { return (i < ns ? i : i - ns + lo) * KV_TILE; };
-  if (t < t1) next.load(kc, ksc, vc, vsc, position_of(t), a.capacity - 1, lane);
-  for (; t < t1; t += KV_WAVES) {
-    const int64_t position = position_of(t);
-    KvTile<D, BITS> tile = next;
-    if (t + KV_WAVES < t1) next.load(kc, ksc, vc, vsc, position_of(t + KV_WAVES), a.capacity - 1, lane);
-    f32x4_t s[2];
+  Tile next;
+  auto fetch = [&](int i) {
+    const int64_t position = static_cast<int64_t>(i < ns ? i : i - ns + lo) * KV_TILE;
+    next.load(kc, ksc, vc, vsc, position, a.capacity - position, lane);
+  };
+  if (t0 + wave < t1) fetch(t0 + wave);
+  for (int t = t0 + wave; t < t1; t += waves) {
+    const int position = (t < ns ? t : t - ns + lo) * KV_TILE;
+    Tile tile = next;
+    if (t + waves < t1) fetch(t + waves);
+    float sc[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      s[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      f32x4_t s = {0.f, 0.f, 0.f, 0.f};
       const float scale = scale_of(tile.ks[h]);
       uint32_t kw[4 * NK];
 #pragma unroll
-      for (int w = 0; w < KvTile<D, BITS>::KW; ++w) held_word<T, BITS>(tile.k[h][w], scale, kw + w * (BITS == 4 ? 4 : 2));
+      for (int w = 0; w < Tile::KW; ++w) held_word<T, BITS>(tile.k[h][w], scale, kw + w * (BITS == 4 ? 4 : 2));
 #pragma unroll
-      for (int x = 0; x < NK; ++x) s[h] = mfma_16x16x32<T>(make_uint4(kw[4 * x], kw[4 * x + 1], kw[4 * x + 2], kw[4 * x + 3]), qf[x], s[h]);
+      for (int x = 0; x < NK; ++x) s = mfma_16x16x32<T>(make_uint4(kw[4 * x], kw[4 * x + 1], kw[4 * x + 2], kw[4 * x + 3]), qf[x], s);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[4 * h + e] = s[e] * a.scale_log2;
     }
     // positions that some row does not see: only where the tile crosses the newest positions or an edge of a window
-    const bool inside = position + KV_TILE - 1 <= qfirst && (position > qlast - window || position + KV_TILE <= a.sinks);
-    float sc[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sc[e] = s[e / 4][e & 3] * a.scale_log2;
-    uint32_t dead = 0;
-    if (!inside) {
+    if (position + KV_TILE - 1 > qfirst || (position <= qlast - a.window && position + KV_TILE > a.sinks)) {
+      const int first = position + 4 * g;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int64_t at = position + 16 * (e / 4) + 4 * g + (e & 3);
-        if (at > qpos || (at <= qpos - window && at >= a.sinks)) { dead |= 1u << e; sc[e] = KV_NEG; }
+        const int at = first + 16 * (e / 4) + (e & 3);
+        sc[e] = (at > qpos) | ((at <= qpos - a.window) & (at >= a.sinks)) ? -INFINITY : sc[e];
         // What no row of the block sees (rows behind the newest, not written yet, among it) must not meet its probability of
         // zero: an inf or NaN there would come through the product.
-        if (at > qlast || (at <= qfirst - window && at >= a.sinks)) {
+        const bool unseen = (at > qlast) | ((at <= qfirst - a.window) & (at >= a.sinks));
 #pragma unroll
-          for (int w = 0; w < KvTile<D, BITS>::VW; ++w) tile.v[e][w] = 0;
-          tile.vs[e] = 127;
-        }
+        for (int w = 0; w < Tile::VW; ++w) tile.v[e][w] = unseen ? 0u : tile.v[e][w];
+        tile.vs[e] = unseen ? 0x7f7f7f7fu : tile.vs[e];
       }
     }
     float top = sc[0];
@@ -338,28 +388,28 @@ __global__ __launch_bounds__(KV_WAVES * 64) void kv_attn_kernel(KvAttn a) {
     }
     float p[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      p[e] = fast_exp2(sc[e] - m);
-      if (!inside && ((dead >> e) & 1u) != 0) p[e] = 0.f;    // m may still be the initial one
-      l += p[e];
-    }
-    // probabilities rounded to the 16-bit type of the product (relative to a maximum at most 2^8 below the true one)
+    for (int e = 0; e < 8; ++e) p[e] = fast_exp2(sc[e] - m);
+    // Probabilities rounded to the 16-bit type of the product (relative to a maximum at most 2^8 below the true one); their sum is
+    // that of the rounded ones, so that the weights the values get add up to one.
     const uint4 pf = make_uint4(round_pair<T>(p[0], p[1]), round_pair<T>(p[2], p[3]), round_pair<T>(p[4], p[5]), round_pair<T>(p[6], p[7]));
+    constexpr uint32_t ONES = elem<T>::dtype == NMTG_BF16 ? 0x3f803f80u : 0x3c003c00u;
+    l = dot2<T>(pf.x, ONES, dot2<T>(pf.y, ONES, dot2<T>(pf.z, ONES, dot2<T>(pf.w, ONES, l))));
     // two positions at a time: pairs of neighbouring elements become pairs of neighbouring positions
     uint32_t vw[NV][4];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       uint32_t x[NV / 2], y[NV / 2];
-      if constexpr (KvTile<D, BITS>::VB == 2) {
-        x[0] = held_pair<T, BITS, 0>(tile.v[e][0], scale_of(tile.vs[e]));
-        x[1] = held_pair<T, BITS, 1>(tile.v[e][0], scale_of(tile.vs[e]));
-        y[0] = held_pair<T, BITS, 0>(tile.v[e + 1][0], scale_of(tile.vs[e + 1]));
-        y[1] = held_pair<T, BITS, 1>(tile.v[e + 1][0], scale_of(tile.vs[e + 1]));
+      const float sx = tile.v_scale(e, r), sy = tile.v_scale(e + 1, r);
+      if constexpr (Tile::VB == 2) {
+        x[0] = held_pair<T, BITS, 0>(tile.v[e][0], sx);
+        x[1] = held_pair<T, BITS, 1>(tile.v[e][0], sx);
+        y[0] = held_pair<T, BITS, 0>(tile.v[e + 1][0], sy);
+        y[1] = held_pair<T, BITS, 1>(tile.v[e + 1][0], sy);
       } else {
 #pragma unroll
-        for (int w = 0; w < KvTile<D, BITS>::VW; ++w) {
-          held_word<T, BITS>(tile.v[e][w], scale_of(tile.vs[e]), x + w * (BITS == 4 ? 4 : 2));
-          held_word<T, BITS>(tile.v[e + 1][w], scale_of(tile.vs[e + 1]), y + w * (BITS == 4 ? 4 : 2));
+        for (int w = 0; w < Tile::VW; ++w) {
+          held_word<T, BITS>(tile.v[e][w], sx, x + w * (BITS == 4 ? 4 : 2));
+          held_word<T, BITS>(tile.v[e + 1][w], sy, y + w * (BITS == 4 ? 4 : 2));
         }
       }
 #pragma unroll
@@ -375,23 +425,25 @@ __global__ __launch_bounds__(KV_WAVES * 64) void kv_attn_kernel(KvAttn a) {
   // the wavefronts' results: lane (r, g) holds elements (4 g + i) D / 16 + j of query row r in o[j][i]
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
-  if (g == 0) { lds_ml[wave][r][0] = m; lds_ml[wave][r][1] = l; }
+  float* lds_o = lds_attn + waves * KV_ROWS * 2;
+  if (g == 0) { lds_attn[(wave * KV_ROWS + r) * 2] = m; lds_attn[(wave * KV_ROWS + r) * 2 + 1] = l; }
+  if (r < nrows) {
+    float* to = lds_o + (wave * nrows + r) * (D + 4);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < NV; ++j) lds_o[wave][r][(4 * g + i) * NV + j] = o[j][i];
+      for (int j = 0; j < NV; ++j) to[(4 * g + i) * NV + j] = o[j][i];
+  }
   __syncthreads();
-  for (int i = static_cast<int>(threadIdx.x); i < nrows * D; i += KV_WAVES * 64) {
+  for (int i = static_cast<int>(threadIdx.x); i < nrows * D; i += static_cast<int>(blockDim.x)) {
     const int rr = i / D, d = i % D;
-    float top = lds_ml[0][rr][0];
-#pragma unroll
-    for (int w = 1; w < KV_WAVES; ++w) top = fmaxf(top, lds_ml[w][rr][0]);
+    float top = KV_FLOOR;
+    for (int w = 0; w < waves; ++w) top = fmaxf(top, lds_attn[(w * KV_ROWS + rr) * 2]);
     float sum = 0.f, val = 0.f;
-#pragma unroll
-    for (int w = 0; w < KV_WAVES; ++w) {
-      const float f = fast_exp2(lds_ml[w][rr][0] - top);
-      sum += f * lds_ml[w][rr][1];
-      val += f * lds_o[w][rr][d];
+    for (int w = 0; w < waves; ++w) {
+      const float f = fast_exp2(lds_attn[(w * KV_ROWS + rr) * 2] - top);
+      sum += f * lds_attn[(w * KV_ROWS + rr) * 2 + 1];
+      val += f * lds_o[(w * nrows + rr) * (D + 4) + d];
     }
     const int qrow = row0 + rr;
     if (a.splits == 1) {
@@ -411,7 +463,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(D) void kv_attn_join_kernel(KvAttn a, int64_t rows_all) {
   const int64_t at = blockIdx.x;
   const int d = static_cast<int>(threadIdx.x);
-  float top = KV_NEG;
+  float top = KV_FLOOR;
   for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[2 * (s * rows_all + at)]);
   float sum = 0.f, val = 0.f;
   for (int s = 0; s < a.splits; ++s) {
@@ -431,11 +483,27 @@ int check_format(const char* what, int64_t batch, int64_t kv_heads, int64_t head
   NMTG_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head dimension %lld (64 and 128 are built)", what, (long long)head_dim);
   NMTG_REQUIRE(bits == 4 || bits == 8, "%s: %d bits per element (4 and 8 are built)", what, bits);
   NMTG_REQUIRE(dtype == NMTG_F16 || dtype == NMTG_BF16, "%s: fp16 or bf16 tensors required", what);
-  NMTG_REQUIRE(batch <= 65535 && kv_heads <= 65535 && capacity < (1ll << 31), "%s: more than 65535 sequences or heads, or 2^31 positions", what);
+  NMTG_REQUIRE(batch <= 65535 && kv_heads <= 65535 && capacity < (1ll << 30), "%s: more than 65535 sequences or heads, or 2^30 positions", what);
   return 0;
 }
 bool rows_view_ok(const void* p, int64_t st, int64_t sb, int64_t sh) {
   return aligned16(p) && st % 8 == 0 && sb % 8 == 0 && sh % 8 == 0 && st >= 0 && sb >= 0 && sh >= 0;
+}
+
+// the tiles of a write or read: as many positions as there are, up to 8 (head_dim 128) or 16
+int row_tiles(const char* what, KvRows& a, const int32_t* starts, int64_t start, int64_t count, int64_t batch, int64_t kv_heads, int64_t capacity,
+              int64_t head_dim, dim3& grid) {
+  const int64_t rows = head_dim == 64 ? RowTile<64>::ROWS : RowTile<128>::ROWS;
+  a.starts = starts; a.start = start; a.capacity = capacity;
+  a.count = static_cast<int>(count); a.batch = static_cast<int>(batch); a.kv_heads = static_cast<int>(kv_heads);
+  a.tshift = 0;
+  while ((2 << a.tshift) <= (head_dim == 64 ? 16 : 8) && (1 << a.tshift) < count) ++a.tshift;
+  const int64_t pairs = batch * kv_heads, pairs_per = rows >> a.tshift, pair_tiles = (pairs + pairs_per - 1) / pairs_per;
+  const int64_t tiles = ((count + (1 << a.tshift) - 1) >> a.tshift) * pair_tiles;
+  NMTG_REQUIRE(pairs < (1ll << 31) && tiles <= 0x7fffffff, "%s: too many rows in one call", what);
+  a.pair_tiles = static_cast<int>(pair_tiles);
+  grid = dim3(static_cast<unsigned>(tiles), 2);
+  return 0;
 }
 
 #define KV_DISPATCH(head_dim, bits, dtype, GO)                                                        \
@@ -447,15 +515,27 @@ bool rows_view_ok(const void* p, int64_t st, int64_t sb, int64_t sh) {
     else { if (bits == 4) GO(bf16_t, 128, 4); else GO(bf16_t, 128, 8); }                              \
   }
 
-// How many blocks share a sequence's positions: enough that the call has four blocks for every compute unit, each with at
-// least two tiles for every wavefront.
-int attn_splits(int64_t tq, int64_t batch, int64_t heads, int64_t kv_heads, int64_t longest, int64_t window, int64_t sinks) {
+template <typename K>
+int attn_launch(K kern, dim3 grid, int waves, int lds, const KvAttn& a, hipStream_t st) {
+  if (lds > 64 * 1024) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return fail(NMTG_ERR_LAUNCH, "kv_cache_attn: cannot reserve %d bytes of LDS: %s", lds, hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL(kern, grid, dim3(64 * waves), lds, st, a);
+  return 0;
+}
+
+// How the positions of a sequence are shared out. Up to 2048 positions in reach one block of eight wavefronts takes them all: a second
+// launch to join parts costs as much as the tiles that more blocks would save (PLANTIME). Beyond, blocks of four
+// wavefronts, of which more fit a compute unit, share them: as many as give every compute unit four, each wavefront two tiles or more.
+struct AttnPlan { int waves, splits; };
+AttnPlan attn_plan(int64_t tq, int64_t batch, int64_t heads, int64_t kv_heads, int64_t longest, int64_t window, int64_t sinks) {
   const int64_t rows = tq * (heads / kv_heads), blocks = batch * kv_heads * ((rows + KV_ROWS - 1) / KV_ROWS);
   const int64_t reach = window > 0 ? std::min(longest, window + tq + sinks) : longest;
   const int64_t tiles = (reach + KV_TILE - 1) / KV_TILE;
-  int64_t splits = (4 * num_cus() + blocks - 1) / std::max<int64_t>(blocks, 1);
-  splits = std::min(splits, tiles / (2 * KV_WAVES));
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, 256)));
+  if (tiles <= 64) return {8, 1};
+  const int64_t splits = std::min((4 * num_cus() + blocks - 1) / std::max<int64_t>(blocks, 1), tiles / 8);
+  return {4, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, 256)))};
 }
 
 }  // namespace
@@ -479,15 +559,12 @@ extern "C" int nmtg_kv_cache_write(const void* k, int64_t k_stride_t, int64_t k_
   NMTG_REQUIRE(aligned16(k_codes) && aligned16(v_codes), "kv_cache_write: 16-byte aligned codes required");
   KvRows a = {};
   a.k = k; a.v = v; a.k_codes = k_codes; a.k_scales = k_scales; a.v_codes = v_codes; a.v_scales = v_scales;
-  a.starts = starts; a.start = start; a.count = count; a.capacity = capacity;
   a.k_st = k_stride_t; a.k_sb = k_stride_b; a.k_sh = k_stride_h; a.v_st = v_stride_t; a.v_sb = v_stride_b; a.v_sh = v_stride_h;
-  a.batch = static_cast<int>(batch); a.kv_heads = static_cast<int>(kv_heads);
-  a.total = count * batch * kv_heads * (head_dim / 8);
-  const int64_t blocks = (a.total + 255) / 256;
-  NMTG_REQUIRE(blocks <= 0x7fffffff, "kv_cache_write: too many rows in one call");
+  dim3 grid;
+  if (int rc = row_tiles("kv_cache_write", a, starts, start, count, batch, kv_heads, capacity, head_dim, grid)) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   TraceScope trace("kv_cache_write", st);
-#define GO(T, D, B) hipLaunchKernelGGL((kv_write_kernel<T, D, B>), dim3(static_cast<unsigned>(blocks), 2), dim3(256), 0, st, a)
+#define GO(T, D, B) hipLaunchKernelGGL((kv_write_kernel<T, D, B>), grid, dim3(256), 0, st, a)
   KV_DISPATCH(head_dim, bits, dtype, GO)
 #undef GO
   NMTG_CHECK_LAUNCH("kv_cache_write");
@@ -508,14 +585,11 @@ extern "C" int nmtg_kv_cache_read(const uint8_t* k_codes, const uint8_t* k_scale
   a.k_out = k; a.v_out = v;
   a.k_codes = const_cast<uint8_t*>(k_codes); a.k_scales = const_cast<uint8_t*>(k_scales);
   a.v_codes = const_cast<uint8_t*>(v_codes); a.v_scales = const_cast<uint8_t*>(v_scales);
-  a.starts = starts; a.start = start; a.count = count; a.capacity = capacity;
-  a.batch = static_cast<int>(batch); a.kv_heads = static_cast<int>(kv_heads);
-  a.total = count * batch * kv_heads * (head_dim / 8);
-  const int64_t blocks = (a.total + 255) / 256;
-  NMTG_REQUIRE(blocks <= 0x7fffffff, "kv_cache_read: too many rows in one call");
+  dim3 grid;
+  if (int rc = row_tiles("kv_cache_read", a, starts, start, count, batch, kv_heads, capacity, head_dim, grid)) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   TraceScope trace("kv_cache_read", st);
-#define GO(T, D, B) hipLaunchKernelGGL((kv_read_kernel<T, D, B>), dim3(static_cast<unsigned>(blocks), 2), dim3(256), 0, st, a)
+#define GO(T, D, B) hipLaunchKernelGGL((kv_read_kernel<T, D, B>), grid, dim3(256), 0, st, a)
   KV_DISPATCH(head_dim, bits, dtype, GO)
 #undef GO
   NMTG_CHECK_LAUNCH("kv_cache_read");
@@ -525,7 +599,7 @@ extern "C" int nmtg_kv_cache_read(const uint8_t* k_codes, const uint8_t* k_scale
 extern "C" int64_t nmtg_kv_cache_attn_workspace_bytes(int64_t tq, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t longest,
                                                       int64_t window, int64_t sinks) {
   if (tq <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0) return 0;
-  const int splits = attn_splits(tq, batch, heads, kv_heads, longest, window, sinks);
+  const int64_t splits = attn_plan(tq, batch, heads, kv_heads, longest, window, sinks).splits;
   return splits == 1 ? 0 : splits * tq * batch * heads * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
@@ -553,8 +627,12 @@ extern "C" int nmtg_kv_cache_attn(const void* q, int64_t q_stride_t, int64_t q_s
   a.q_st = q_stride_t; a.q_sb = q_stride_b; a.q_sh = q_stride_h; a.o_st = out_stride_t; a.o_sb = out_stride_b; a.o_sh = out_stride_h;
   a.capacity = capacity;
   a.tq = static_cast<int>(tq); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads); a.group = static_cast<int>(group);
-  a.rows = static_cast<int>(rows); a.window = window; a.sinks = window > 0 ? sinks : 0; a.scale_log2 = scale * KV_LOG2E;
-  a.splits = attn_splits(tq, batch, heads, kv_heads, longest, window, sinks);
+  a.rows = static_cast<int>(rows); a.scale_log2 = scale * KV_LOG2E;
+  // both fit 31 bits: nothing lies behind the capacity
+  a.window = static_cast<int>(window > 0 ? std::min(window, capacity + tq) : capacity + tq);
+  a.sinks = static_cast<int>(window > 0 ? std::min(sinks, capacity) : 0);
+  const AttnPlan plan = attn_plan(tq, batch, heads, kv_heads, longest, window, sinks);
+  a.splits = plan.splits;
   const int64_t rows_all = batch * kv_heads * rows;
   if (a.splits > 1) {
     const int64_t need = a.splits * rows_all * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
@@ -568,9 +646,12 @@ extern "C" int nmtg_kv_cache_attn(const void* q, int64_t q_stride_t, int64_t q_s
   const dim3 grid(static_cast<unsigned>(a.splits), static_cast<unsigned>(kv_heads * row_blocks), static_cast<unsigned>(batch));
   {
     TraceScope trace("kv_cache_attn", st);
-#define GO(T, D, B) hipLaunchKernelGGL((kv_attn_kernel<T, D, B>), grid, dim3(KV_WAVES * 64), 0, st, a)
+    const int lds = plan.waves * (KV_ROWS * 2 + static_cast<int>(std::min<int64_t>(rows, KV_ROWS) * (head_dim + 4))) * static_cast<int>(sizeof(float));
+    int launched = 0;
+#define GO(T, D, B) launched = attn_launch(kv_attn_kernel<T, D, B>, grid, plan.waves, lds, a, st)
     KV_DISPATCH(head_dim, bits, dtype, GO)
 #undef GO
+    if (launched) return launched;
   }
   if (a.splits > 1) {
     TraceScope trace("kv_cache_attn_join", st);
