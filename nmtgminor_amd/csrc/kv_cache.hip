@@ -26,6 +26,8 @@ constexpr float KV_LOG2E = 1.4426950408889634f;
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef short s16x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
@@ -61,7 +63,9 @@ __device__ __forceinline__ void held_word(uint32_t word, float scale, uint32_t* 
 // A block takes a tile of 16-bit rows: 2^tshift neighbouring positions of as many (sequence, head) pairs as 128 (head_dim 64) or
 // 64 rows make. In the 16-bit tensors neighbouring pairs lie side by side, in the cache neighbouring positions do: with 8 or 16
 // positions a tile is read and written in pieces of at least 256 bytes on both sides. (One row after the other in the order of the
-// 16-bit tensors left the cache side with pieces of 32 or 64 bytes, half of a line, and took half of the time for 64-bit divisions: ROWTIME)
+// 16-bit tensors left the cache side with pieces of 32 or 64 bytes, half of a line, and cost 64-bit divisions: 32768 positions of 4 x 8
+// heads of 128 in 4 bits read back in 220 us, now 113: 6.0 TB/s.) Rows, codes and results pass by
+// the L2, which they would only fill: writing 8192 positions of 8 x 8 heads 86 -> 68 us, 5.0 TB/s.
 struct KvRows {
   const void *k, *v;              // write: 16-bit rows [count, batch, kv_heads, head_dim] by three strides
   void *k_out, *v_out;            // read: dense [count, batch, kv_heads, head_dim]
@@ -104,9 +108,10 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvRows a) {
   for (int i = 0; i < R::PASSES; ++i) {            // all loads on their way before the first is looked at
     const KvRow r = kv_row(a, blockIdx.x, R::ROWS, i * R::STEP + static_cast<int>(threadIdx.x) / R::CH);
     held[i] = r.live ? r.held : -1;
-    pack<T, 8> raw = {};
-    if (held[i] >= 0) raw = load_raw<T, 8>(src + r.t * st + r.b * sb + r.h * sh + 8 * c);
-    __builtin_memcpy(w[i], &raw, 16);
+    u32x4_t raw = {0, 0, 0, 0};
+    if (held[i] >= 0) raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(src + r.t * st + r.b * sb + r.h * sh + 8 * c));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[i][e] = raw[e];
   }
 #pragma unroll
   for (int i = 0; i < R::PASSES; ++i) {
@@ -139,7 +144,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvRows a) {
         out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[i][2]), scale, 2);
         out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(out, __builtin_bit_cast(f16x2_t, w[i][3]), scale, 3);
       }
-      *reinterpret_cast<uint32_t*>(codes) = finite ? out : 0u;
+      __builtin_nontemporal_store(finite ? out : 0u, reinterpret_cast<uint32_t*>(codes));
     } else {
       s16x2_t out[2] = {{0, 0}, {0, 0}};
 #pragma unroll
@@ -152,8 +157,8 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvRows a) {
           out[e] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(out[e], __builtin_bit_cast(f16x2_t, w[i][2 * e + 1]), scale, true);
         }
       }
-      uint2 two = make_uint2(__builtin_bit_cast(uint32_t, out[0]), __builtin_bit_cast(uint32_t, out[1]));
-      *reinterpret_cast<uint2*>(codes) = finite ? two : make_uint2(0, 0);
+      const u32x2_t two = {finite ? __builtin_bit_cast(uint32_t, out[0]) : 0u, finite ? __builtin_bit_cast(uint32_t, out[1]) : 0u};
+      __builtin_nontemporal_store(two, reinterpret_cast<u32x2_t*>(codes));
     }
     if ((c & 3) == 0) (keys ? a.k_scales : a.v_scales)[held[i] * (D / KV_BLOCK) + c / 4] = static_cast<uint8_t>(byte);
   }
@@ -176,8 +181,12 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRows a) {
     byte[i] = 127;
     if (r.live && r.held >= 0) {
       const uint8_t* codes = kc + r.held * (D * BITS / 8) + c * BITS;
-      if constexpr (BITS == 4) raw[i].x = *reinterpret_cast<const uint32_t*>(codes);
-      else raw[i] = *reinterpret_cast<const uint2*>(codes);
+      if constexpr (BITS == 4) {
+        raw[i].x = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(codes));
+      } else {
+        const u32x2_t two = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(codes));
+        raw[i] = make_uint2(two[0], two[1]);
+      }
       byte[i] = ksc[r.held * (D / KV_BLOCK) + c / 4];
     }
   }
@@ -187,7 +196,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRows a) {
     uint32_t w[4];
     held_word<T, BITS>(raw[i].x, scale_of(byte[i]), w);
     if constexpr (BITS == 8) held_word<T, BITS>(raw[i].y, scale_of(byte[i]), w + 2);
-    static_cast<uint4*>(keys ? a.k_out : a.v_out)[to[i] * R::CH + c] = make_uint4(w[0], w[1], w[2], w[3]);
+    const u32x4_t row = {w[0], w[1], w[2], w[3]};
+    __builtin_nontemporal_store(row, static_cast<u32x4_t*>(keys ? a.k_out : a.v_out) + (to[i] * R::CH + c));
   }
 }
 
@@ -291,8 +301,11 @@ struct KvTile {
     if constexpr (VB == 2) v[e][0] = *reinterpret_cast<const uint16_t*>(p);
     else __builtin_memcpy(v[e], __builtin_assume_aligned(p, VB), VB);
   }
-  // scale of the lane's elements of position e: byte r SB / 16 of its scales
-  __device__ __forceinline__ float v_scale(int e, int r) const { return scale_of((vs[e] >> (8 * (r * SB / 16))) & 0xffu); }
+  // scale of the lane's elements of position e, byte r SB / 16 of its scales, rotated into the exponent's place. What else
+  // the word holds lands in sign and fraction, which the conversion instructions do not look at.
+  __device__ __forceinline__ float v_scale(int e, int r) const {
+    return __uint_as_float(__builtin_amdgcn_alignbit(vs[e], vs[e], static_cast<uint32_t>(8 * (r * SB / 16) + 9) & 31u));
+  }
 };
 
 // Wavefronts per block: 4 or 8, see attn_plan().
@@ -334,17 +347,16 @@ __global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m = KV_FLOOR, l = 0.f;
+  const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
 
-  Tile next;
-  auto fetch = [&](int i) {
-    const int64_t position = static_cast<int64_t>(i < ns ? i : i - ns + lo) * KV_TILE;
-    next.load(kc, ksc, vc, vsc, position, a.capacity - position, lane);
+  auto position_of = [&](int i) { return (i < ns ? i : i - ns + lo) * KV_TILE; };
+  auto fetch = [&](Tile& to, int i) {
+    const int64_t position = position_of(i);
+    to.load(kc, ksc, vc, vsc, position, a.capacity - position, lane);
   };
-  if (t0 + wave < t1) fetch(t0 + wave);
-  for (int t = t0 + wave; t < t1; t += waves) {
-    const int position = (t < ns ? t : t - ns + lo) * KV_TILE;
-    Tile tile = next;
-    if (t + waves < t1) fetch(t + waves);
+  const auto visit = [&](int t, Tile& tile, Tile& next) __attribute__((always_inline)) {
+    const int position = position_of(t);
+    if (t + waves < t1) fetch(next, t + waves);
     float sc[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -356,7 +368,7 @@ __global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
 #pragma unroll
       for (int x = 0; x < NK; ++x) s = mfma_16x16x32<T>(make_uint4(kw[4 * x], kw[4 * x + 1], kw[4 * x + 2], kw[4 * x + 3]), qf[x], s);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sc[4 * h + e] = s[e] * a.scale_log2;
+      for (int e = 0; e < 4; ++e) sc[4 * h + e] = s[e];
     }
     // positions that some row does not see: only where the tile crosses the newest positions or an edge of a window
     if (position + KV_TILE - 1 > qfirst || (position <= qlast - a.window && position + KV_TILE > a.sinks)) {
@@ -364,7 +376,7 @@ __global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int at = first + 16 * (e / 4) + (e & 3);
-        sc[e] = (at > qpos) | ((at <= qpos - a.window) & (at >= a.sinks)) ? -INFINITY : sc[e];
+        sc[e] = (at > qpos) | ((at <= qpos - a.window) & (at >= a.sinks)) ? hidden : sc[e];
         // What no row of the block sees (rows behind the newest, not written yet, among it) must not meet its probability of
         // zero: an inf or NaN there would come through the product.
         const bool unseen = (at > qlast) | ((at <= qfirst - a.window) & (at >= a.sinks));
@@ -374,8 +386,14 @@ __global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
       }
     }
     float top = sc[0];
+    if (a.scale_log2 >= 0.f) {
 #pragma unroll
-    for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[e]);
+      for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[e]);
+    } else {
+#pragma unroll
+      for (int e = 1; e < 8; ++e) top = fminf(top, sc[e]);
+    }
+    top *= a.scale_log2;
     if (__builtin_amdgcn_ballot_w64(top > m + KV_LAZY) != 0) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
@@ -388,7 +406,7 @@ __global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
     }
     float p[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = fast_exp2(sc[e] - m);
+    for (int e = 0; e < 8; ++e) p[e] = fast_exp2(__builtin_fmaf(sc[e], a.scale_log2, -m));
     // Probabilities rounded to the 16-bit type of the product (relative to a maximum at most 2^8 below the true one); their sum is
     // that of the rounded ones, so that the weights the values get add up to one.
     const uint4 pf = make_uint4(round_pair<T>(p[0], p[1]), round_pair<T>(p[2], p[3]), round_pair<T>(p[4], p[5]), round_pair<T>(p[6], p[7]));
@@ -420,6 +438,13 @@ __global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) o[j] = mfma_16x16x32<T>(make_uint4(vw[j][0], vw[j][1], vw[j][2], vw[j][3]), pf, o[j]);
+  };
+  // two sets of registers in turn, so that nothing is moved from one to the other
+  Tile even, odd;
+  if (t0 + wave < t1) fetch(even, t0 + wave);
+  for (int t = t0 + wave; t < t1; t += 2 * waves) {
+    visit(t, even, odd);
+    if (t + waves < t1) visit(t + waves, odd, even);
   }
 
   // the wavefronts' results: lane (r, g) holds elements (4 g + i) D / 16 + j of query row r in o[j][i]
@@ -627,7 +652,7 @@ extern "C" int nmtg_kv_cache_attn(const void* q, int64_t q_stride_t, int64_t q_s
   a.q_st = q_stride_t; a.q_sb = q_stride_b; a.q_sh = q_stride_h; a.o_st = out_stride_t; a.o_sb = out_stride_b; a.o_sh = out_stride_h;
   a.capacity = capacity;
   a.tq = static_cast<int>(tq); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads); a.group = static_cast<int>(group);
-  a.rows = static_cast<int>(rows); a.scale_log2 = scale * KV_LOG2E;
+  a.rows = static_cast<int>(rows); a.scale_log2 = scale == 0.f ? 1e-30f : scale * KV_LOG2E;   // (hidden scores are infinite, and stay so under a scale this small)
   // both fit 31 bits: nothing lies behind the capacity
   a.window = static_cast<int>(window > 0 ? std::min(window, capacity + tq) : capacity + tq);
   a.sinks = static_cast<int>(window > 0 ? std::min(sinks, capacity) : 0);
