@@ -246,8 +246,8 @@ __device__ __forceinline__ uint32_t round_pair(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, typename pair16<T>::type));
 }
 
-// The codes and scales of one tile in a lane's registers.
-template <int D, int BITS>
+// The codes and scales of one tile in a lane's registers. STREAM: the codes pass by the L2.
+template <int D, int BITS, bool STREAM>
 struct KvTile {
   static constexpr int RB = D * BITS / 8, SB = D / KV_BLOCK;        // bytes of a row's codes and scales
   static constexpr int KW = RB / 16;                                // words of a quarter row
@@ -293,13 +293,23 @@ struct KvTile {
     }
   }
   __device__ __forceinline__ void load_k(int m, const uint8_t* kp, const uint8_t* ksp, uint32_t row, int g) {
-    __builtin_memcpy(k[m], __builtin_assume_aligned(kp + (row * RB + g * (RB / 4)), RB / 4 >= 16 ? 16 : RB / 4), 4 * KW);
+    constexpr int N = KW >= 4 ? 4 : KW;
+#pragma unroll
+    for (int i = 0; i < KW; i += N) load_words<N>(k[m] + i, kp + (row * RB + g * (RB / 4)) + 4 * i);
     ks[m] = ksp[row * SB + static_cast<uint32_t>(g) * SB / 4];
   }
   __device__ __forceinline__ void load_v(int e, const uint8_t* vp, uint32_t row, int r) {
     const uint8_t* p = vp + (row * RB + r * VB);
     if constexpr (VB == 2) v[e][0] = *reinterpret_cast<const uint16_t*>(p);
-    else __builtin_memcpy(v[e], __builtin_assume_aligned(p, VB), VB);
+    else load_words<VW>(v[e], p);
+  }
+  template <int N>
+  static __device__ __forceinline__ void load_words(uint32_t* to, const uint8_t* p) {
+    typedef uint32_t words __attribute__((ext_vector_type(N)));
+    words w;
+    if constexpr (STREAM) w = __builtin_nontemporal_load(reinterpret_cast<const words*>(p));
+    else w = *reinterpret_cast<const words*>(p);
+    __builtin_memcpy(to, &w, 4 * N);
   }
   // scale of the lane's elements of position e, byte r SB / 16 of its scales, rotated into the exponent's place. What else
   // the word holds lands in sign and fraction, which the conversion instructions do not look at.
@@ -309,10 +319,10 @@ struct KvTile {
 };
 
 // Wavefronts per block: 4 or 8, see attn_plan().
-template <typename T, int D, int BITS>
+template <typename T, int D, int BITS, bool STREAM>
 __global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
   constexpr int NK = D / 32, NV = D / 16;
-  using Tile = KvTile<D, BITS>;
+  using Tile = KvTile<D, BITS, STREAM>;
   extern __shared__ __align__(16) float lds_attn[];                 // [waves][KV_ROWS][2] maximum and sum, [waves][rows][D + 4]
   const int waves = static_cast<int>(blockDim.x) >> 6;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -551,16 +561,19 @@ int attn_launch(K kern, dim3 grid, int waves, int lds, const KvAttn& a, hipStrea
 }
 
 // How the positions of a sequence are shared out. Up to 2048 positions in reach one block of eight wavefronts takes them all: a second
-// launch to join parts costs as much as the tiles that more blocks would save (PLANTIME). Beyond, blocks of four
-// wavefronts, of which more fit a compute unit, share them: as many as give every compute unit four, each wavefront two tiles or more.
-struct AttnPlan { int waves, splits; };
+// launch to join parts costs what more blocks would save (64 sequences of 1024 positions in reach, 4 heads of 64 in 8 bits: 17.1 us
+// with four blocks each, 9.7 with one). Beyond, blocks of four wavefronts share them, as many as give every compute unit
+// four, each wavefront two tiles or more; fewer leave ragged lengths unbalanced (32 sequences of 16384 to 32768 positions, 8 heads of
+// 128 in 4 bits: 154 us with four, 162 with two), more cost in the join. Such a reach does not stay in the caches from one step to the
+// next, and its codes pass by the L2 (144 us, 5.9 TB/s); a short one mostly does (9.7 us, 10.0 past the L2).
+struct AttnPlan { int waves, splits; bool stream; };
 AttnPlan attn_plan(int64_t tq, int64_t batch, int64_t heads, int64_t kv_heads, int64_t longest, int64_t window, int64_t sinks) {
   const int64_t rows = tq * (heads / kv_heads), blocks = batch * kv_heads * ((rows + KV_ROWS - 1) / KV_ROWS);
   const int64_t reach = window > 0 ? std::min(longest, window + tq + sinks) : longest;
   const int64_t tiles = (reach + KV_TILE - 1) / KV_TILE;
-  if (tiles <= 64) return {8, 1};
+  if (tiles <= 64) return {8, 1, false};
   const int64_t splits = std::min((4 * num_cus() + blocks - 1) / std::max<int64_t>(blocks, 1), tiles / 8);
-  return {4, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, 256)))};
+  return {4, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, 256))), true};
 }
 
 }  // namespace
@@ -673,7 +686,7 @@ extern "C" int nmtg_kv_cache_attn(const void* q, int64_t q_stride_t, int64_t q_s
     TraceScope trace("kv_cache_attn", st);
     const int lds = plan.waves * (KV_ROWS * 2 + static_cast<int>(std::min<int64_t>(rows, KV_ROWS) * (head_dim + 4))) * static_cast<int>(sizeof(float));
     int launched = 0;
-#define GO(T, D, B) launched = attn_launch(kv_attn_kernel<T, D, B>, grid, plan.waves, lds, a, st)
+#define GO(T, D, B) launched = plan.stream ? attn_launch(kv_attn_kernel<T, D, B, true>, grid, plan.waves, lds, a, st) : attn_launch(kv_attn_kernel<T, D, B, false>, grid, plan.waves, lds, a, st)
     KV_DISPATCH(head_dim, bits, dtype, GO)
 #undef GO
     if (launched) return launched;
