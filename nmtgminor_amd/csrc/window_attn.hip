@@ -42,7 +42,9 @@ struct WaView { const void* p; int64_t st, sb, sh; };   // [len, batch, heads, h
 
 struct WaArgs {
   WaView q, k, v, o, d_o, dq, dk, dv;
-  float *lse, *delta;        // [batch, heads, len]
+  float* lse;                // [batch, heads, len]
+  float* stats;              // backward: [batch, heads][2][stat_rows], log-sum-exp in units of log2 and D, rows up to a whole block
+  int stat_rows;
   const int32_t* lengths;    // [batch] or null: every sequence fills `len`
   int len, batch, heads, kv_heads, group;
   int64_t window, sinks;
@@ -88,6 +90,14 @@ __device__ __forceinline__ uint4 img_columns(const uint8_t* img, int i, int kk, 
   return cv.u;
 }
 
+// Lane l copies the 4 bytes at sbase + voff(l) to LDS address lds_addr + 4 l (dma16's sibling).
+__device__ __forceinline__ void dma4(uint32_t voff, const void* sbase, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+               :
+               : "v"(voff), "s"(sbase), "s"(lds_addr)
+               : "memory", "m0");
+}
+
 // Transfers of one tile of ROWS rows into an image, shared out over the block's wavefronts: lane l of transfer n fills chunk
 // 64 n + l. Rows behind `last` are read as row `last` (in bounds, finite where the sequence is; they are masked by the caller).
 template <typename T, int D, int ROWS = FA_TILE>
@@ -118,20 +128,24 @@ struct TileLoader {
   }
 };
 
-// visit(i, buffer) for i from i0 to i1, the two buffers in turn: constants, so that LDS addresses need no arithmetic per tile.
-template <typename F>
+// visit(i, buffer) for i from i0 to i1, the buffers in turn: constants, so that LDS addresses need no arithmetic per tile.
+template <int STAGES, typename F>
 __device__ __forceinline__ void in_turn(int i0, int i1, const F& visit) {
-  for (int i = i0; i < i1; i += 2) {
+  for (int i = i0; i < i1; i += STAGES) {
     visit(i, std::integral_constant<int, 0>{});
     if (i + 1 < i1) visit(i + 1, std::integral_constant<int, 1>{});
+    if constexpr (STAGES == 3) if (i + 2 < i1) visit(i + 2, std::integral_constant<int, 2>{});
   }
 }
 
-// The transfers of the next tile have landed for the whole block, and its reads of the tile before are done.
-__device__ __forceinline__ void next_tile() {
-  wait_vmcnt<0>();
+// Transfers run STAGES - 1 tiles ahead. The tile in front of `left` others has landed for the whole block, and the block's reads of
+// the tile before it are done (PT: a wavefront's transfers per tile).
+template <int STAGES, int PT>
+__device__ __forceinline__ void next_tile(int left) {
+  wait_vmcnt_upto<(STAGES - 2) * PT, PT>(min(left, STAGES - 2) * PT);
   ring_barrier();
 }
+template <int STAGES> constexpr int stage_before(int buffer) { return (buffer + STAGES - 1) % STAGES; }
 
 // the tiles of a block whose queries are first .. last: those of the sinks, then those from the first query's window on
 struct TileList {
@@ -173,7 +187,7 @@ constexpr float WA_FLOOR = -5e29f;   // a running maximum before the first visib
 template <typename T, int D>
 __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_kernel(WaArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
-  constexpr int IMG = FA_TILE * D * 2;
+  constexpr int IMG = FA_TILE * D * 2, STAGES = 2, PT = 2 * TileLoader<T, D>::N;
   const WaBlock block = query_block((a.len + WA_ROWS - 1) / WA_ROWS, a.group, a.kv_heads);
   const int b = block.b, h = block.h, q0 = block.x * WA_ROWS;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
@@ -200,14 +214,14 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_ker
     ldk.start(kb, a.k.st, row, n - 1, to);
     ldv.start(vb, a.v.st, row, n - 1, to + IMG);
   };
-  if (count > 0) start(0, 0);
+  for (int i = 0; i < STAGES - 1 && i < count; ++i) start(i, i);
   const int first = qw, last = qw + 31;                         // the wavefront's queries
   const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
   constexpr uint32_t ONES = elem<T>::dtype == NMTG_BF16 ? 0x3f803f80u : 0x3c003c00u;
   const auto visit = [&](int i, auto buffer) __attribute__((always_inline)) {
     const int k0 = tiles[i] * FA_TILE;
-    next_tile();
-    if (i + 1 < count) start(i + 1, 1 - buffer);
+    next_tile<STAGES, PT>(count - 1 - i);
+    if (i + STAGES - 1 < count) start(i + STAGES - 1, stage_before<STAGES>(buffer));
     const uint8_t* kimg = lds_raw + buffer * (2 * IMG);
     const uint8_t* vimg = kimg + IMG;
     if (nothing_seen(a, n, first, last, k0)) return;
@@ -251,23 +265,20 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_ker
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
     }
-    uint4 pf[FA_TILE / 16];
 #pragma unroll
     for (int kk = 0; kk < FA_TILE / 16; ++kk) {
       float pv[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) pv[e] = fast_exp2(__builtin_fmaf(s[kk / 2][8 * (kk % 2) + e], a.scale_log2, -m));
-      pf[kk] = acc_to_operand<T>(pv);
+      const uint4 pf = acc_to_operand<T>(pv);
       // The sum is that of the rounded probabilities: the weights that the values get add up to one, and two of them cost
       // one instruction.
-      l = dot2<T>(pf[kk].x, ONES, dot2<T>(pf[kk].y, ONES, dot2<T>(pf[kk].z, ONES, dot2<T>(pf[kk].w, ONES, l))));
+      l = dot2<T>(pf.x, ONES, dot2<T>(pf.y, ONES, dot2<T>(pf.z, ONES, dot2<T>(pf.w, ONES, l))));
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) mfma<T>::run(img_columns<D>(vimg, j, kk, lane), pf, o[j]);
     }
-#pragma unroll
-    for (int kk = 0; kk < FA_TILE / 16; ++kk)
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) mfma<T>::run(img_columns<D>(vimg, j, kk, lane), pf[kk], o[j]);
   };
-  in_turn(0, count, visit);
+  in_turn<STAGES>(0, count, visit);
   __syncthreads();                                              // every wavefront is done with the images
   const float sum = pair_sum(l);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -277,10 +288,12 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_ker
 }
 
 // ------------------------------------------------------------------------------------ backward: dQ, and D = rowsum(dO O)
+template <int D> constexpr int dq_stages() { return D == 64 ? 3 : 2; }
+
 template <typename T, int D>
 __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_kernel(WaArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
-  constexpr int IMG = FA_TILE * D * 2;
+  constexpr int IMG = FA_TILE * D * 2, STAGES = dq_stages<D>(), PT = 2 * TileLoader<T, D>::N;
   const WaBlock block = query_block((a.len + WA_ROWS - 1) / WA_ROWS, a.group, a.kv_heads);
   const int b = block.b, h = block.h, q0 = block.x * WA_ROWS;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
@@ -312,11 +325,13 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_
     }
     delta = pair_sum(delta);
     if (qrow < n) {
-      const int64_t at = static_cast<int64_t>(bh) * a.len + qrow;
-      const float v = a.lse[at];
+      const float v = a.lse[static_cast<int64_t>(bh) * a.len + qrow];
       lse2 = v == -INFINITY ? -FA_NEG : v * FA_LOG2E;
-      if (half == 0) a.delta[at] = delta;
     }
+    // for the kernel of dK and dV: whole blocks of rows, so that it reads tiles without looking at lengths
+    float* to = a.stats + static_cast<int64_t>(bh) * 2 * a.stat_rows + qrow;
+    if (half == 0) to[0] = lse2;
+    else to[a.stat_rows] = delta;
   }
   acc16_t dq[D / 32];
 #pragma unroll
@@ -324,13 +339,13 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
   registers_landed(qf);
-  if (count > 0) start(0, 0);
+  for (int i = 0; i < STAGES - 1 && i < count; ++i) start(i, i);
   const int first = qw, last = qw + 31;
   const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
   const auto visit = [&](int i, auto buffer) __attribute__((always_inline)) {
     const int k0 = tiles[i] * FA_TILE;
-    next_tile();
-    if (i + 1 < count) start(i + 1, 1 - buffer);
+    next_tile<STAGES, PT>(count - 1 - i);
+    if (i + STAGES - 1 < count) start(i + STAGES - 1, stage_before<STAGES>(buffer));
     const uint8_t* kimg = lds_raw + buffer * (2 * IMG);
     const uint8_t* vimg = kimg + IMG;
     if (nothing_seen(a, n, first, last, k0)) return;
@@ -360,7 +375,7 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_
       }
     }
   };
-  in_turn(0, count, visit);
+  in_turn<STAGES>(0, count, visit);
   __syncthreads();
   store_rows_out<T, D>(dq, a.scale, lds_raw + wave * (32 * D * 2), out_head<T>(a.dq, b, h), a.dq.st, qw, a.len, lane);
 }
@@ -390,12 +405,13 @@ __device__ __forceinline__ void store_part(const acc16_t (&acc)[D / 32], float m
 // under the waits of the other: 8192 positions, window 1024, 32 heads of 128: 1178 us against 784.
 template <int D> constexpr int dkv_tile() { return D == 64 ? 64 : 32; }
 template <int D> constexpr int dkv_buf() { return 2 * dkv_tile<D>() * D * 2 + 2 * dkv_tile<D>() * 4; }   // Q, dO, lse2, D
+template <int D> constexpr int dkv_stages() { return D == 64 ? 3 : 2; }
 template <int D> constexpr int dkv_keys() { return D == 64 ? 0 : WA_ROWS * D * 2; }
 
 template <typename T, int D>
 __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
-  constexpr int TILE = dkv_tile<D>(), IMG = TILE * D * 2, BUF = dkv_buf<D>();
+  constexpr int TILE = dkv_tile<D>(), IMG = TILE * D * 2, BUF = dkv_buf<D>(), STAGES = dkv_stages<D>(), PT = 2 * TileLoader<T, D, TILE>::N + 1;
   constexpr bool KEYS_IN_LDS = dkv_keys<D>() > 0;
   // the key blocks' parts first, then, shorter and so the ones to end with, the chunks of queries that see a block's keys as sinks only
   const uint32_t own = static_cast<uint32_t>(a.key_blocks * a.parts), heads = static_cast<uint32_t>(a.kv_heads) * a.batch;
@@ -408,9 +424,9 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
   const int n = seq_len(a, b), kw = k0 + 32 * wave, krow = kw + (lane & 31);
   uint4 kf[KEYS_IN_LDS ? 1 : D / 16], vf[D / 16];
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw)));
-  const uint8_t* keys = lds_raw + 2 * BUF + wave * (32 * D * 2);
+  const uint8_t* keys = lds_raw + STAGES * BUF + wave * (32 * D * 2);
   if constexpr (KEYS_IN_LDS) {
-    if (k0 < n) TileLoader<T, D, WA_ROWS>(a.k.st, wave, lane).start(at_head<T>(a.k, b, h), a.k.st, k0, n - 1, lds0 + 2 * BUF);
+    if (k0 < n) TileLoader<T, D, WA_ROWS>(a.k.st, wave, lane).start(at_head<T>(a.k, b, h), a.k.st, k0, n - 1, lds0 + STAGES * BUF);
   } else {
     load_resident<T, D>(kf, at_head<T>(a.k, b, h), a.k.st, krow, n, lane);
   }
@@ -430,33 +446,22 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
   const int i0 = static_cast<int>(static_cast<int64_t>(all) * share / static_cast<int>(shares)), i1 = static_cast<int>(static_cast<int64_t>(all) * (share + 1) / static_cast<int>(shares));
   const TileLoader<T, D, TILE> ldq(a.q.st, wave, lane), ldg(a.d_o.st, wave, lane);
   const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
-  float st_raw = 0.f;
-  const int tid = static_cast<int>(threadIdx.x);
-  // threads 0..63: the log-sum-exp of the tile's queries (-inf behind the end), 64..127: their D; asked for ahead of the tile's
-  // transfers and looked at behind them, at the end of the iteration
-  auto start = [&](int i, uint32_t to) {
+  // Beside a tile's rows, what the backward keeps of its queries: log-sum-exp, D. Tiles of 64: 64 floats a transfer, by two
+  // wavefronts each (the same values); of 32: both in one, by all four.
+  const uint32_t stat_off = TILE == 64 ? static_cast<uint32_t>((wave & 1) * a.stat_rows + lane) * 4 : static_cast<uint32_t>((lane >> 5) * a.stat_rows + (lane & 31)) * 4;
+  auto start = [&](int i, int buffer) {
     const int hq = h * a.group + i / per, q0 = (t0 + i % per) * TILE;
-    if (tid < 2 * TILE) {
-      const int qi = q0 + (tid & (TILE - 1));
-      const float* src = (tid < TILE ? a.lse : a.delta) + (static_cast<int64_t>(b) * a.heads + hq) * a.len;
-      st_raw = tid < TILE ? -INFINITY : 0.f;
-      if (qi < n) st_raw = src[qi];
-    }
+    const uint32_t to = lds0 + static_cast<uint32_t>(buffer) * BUF;
     ldq.start(at_head<T>(a.q, b, hq), a.q.st, q0, n - 1, to);
     ldg.start(at_head<T>(a.d_o, b, hq), a.d_o.st, q0, n - 1, to + IMG);
+    dma4(stat_off, a.stats + (static_cast<int64_t>(b) * a.heads + hq) * 2 * a.stat_rows + q0, to + 2 * IMG + (TILE == 64 ? (wave & 1) * 256 : 0));
   };
-  auto store_stats = [&](uint8_t* buf) {
-    if (tid < 2 * TILE) reinterpret_cast<float*>(buf + 2 * IMG)[tid] = tid < TILE ? (st_raw == -INFINITY ? -FA_NEG : st_raw * FA_LOG2E) : st_raw;
-  };
-  if (i0 < i1) {
-    start(i0, lds0);
-    store_stats(lds_raw);
-  }
+  wait_vmcnt<0>();      // the resident rows: waited for at their first use, they would be in every tile, behind its transfers
+  for (int i = 0; i < STAGES - 1 && i0 + i < i1; ++i) start(i0 + i, i);
   const auto visit = [&](int i, auto buffer) __attribute__((always_inline)) {
     const int q0 = (t0 + i % per) * TILE;
-    wait_vmcnt<0>();
-    __syncthreads();
-    if (i + 1 < i1) start(i + 1, lds0 + (1 - buffer) * BUF);
+    next_tile<STAGES, PT>(i1 - 1 - i);
+    if (i + STAGES - 1 < i1) start(i + STAGES - 1, stage_before<STAGES>(buffer));
     const uint8_t* qimg = lds_raw + buffer * BUF;
     const uint8_t* gimg = qimg + IMG;
     const float* stats = reinterpret_cast<const float*>(qimg + 2 * IMG);
@@ -467,7 +472,6 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
       // 32 queries at a time, so that scores, their gradients and their operands need half the registers
 #pragma unroll
       for (int nn = 0; nn < TILE / 32; ++nn) {
-        uint4 pf[2], df[2];
         acc16_t s, dp;
 #pragma unroll
         for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
@@ -509,21 +513,17 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
           float pv[8], dsv[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) { pv[e] = dp[8 * kk + e]; dsv[e] = s[8 * kk + e]; }
-          pf[kk] = acc_to_operand<T>(pv);
-          df[kk] = acc_to_operand<T>(dsv);
-        }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+          const uint4 pf = acc_to_operand<T>(pv), df = acc_to_operand<T>(dsv);
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
-            mfma<T>::run(img_columns<D>(gimg, j, 2 * nn + kk, lane), pf[kk], dv[j]);
-            mfma<T>::run(img_columns<D>(qimg, j, 2 * nn + kk, lane), df[kk], dk[j]);
+            mfma<T>::run(img_columns<D>(gimg, j, 2 * nn + kk, lane), pf, dv[j]);
+            mfma<T>::run(img_columns<D>(qimg, j, 2 * nn + kk, lane), df, dk[j]);
           }
+        }
       }
     }
-    if (i + 1 < i1) store_stats(lds_raw + (1 - buffer) * BUF);
   };
-  in_turn(i0, i1, visit);
+  in_turn<STAGES>(i0, i1, visit);
   wait_vmcnt<0>();                                              // of a share without a tile: the keys' transfers
   const bool in_parts = sink_chunk || a.parts > 1 || k0 < a.sink_blocks * WA_ROWS;
   if (in_parts) {
@@ -603,15 +603,15 @@ int launch_tiled(K kern, int lds, dim3 grid, const WaArgs& a, hipStream_t st, co
   hipLaunchKernelGGL(kern, grid, dim3(64 * WA_WAVES), lds, st, a);
   return 0;
 }
-template <int D> constexpr int tiles_lds() { return std::max(4 * FA_TILE * D * 2, WA_WAVES * 32 * D * 2); }
-template <int D> constexpr int dkv_lds() { return std::max(2 * dkv_buf<D>() + dkv_keys<D>(), WA_WAVES * 32 * D * 2); }
+template <int D, int STAGES> constexpr int tiles_lds() { return std::max(STAGES * 2 * FA_TILE * D * 2, WA_WAVES * 32 * D * 2); }
+template <int D> constexpr int dkv_lds() { return std::max(dkv_stages<D>() * dkv_buf<D>() + dkv_keys<D>(), WA_WAVES * 32 * D * 2); }
 dim3 linear_grid(const WaArgs& a, int64_t blocks, int64_t heads) { return dim3(static_cast<unsigned>(blocks * heads * a.batch)); }
 int64_t row_blocks(const WaArgs& a) { return (a.len + WA_ROWS - 1) / WA_ROWS; }
 
 template <typename T, int D>
 int fwd_launch(const WaArgs& a, hipStream_t st) {
   TraceScope trace("window_attn_fwd", st);
-  return launch_tiled(window_fwd_kernel<T, D>, tiles_lds<D>(), linear_grid(a, row_blocks(a), a.heads), a, st, "window_attn_fwd");
+  return launch_tiled(window_fwd_kernel<T, D>, tiles_lds<D, 2>(), linear_grid(a, row_blocks(a), a.heads), a, st, "window_attn_fwd");
 }
 // How the blocks of dK and dV are laid out, and the floats they leave behind.
 struct DkvPlan {
@@ -633,13 +633,14 @@ struct DkvPlan {
     sink_floats = batch * kv_heads * chunks * sink_rows * 2 * head_dim;
   }
 };
-int64_t delta_floats(int64_t len, int64_t batch, int64_t heads) { return (batch * heads * len + 63) / 64 * 64; }
+int stat_rows(int64_t len) { return static_cast<int>((len + WA_ROWS - 1) / WA_ROWS * WA_ROWS); }
+int64_t stat_floats(int64_t len, int64_t batch, int64_t heads) { return batch * heads * 2 * stat_rows(len); }
 
 template <typename T, int D>
 int bwd_launch(const WaArgs& a, hipStream_t st) {
   {
     TraceScope trace("window_attn_bwd_dq", st);
-    if (int rc = launch_tiled(window_bwd_dq_kernel<T, D>, tiles_lds<D>(), linear_grid(a, row_blocks(a), a.heads), a, st, "window_attn_bwd")) return rc;
+    if (int rc = launch_tiled(window_bwd_dq_kernel<T, D>, tiles_lds<D, dq_stages<D>()>(), linear_grid(a, row_blocks(a), a.heads), a, st, "window_attn_bwd")) return rc;
   }
   {
     TraceScope trace("window_attn_bwd_dkv", st);
@@ -688,7 +689,7 @@ extern "C" int64_t nmtg_window_attn_bwd_workspace_bytes(int64_t len, int64_t bat
   if (len <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || window <= 0 || sinks < 0) return 0;
   if (heads % kv_heads != 0) return 0;
   const DkvPlan plan(len, batch, heads, kv_heads, head_dim, window, sinks);
-  return (delta_floats(len, batch, heads) + plan.part_floats + plan.sink_floats) * static_cast<int64_t>(sizeof(float));
+  return (stat_floats(len, batch, heads) + plan.part_floats + plan.sink_floats) * static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* softmax_lse,
@@ -707,9 +708,10 @@ extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void*
   if (int rc = check_views(what, views, pointers, strides, 8)) return rc;
   WaArgs a = {};
   a.d_o = views[0]; a.q = views[1]; a.k = views[2]; a.v = views[3]; a.o = views[4]; a.dq = views[5]; a.dk = views[6]; a.dv = views[7];
-  a.lse = const_cast<float*>(softmax_lse); a.delta = static_cast<float*>(workspace);
+  a.lse = const_cast<float*>(softmax_lse); a.stats = static_cast<float*>(workspace);
+  a.stat_rows = stat_rows(len);
   const DkvPlan plan(len, batch, heads, kv_heads, head_dim, window, sinks);
-  a.part = a.delta + delta_floats(len, batch, heads);
+  a.part = a.stats + stat_floats(len, batch, heads);
   a.sink_part = a.part + plan.part_floats;
   a.key_blocks = plan.key_blocks; a.sink_blocks = plan.sink_blocks; a.parts = plan.parts; a.chunks = plan.chunks;
   a.part_rows = plan.part_rows; a.sink_rows = plan.sink_rows;

@@ -22,6 +22,8 @@ from .quantized_cache import QuantizedKVCache
 
 
 def window_attn_func(q, k, v, window, sinks=0, softmax_scale=None, lengths=None):
+    if not torch.is_autocast_enabled():             # (the context manager costs half of a short call)
+        return L.host().window_attention(q, k, v, window, sinks, softmax_scale, lengths)
     q, k, v = cast_if_autocast_enabled(q, k, v)
     with no_autocast():
         return L.host().window_attention(q, k, v, window, sinks, softmax_scale, lengths)
