@@ -47,7 +47,7 @@ struct WaArgs {
   int stat_rows;
   const int32_t* lengths;    // [batch] or null: every sequence fills `len`
   int len, batch, heads, kv_heads, group;
-  int64_t window, sinks;
+  int window, sinks;         // at most len + 1 and len: beyond, nothing changes
   float scale, scale_log2;
   // backward, dK and dV in parts (see DkvPlan): fp32 [parts][batch, kv_heads, part_rows][2][head_dim] of the key blocks, then
   // [chunks][batch, kv_heads, sink_rows][2][head_dim] of the blocks that hold sinks
@@ -151,10 +151,9 @@ template <int STAGES> constexpr int stage_before(int buffer) { return (buffer + 
 struct TileList {
   int sinks, lo, count;
   __device__ __forceinline__ TileList(const WaArgs& a, int first, int end) {
-    const int64_t from = static_cast<int64_t>(first) - a.window + 1;
     const int tiles = (end + FA_TILE - 1) / FA_TILE;
-    lo = min(from > 0 ? static_cast<int>(from / FA_TILE) : 0, tiles);
-    sinks = min(static_cast<int>(((a.sinks < end ? a.sinks : end) + FA_TILE - 1) / FA_TILE), lo);
+    lo = min(max(first - a.window + 1, 0) / FA_TILE, tiles);
+    sinks = min((min(a.sinks, end) + FA_TILE - 1) / FA_TILE, lo);
     count = sinks + tiles - lo;
   }
   __device__ __forceinline__ int operator[](int i) const { return i < sinks ? i : i - sinks + lo; }
@@ -171,9 +170,8 @@ __device__ __forceinline__ bool some_hidden(const WaArgs& a, int n, int first, i
 // Scores of one query against keys key0 + 8 (r / 4) + r % 4 (register r): those it does not see become `hidden`, the infinity
 // that the scale turns negative, whose probability is zero.
 __device__ __forceinline__ void hide_keys(acc16_t& s, const WaArgs& a, int n, int qrow, int key0, float hidden) {
-  const int64_t front = qrow - a.window;                        // keys up to here are in front of the window
-  const int from = static_cast<int>(front > -1 ? front : -1) - key0, to = (qrow < n ? qrow : -1) - key0;
-  const int sinks = static_cast<int>(a.sinks < n ? a.sinks : n) - key0;
+  // keys up to `from` are in front of the window
+  const int from = qrow - a.window - key0, to = (qrow < n ? qrow : -1) - key0, sinks = a.sinks - key0;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     const int key = 8 * (r / 4) + r % 4;
@@ -438,8 +436,7 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
     for (int r = 0; r < 16; ++r) { dk[i][r] = 0.f; dv[i][r] = 0.f; }
 
   // the query tiles up to the end of the last key's window, and those behind it
-  const int64_t reach = static_cast<int64_t>(k0) + WA_ROWS - 1 + a.window;
-  const int tw = static_cast<int>(((reach < n ? reach : n) + TILE - 1) / TILE), tn = (n + TILE - 1) / TILE;
+  const int tw = (min(k0 + WA_ROWS - 1 + a.window, n) + TILE - 1) / TILE, tn = (n + TILE - 1) / TILE;
   const int t0 = sink_chunk ? tw : k0 / TILE, t1 = sink_chunk ? tn : tw;
   const int per = k0 < n ? t1 - t0 : 0, all = per * a.group;
   // this block's share of the (head, tile) pairs
@@ -449,23 +446,31 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
   // Beside a tile's rows, what the backward keeps of its queries: log-sum-exp, D. Tiles of 64: 64 floats a transfer, by two
   // wavefronts each (the same values); of 32: both in one, by all four.
   const uint32_t stat_off = TILE == 64 ? static_cast<uint32_t>((wave & 1) * a.stat_rows + lane) * 4 : static_cast<uint32_t>((lane >> 5) * a.stat_rows + (lane & 31)) * 4;
-  auto start = [&](int i, int buffer) {
-    const int hq = h * a.group + i / per, q0 = (t0 + i % per) * TILE;
+  // (head, tile) of the next transfers and of the next products
+  struct Cursor { int head, tile; };
+  auto advance = [&](Cursor& c) {
+    if (++c.tile == t1) { c.tile = t0; ++c.head; }
+  };
+  Cursor ahead = {h * a.group + (per > 0 ? i0 / per : 0), t0 + (per > 0 ? i0 % per : 0)}, here = ahead;
+  auto start = [&](int buffer) {
+    const int hq = ahead.head, q0 = ahead.tile * TILE;
+    advance(ahead);
     const uint32_t to = lds0 + static_cast<uint32_t>(buffer) * BUF;
     ldq.start(at_head<T>(a.q, b, hq), a.q.st, q0, n - 1, to);
     ldg.start(at_head<T>(a.d_o, b, hq), a.d_o.st, q0, n - 1, to + IMG);
     dma4(stat_off, a.stats + (static_cast<int64_t>(b) * a.heads + hq) * 2 * a.stat_rows + q0, to + 2 * IMG + (TILE == 64 ? (wave & 1) * 256 : 0));
   };
   wait_vmcnt<0>();      // the resident rows: waited for at their first use, they would be in every tile, behind its transfers
-  for (int i = 0; i < STAGES - 1 && i0 + i < i1; ++i) start(i0 + i, i);
+  for (int i = 0; i < STAGES - 1 && i0 + i < i1; ++i) start(i);
   const auto visit = [&](int i, auto buffer) __attribute__((always_inline)) {
-    const int q0 = (t0 + i % per) * TILE;
+    const int q0 = here.tile * TILE;
+    advance(here);
     next_tile<STAGES, PT>(i1 - 1 - i);
-    if (i + STAGES - 1 < i1) start(i + STAGES - 1, stage_before<STAGES>(buffer));
+    if (i + STAGES - 1 < i1) start(stage_before<STAGES>(buffer));
     const uint8_t* qimg = lds_raw + buffer * BUF;
     const uint8_t* gimg = qimg + IMG;
     const float* stats = reinterpret_cast<const float*>(qimg + 2 * IMG);
-    const int64_t klast = kw + 31;
+    const int klast = kw + 31;
     const bool nothing = q0 + TILE - 1 < kw || kw >= n || (q0 - a.window >= klast && kw >= a.sinks);
     if (!nothing) {
       const bool edge = q0 < klast || klast >= n || (q0 + TILE - 1 - a.window >= kw && klast >= a.sinks);
@@ -486,8 +491,7 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
         if (edge) {
           // queries that do not see this lane's key: in front of it, or behind its window (a sink has none)
           const int at = q0 + 32 * nn + 4 * half;
-          const int64_t behind = krow < a.sinks ? n : krow + a.window;
-          const int from = krow < n ? krow - at : n, to = static_cast<int>(behind < n ? behind : n) - at;
+          const int from = krow < n ? krow - at : n, to = (krow < a.sinks ? n : min(krow + a.window, n)) - at;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int qi = 8 * (r / 4) + r % 4;
@@ -674,7 +678,7 @@ extern "C" int nmtg_window_attn_fwd(const void* q, const void* k, const void* v,
   WaArgs a = {};
   a.q = views[0]; a.k = views[1]; a.v = views[2]; a.o = views[3];
   a.lse = softmax_lse; a.lengths = lengths; a.len = static_cast<int>(len); a.batch = static_cast<int>(batch); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
-  a.group = static_cast<int>(heads / kv_heads); a.window = window; a.sinks = sinks; a.scale = softmax_scale; a.scale_log2 = log2_scale(softmax_scale);
+  a.group = static_cast<int>(heads / kv_heads); a.window = static_cast<int>(std::min(window, len + 1)); a.sinks = static_cast<int>(std::min(sinks, len)); a.scale = softmax_scale; a.scale_log2 = log2_scale(softmax_scale);
   hipStream_t st = static_cast<hipStream_t>(stream);
   int rc;
   if (dtype == NMTG_F16) rc = head_dim == 64 ? fwd_launch<f16_t, 64>(a, st) : fwd_launch<f16_t, 128>(a, st);
@@ -717,7 +721,7 @@ extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void*
   a.part_rows = plan.part_rows; a.sink_rows = plan.sink_rows;
   a.lengths = lengths; a.len = static_cast<int>(len);
   a.batch = static_cast<int>(batch); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads); a.group = static_cast<int>(heads / kv_heads);
-  a.window = window; a.sinks = sinks; a.scale = softmax_scale; a.scale_log2 = log2_scale(softmax_scale);
+  a.window = static_cast<int>(std::min(window, len + 1)); a.sinks = static_cast<int>(std::min(sinks, len)); a.scale = softmax_scale; a.scale_log2 = log2_scale(softmax_scale);
   hipStream_t st = static_cast<hipStream_t>(stream);
   int rc;
   if (dtype == NMTG_F16) rc = head_dim == 64 ? bwd_launch<f16_t, 64>(a, st) : bwd_launch<f16_t, 128>(a, st);
