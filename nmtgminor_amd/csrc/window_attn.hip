@@ -38,6 +38,9 @@ __device__ __forceinline__ WaBlock query_block(int blocks, int group, int kv_hea
   return {static_cast<int>(rest % blocks), static_cast<int>(kv % kv_heads * group + id % group), static_cast<int>(kv / kv_heads)};
 }
 
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
 struct WaView { const void* p; int64_t st, sb, sh; };   // [len, batch, heads, head_dim], head_dim contiguous
 
 struct WaArgs {
@@ -69,26 +72,39 @@ __device__ __forceinline__ int seq_len(const WaArgs& a, int b) {
 // ---- the LDS image ----
 template <int D>
 __device__ __forceinline__ int img_swizzle(int r) { return D == 64 ? (4 * ((r >> 1) & 1) | ((r >> 2) & 3)) : (4 * (r & 3) | ((r >> 2) & 3)); }
-template <int D>
-__device__ __forceinline__ uint32_t img_at(int r, int c) { return static_cast<uint32_t>(r * (2 * D) + (c ^ img_swizzle<D>(r)) * 16); }
-// A operand: rows 32 i + (lane & 31), columns 16 s + 8 (lane >> 5) .. + 7
-template <int D>
-__device__ __forceinline__ uint4 img_rows(const uint8_t* img, int i, int s, int lane) {
-  return *reinterpret_cast<const uint4*>(img + img_at<D>(32 * i + (lane & 31), 2 * s + (lane >> 5)));
+
+// The lane's LDS addresses, which differ between the pieces of an operand by an exclusive-or and a constant: two registers
+// instead of one per piece, which the compiler would keep through the loop (`per tile` hides from it that they do not change).
+template <typename V>
+__device__ __forceinline__ const __attribute__((address_space(3))) V* lds_ptr(uint32_t at) {
+  return reinterpret_cast<const __attribute__((address_space(3))) V*>(at);
 }
-// A operand of the transposed tile: columns 32 i + (lane & 31), rows 16 kk + 8 (lane >> 5) .. + 7
 template <int D>
-__device__ __forceinline__ uint4 img_columns(const uint8_t* img, int i, int kk, int lane) {
-  const int r = 16 * kk + 8 * (lane >> 5) + ((lane >> 2) & 3);
-  const int c = 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-  const uint8_t* p = img + (lane & 1) * 8;
-  const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p + img_at<D>(r, c)));
-  const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p + img_at<D>(r + 4, c)));
-  union { s16x4_t s[2]; uint4 u; } cv;
-  cv.s[0] = lo;
-  cv.s[1] = hi;
-  return cv.u;
-}
+struct ImgReader {
+  uint32_t rows, columns;
+  // base: LDS address of the images, a multiple of 256
+  __device__ __forceinline__ ImgReader(uint32_t base, int lane) {
+    const int r = lane & 31, rt = 8 * (lane >> 5) + ((lane >> 2) & 3), ct = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+    rows = base + static_cast<uint32_t>(r * (2 * D) + ((lane >> 5) ^ img_swizzle<D>(r)) * 16);
+    columns = base + static_cast<uint32_t>(rt * (2 * D) + (ct ^ img_swizzle<D>(rt)) * 16 + (lane & 1) * 8);
+  }
+  __device__ __forceinline__ void per_tile() { asm volatile("" : "+v"(rows), "+v"(columns)); }
+  // A operand: rows 32 i + (lane & 31), columns 16 s + 8 (lane >> 5) .. + 7 of the image at `img`
+  __device__ __forceinline__ uint4 row_operand(int img, int i, int s) const {
+    const u32x4_t v = *lds_ptr<u32x4_t>((rows ^ static_cast<uint32_t>(32 * s)) + static_cast<uint32_t>(img + 32 * i * 2 * D));
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  }
+  // A operand of the transposed image: columns 32 i + (lane & 31), rows 16 kk + 8 (lane >> 5) .. + 7
+  __device__ __forceinline__ uint4 column_operand(int img, int i, int kk) const {
+    const uint32_t at = columns ^ static_cast<uint32_t>(64 * i), off = static_cast<uint32_t>(img + 16 * kk * 2 * D);
+    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<__attribute__((address_space(3))) s16x4_t*>(lds_ptr<s16x4_t>(at + off)));
+    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<__attribute__((address_space(3))) s16x4_t*>(lds_ptr<s16x4_t>((at ^ 16u) + (off + 4 * 2 * D))));
+    union { s16x4_t s[2]; uint4 u; } cv;
+    cv.s[0] = lo;
+    cv.s[1] = hi;
+    return cv.u;
+  }
+};
 
 // Lane l copies the 4 bytes at sbase + voff(l) to LDS address lds_addr + 4 l (dma16's sibling).
 __device__ __forceinline__ void dma4(uint32_t voff, const void* sbase, uint32_t lds_addr) {
@@ -128,43 +144,43 @@ struct TileLoader {
   }
 };
 
-// visit(i, buffer) for i from i0 to i1, the buffers in turn: constants, so that LDS addresses need no arithmetic per tile.
-template <int STAGES, typename F>
+// visit(i, buffer) for i from i0 to i1, the two buffers in turn: constants, so that LDS addresses need no arithmetic per tile.
+template <typename F>
 __device__ __forceinline__ void in_turn(int i0, int i1, const F& visit) {
-  for (int i = i0; i < i1; i += STAGES) {
+  for (int i = i0; i < i1; i += 2) {
     visit(i, std::integral_constant<int, 0>{});
     if (i + 1 < i1) visit(i + 1, std::integral_constant<int, 1>{});
-    if constexpr (STAGES == 3) if (i + 2 < i1) visit(i + 2, std::integral_constant<int, 2>{});
   }
 }
 
-// Transfers run STAGES - 1 tiles ahead. The tile in front of `left` others has landed for the whole block, and the block's reads of
-// the tile before it are done (PT: a wavefront's transfers per tile).
-template <int STAGES, int PT>
-__device__ __forceinline__ void next_tile(int left) {
-  wait_vmcnt_upto<(STAGES - 2) * PT, PT>(min(left, STAGES - 2) * PT);
+// The next tile's transfers have landed for the whole block, and the block's reads of the tile before are done. (Transfers two
+// tiles ahead, into three buffers, gained nothing: LDS for fewer blocks on a compute unit cost as much as the longer lead gave.)
+__device__ __forceinline__ void next_tile() {
+  wait_vmcnt<0>();
   ring_barrier();
 }
-template <int STAGES> constexpr int stage_before(int buffer) { return (buffer + STAGES - 1) % STAGES; }
 
 // the tiles of a block whose queries are first .. last: those of the sinks, then those from the first query's window on
+template <int TILE = FA_TILE>
 struct TileList {
   int sinks, lo, count;
   __device__ __forceinline__ TileList(const WaArgs& a, int first, int end) {
-    const int tiles = (end + FA_TILE - 1) / FA_TILE;
-    lo = min(max(first - a.window + 1, 0) / FA_TILE, tiles);
-    sinks = min((min(a.sinks, end) + FA_TILE - 1) / FA_TILE, lo);
+    const int tiles = (end + TILE - 1) / TILE;
+    lo = min(max(first - a.window + 1, 0) / TILE, tiles);
+    sinks = min((min(a.sinks, end) + TILE - 1) / TILE, lo);
     count = sinks + tiles - lo;
   }
   __device__ __forceinline__ int operator[](int i) const { return i < sinks ? i : i - sinks + lo; }
 };
 
 // Whether queries first .. last of a sequence of n see nothing, or do not see everything, of the tile of keys from k0 on.
+template <int TILE = FA_TILE>
 __device__ __forceinline__ bool nothing_seen(const WaArgs& a, int n, int first, int last, int k0) {
-  return k0 > last || first >= n || (k0 + FA_TILE - 1 <= first - a.window && k0 >= a.sinks);
+  return k0 > last || first >= n || (k0 + TILE - 1 <= first - a.window && k0 >= a.sinks);
 }
+template <int TILE = FA_TILE>
 __device__ __forceinline__ bool some_hidden(const WaArgs& a, int n, int first, int last, int k0) {
-  return k0 + FA_TILE - 1 > first || last >= n || (k0 <= last - a.window && k0 + FA_TILE > a.sinks);
+  return k0 + TILE - 1 > first || last >= n || (k0 <= last - a.window && k0 + TILE > a.sinks);
 }
 
 // Scores of one query against keys key0 + 8 (r / 4) + r % 4 (register r): those it does not see become `hidden`, the infinity
@@ -182,10 +198,15 @@ __device__ __forceinline__ void hide_keys(acc16_t& s, const WaArgs& a, int n, in
 // ------------------------------------------------------------------------------------------------------------- forward
 constexpr float WA_FLOOR = -5e29f;   // a running maximum before the first visible key: finite, and far above the -inf of hidden ones
 
+// Key tiles of 64, or of 32 for head_dim 128: with the scores of 32 keys a wavefront needs 168 registers there, and three of them
+// share a SIMD (32 KB of LDS a block). What bounds the kernel is how much of the softmax runs under other wavefronts' products:
+// prompt of 16384 positions, window 4096, 32 heads of 128: 1088 us with two wavefronts and tiles of 64, 1023 with three.
+template <int D> constexpr int fwd_tile() { return D == 64 ? 64 : 32; }
+
 template <typename T, int D>
-__global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_kernel(WaArgs a) {
-  extern __shared__ __align__(16) uint8_t lds_raw[];
-  constexpr int IMG = FA_TILE * D * 2, STAGES = 2, PT = 2 * TileLoader<T, D>::N;
+__global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) {
+  extern __shared__ __align__(256) uint8_t lds_raw[];
+  constexpr int TILE = fwd_tile<D>(), IMG = TILE * D * 2;
   const WaBlock block = query_block((a.len + WA_ROWS - 1) / WA_ROWS, a.group, a.kv_heads);
   const int b = block.b, h = block.h, q0 = block.x * WA_ROWS;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
@@ -202,50 +223,52 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_ker
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
   registers_landed(qf);
-  const TileList tiles(a, q0, end > q0 ? end : 0);
+  const TileList<TILE> tiles(a, q0, end > q0 ? end : 0);
   const int count = end > q0 ? tiles.count : 0;
-  const TileLoader<T, D> ldk(a.k.st, wave, lane), ldv(a.v.st, wave, lane);
+  const TileLoader<T, D, TILE> ldk(a.k.st, wave, lane), ldv(a.v.st, wave, lane);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw)));
+  const ImgReader<D> reader(lds0, lane);
   auto start = [&](int i, int buffer) {
-    const int row = tiles[i] * FA_TILE;
+    const int row = tiles[i] * TILE;
     const uint32_t to = lds0 + static_cast<uint32_t>(buffer) * 2 * IMG;
     ldk.start(kb, a.k.st, row, n - 1, to);
     ldv.start(vb, a.v.st, row, n - 1, to + IMG);
   };
-  for (int i = 0; i < STAGES - 1 && i < count; ++i) start(i, i);
+  if (count > 0) start(0, 0);
   const int first = qw, last = qw + 31;                         // the wavefront's queries
   const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
   constexpr uint32_t ONES = elem<T>::dtype == NMTG_BF16 ? 0x3f803f80u : 0x3c003c00u;
   const auto visit = [&](int i, auto buffer) __attribute__((always_inline)) {
-    const int k0 = tiles[i] * FA_TILE;
-    next_tile<STAGES, PT>(count - 1 - i);
-    if (i + STAGES - 1 < count) start(i + STAGES - 1, stage_before<STAGES>(buffer));
-    const uint8_t* kimg = lds_raw + buffer * (2 * IMG);
-    const uint8_t* vimg = kimg + IMG;
-    if (nothing_seen(a, n, first, last, k0)) return;
-    acc16_t s[2];
+    const int k0 = tiles[i] * TILE;
+    next_tile();
+    if (i + 1 < count) start(i + 1, 1 - buffer);
+    constexpr int kimg = decltype(buffer)::value * 2 * IMG, vimg = kimg + IMG;
+    ImgReader<D> img = reader;
+    img.per_tile();
+    if (nothing_seen<TILE>(a, n, first, last, k0)) return;
+    acc16_t s[TILE / 32];
 #pragma unroll
-    for (int nn = 0; nn < 2; ++nn)
+    for (int nn = 0; nn < TILE / 32; ++nn)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[nn][r] = 0.f;
 #pragma unroll
     for (int ss = 0; ss < D / 16; ++ss)
 #pragma unroll
-      for (int nn = 0; nn < 2; ++nn) mfma<T>::run(img_rows<D>(kimg, nn, ss, lane), qf[ss], s[nn]);
-    if (some_hidden(a, n, first, last, k0)) {
+      for (int nn = 0; nn < TILE / 32; ++nn) mfma<T>::run(img.row_operand(kimg, nn, ss), qf[ss], s[nn]);
+    if (some_hidden<TILE>(a, n, first, last, k0)) {
 #pragma unroll
-      for (int nn = 0; nn < 2; ++nn) hide_keys(s[nn], a, n, qrow, k0 + 32 * nn + 4 * half, hidden);
+      for (int nn = 0; nn < TILE / 32; ++nn) hide_keys(s[nn], a, n, qrow, k0 + 32 * nn + 4 * half, hidden);
     }
     // the tile's maximum from the extreme raw score
     float top = s[0][0];
     if (a.scale_log2 >= 0.f) {
 #pragma unroll
-      for (int nn = 0; nn < 2; ++nn)
+      for (int nn = 0; nn < TILE / 32; ++nn)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[nn][r]);
     } else {
 #pragma unroll
-      for (int nn = 0; nn < 2; ++nn)
+      for (int nn = 0; nn < TILE / 32; ++nn)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fminf(top, s[nn][r]);
     }
@@ -264,7 +287,7 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_ker
         for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
     }
 #pragma unroll
-    for (int kk = 0; kk < FA_TILE / 16; ++kk) {
+    for (int kk = 0; kk < TILE / 16; ++kk) {
       float pv[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) pv[e] = fast_exp2(__builtin_fmaf(s[kk / 2][8 * (kk % 2) + e], a.scale_log2, -m));
@@ -273,10 +296,10 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_ker
       // one instruction.
       l = dot2<T>(pf.x, ONES, dot2<T>(pf.y, ONES, dot2<T>(pf.z, ONES, dot2<T>(pf.w, ONES, l))));
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) mfma<T>::run(img_columns<D>(vimg, j, kk, lane), pf, o[j]);
+      for (int j = 0; j < D / 32; ++j) mfma<T>::run(img.column_operand(vimg, j, kk), pf, o[j]);
     }
   };
-  in_turn<STAGES>(0, count, visit);
+  in_turn(0, count, visit);
   __syncthreads();                                              // every wavefront is done with the images
   const float sum = pair_sum(l);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -286,12 +309,10 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_fwd_ker
 }
 
 // ------------------------------------------------------------------------------------ backward: dQ, and D = rowsum(dO O)
-template <int D> constexpr int dq_stages() { return D == 64 ? 3 : 2; }
-
 template <typename T, int D>
-__global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_kernel(WaArgs a) {
-  extern __shared__ __align__(16) uint8_t lds_raw[];
-  constexpr int IMG = FA_TILE * D * 2, STAGES = dq_stages<D>(), PT = 2 * TileLoader<T, D>::N;
+__global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_kernel(WaArgs a) {
+  extern __shared__ __align__(256) uint8_t lds_raw[];
+  constexpr int IMG = FA_TILE * D * 2;
   const WaBlock block = query_block((a.len + WA_ROWS - 1) / WA_ROWS, a.group, a.kv_heads);
   const int b = block.b, h = block.h, q0 = block.x * WA_ROWS;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
@@ -299,10 +320,11 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_
   const int end = min(q0 + WA_ROWS, n), qw = q0 + 32 * wave, qrow = qw + (lane & 31);
   const T *kb = at_head<T>(a.k, b, h / a.group), *vb = at_head<T>(a.v, b, h / a.group);
 
-  const TileList tiles(a, q0, end > q0 ? end : 0);
+  const TileList<> tiles(a, q0, end > q0 ? end : 0);
   const int count = end > q0 ? tiles.count : 0;
   const TileLoader<T, D> ldk(a.k.st, wave, lane), ldv(a.v.st, wave, lane);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw)));
+  const ImgReader<D> reader(lds0, lane);
   auto start = [&](int i, int buffer) {
     const int row = tiles[i] * FA_TILE;
     const uint32_t to = lds0 + static_cast<uint32_t>(buffer) * 2 * IMG;
@@ -337,15 +359,16 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
   registers_landed(qf);
-  for (int i = 0; i < STAGES - 1 && i < count; ++i) start(i, i);
+  if (count > 0) start(0, 0);
   const int first = qw, last = qw + 31;
   const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
   const auto visit = [&](int i, auto buffer) __attribute__((always_inline)) {
     const int k0 = tiles[i] * FA_TILE;
-    next_tile<STAGES, PT>(count - 1 - i);
-    if (i + STAGES - 1 < count) start(i + STAGES - 1, stage_before<STAGES>(buffer));
-    const uint8_t* kimg = lds_raw + buffer * (2 * IMG);
-    const uint8_t* vimg = kimg + IMG;
+    next_tile();
+    if (i + 1 < count) start(i + 1, 1 - buffer);
+    constexpr int kimg = decltype(buffer)::value * 2 * IMG, vimg = kimg + IMG;
+    ImgReader<D> img = reader;
+    img.per_tile();
     if (nothing_seen(a, n, first, last, k0)) return;
     const bool edge = some_hidden(a, n, first, last, k0);
     // 32 keys at a time, so that scores, score gradients and their operands need half the registers
@@ -356,8 +379,8 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_
       for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
 #pragma unroll
       for (int ss = 0; ss < D / 16; ++ss) {
-        mfma<T>::run(img_rows<D>(kimg, nn, ss, lane), qf[ss], s);
-        mfma<T>::run(img_rows<D>(vimg, nn, ss, lane), gf[ss], dp);
+        mfma<T>::run(img.row_operand(kimg, nn, ss), qf[ss], s);
+        mfma<T>::run(img.row_operand(vimg, nn, ss), gf[ss], dp);
       }
       if (edge) hide_keys(s, a, n, qrow, k0 + 32 * nn + 4 * half, hidden);
 #pragma unroll
@@ -369,11 +392,11 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dq_
         for (int e = 0; e < 8; ++e) dsv[e] = s[8 * kk + e];
         const uint4 df = acc_to_operand<T>(dsv);
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) mfma<T>::run(img_columns<D>(kimg, j, 2 * nn + kk, lane), df, dq[j]);
+        for (int j = 0; j < D / 32; ++j) mfma<T>::run(img.column_operand(kimg, j, 2 * nn + kk), df, dq[j]);
       }
     }
   };
-  in_turn<STAGES>(0, count, visit);
+  in_turn(0, count, visit);
   __syncthreads();
   store_rows_out<T, D>(dq, a.scale, lds_raw + wave * (32 * D * 2), out_head<T>(a.dq, b, h), a.dq.st, qw, a.len, lane);
 }
@@ -403,13 +426,12 @@ __device__ __forceinline__ void store_part(const acc16_t (&acc)[D / 32], float m
 // under the waits of the other: 8192 positions, window 1024, 32 heads of 128: 1178 us against 784.
 template <int D> constexpr int dkv_tile() { return D == 64 ? 64 : 32; }
 template <int D> constexpr int dkv_buf() { return 2 * dkv_tile<D>() * D * 2 + 2 * dkv_tile<D>() * 4; }   // Q, dO, lse2, D
-template <int D> constexpr int dkv_stages() { return D == 64 ? 3 : 2; }
 template <int D> constexpr int dkv_keys() { return D == 64 ? 0 : WA_ROWS * D * 2; }
 
 template <typename T, int D>
-__global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs a) {
-  extern __shared__ __align__(16) uint8_t lds_raw[];
-  constexpr int TILE = dkv_tile<D>(), IMG = TILE * D * 2, BUF = dkv_buf<D>(), STAGES = dkv_stages<D>(), PT = 2 * TileLoader<T, D, TILE>::N + 1;
+__global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dkv_kernel(WaArgs a) {
+  extern __shared__ __align__(256) uint8_t lds_raw[];
+  constexpr int TILE = dkv_tile<D>(), IMG = TILE * D * 2, BUF = dkv_buf<D>();
   constexpr bool KEYS_IN_LDS = dkv_keys<D>() > 0;
   // the key blocks' parts first, then, shorter and so the ones to end with, the chunks of queries that see a block's keys as sinks only
   const uint32_t own = static_cast<uint32_t>(a.key_blocks * a.parts), heads = static_cast<uint32_t>(a.kv_heads) * a.batch;
@@ -422,9 +444,9 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
   const int n = seq_len(a, b), kw = k0 + 32 * wave, krow = kw + (lane & 31);
   uint4 kf[KEYS_IN_LDS ? 1 : D / 16], vf[D / 16];
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw)));
-  const uint8_t* keys = lds_raw + STAGES * BUF + wave * (32 * D * 2);
+  const ImgReader<D> reader(lds0, lane);
   if constexpr (KEYS_IN_LDS) {
-    if (k0 < n) TileLoader<T, D, WA_ROWS>(a.k.st, wave, lane).start(at_head<T>(a.k, b, h), a.k.st, k0, n - 1, lds0 + STAGES * BUF);
+    if (k0 < n) TileLoader<T, D, WA_ROWS>(a.k.st, wave, lane).start(at_head<T>(a.k, b, h), a.k.st, k0, n - 1, lds0 + 2 * BUF);
   } else {
     load_resident<T, D>(kf, at_head<T>(a.k, b, h), a.k.st, krow, n, lane);
   }
@@ -461,15 +483,15 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
     dma4(stat_off, a.stats + (static_cast<int64_t>(b) * a.heads + hq) * 2 * a.stat_rows + q0, to + 2 * IMG + (TILE == 64 ? (wave & 1) * 256 : 0));
   };
   wait_vmcnt<0>();      // the resident rows: waited for at their first use, they would be in every tile, behind its transfers
-  for (int i = 0; i < STAGES - 1 && i0 + i < i1; ++i) start(i);
+  if (i0 < i1) start(0);
   const auto visit = [&](int i, auto buffer) __attribute__((always_inline)) {
     const int q0 = here.tile * TILE;
     advance(here);
-    next_tile<STAGES, PT>(i1 - 1 - i);
-    if (i + STAGES - 1 < i1) start(stage_before<STAGES>(buffer));
-    const uint8_t* qimg = lds_raw + buffer * BUF;
-    const uint8_t* gimg = qimg + IMG;
-    const float* stats = reinterpret_cast<const float*>(qimg + 2 * IMG);
+    next_tile();
+    if (i + 1 < i1) start(1 - buffer);
+    constexpr int qimg = decltype(buffer)::value * BUF, gimg = qimg + IMG, stats = gimg + IMG;
+    ImgReader<D> img = reader;
+    img.per_tile();
     const int klast = kw + 31;
     const bool nothing = q0 + TILE - 1 < kw || kw >= n || (q0 - a.window >= klast && kw >= a.sinks);
     if (!nothing) {
@@ -483,10 +505,10 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
 #pragma unroll
         for (int ss = 0; ss < D / 16; ++ss) {
           uint4 key;
-          if constexpr (KEYS_IN_LDS) key = img_rows<D>(keys, 0, ss, lane);
+          if constexpr (KEYS_IN_LDS) key = img.row_operand(2 * BUF, wave, ss);
           else key = kf[ss];
-          mfma<T>::run(img_rows<D>(qimg, nn, ss, lane), key, s);
-          mfma<T>::run(img_rows<D>(gimg, nn, ss, lane), vf[ss], dp);
+          mfma<T>::run(img.row_operand(qimg, nn, ss), key, s);
+          mfma<T>::run(img.row_operand(gimg, nn, ss), vf[ss], dp);
         }
         if (edge) {
           // queries that do not see this lane's key: in front of it, or behind its window (a sink has none)
@@ -501,9 +523,8 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int ql = 32 * nn + 8 * g + 4 * half;            // first of four consecutive queries, within the tile
-          const float4 l4 = *reinterpret_cast<const float4*>(stats + ql);
-          const float4 d4 = *reinterpret_cast<const float4*>(stats + TILE + ql);
-          const float lse2[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
+          const f32x4_t lse2 = *lds_ptr<f32x4_t>(lds0 + 16 * half + static_cast<uint32_t>(stats + 4 * (ql - 4 * half)));
+          const f32x4_t dl = *lds_ptr<f32x4_t>(lds0 + 16 * half + static_cast<uint32_t>(stats + 4 * (TILE + ql - 4 * half)));
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int r = 4 * g + e;
@@ -520,14 +541,14 @@ __global__ __launch_bounds__(64 * WA_WAVES, 2) void window_bwd_dkv_kernel(WaArgs
           const uint4 pf = acc_to_operand<T>(pv), df = acc_to_operand<T>(dsv);
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
-            mfma<T>::run(img_columns<D>(gimg, j, 2 * nn + kk, lane), pf, dv[j]);
-            mfma<T>::run(img_columns<D>(qimg, j, 2 * nn + kk, lane), df, dk[j]);
+            mfma<T>::run(img.column_operand(gimg, j, 2 * nn + kk), pf, dv[j]);
+            mfma<T>::run(img.column_operand(qimg, j, 2 * nn + kk), df, dk[j]);
           }
         }
       }
     }
   };
-  in_turn<STAGES>(i0, i1, visit);
+  in_turn(i0, i1, visit);
   wait_vmcnt<0>();                                              // of a share without a tile: the keys' transfers
   const bool in_parts = sink_chunk || a.parts > 1 || k0 < a.sink_blocks * WA_ROWS;
   if (in_parts) {
@@ -607,15 +628,15 @@ int launch_tiled(K kern, int lds, dim3 grid, const WaArgs& a, hipStream_t st, co
   hipLaunchKernelGGL(kern, grid, dim3(64 * WA_WAVES), lds, st, a);
   return 0;
 }
-template <int D, int STAGES> constexpr int tiles_lds() { return std::max(STAGES * 2 * FA_TILE * D * 2, WA_WAVES * 32 * D * 2); }
-template <int D> constexpr int dkv_lds() { return std::max(dkv_stages<D>() * dkv_buf<D>() + dkv_keys<D>(), WA_WAVES * 32 * D * 2); }
+template <int D, int TILE> constexpr int tiles_lds() { return std::max(4 * TILE * D * 2, WA_WAVES * 32 * D * 2); }
+template <int D> constexpr int dkv_lds() { return std::max(2 * dkv_buf<D>() + dkv_keys<D>(), WA_WAVES * 32 * D * 2); }
 dim3 linear_grid(const WaArgs& a, int64_t blocks, int64_t heads) { return dim3(static_cast<unsigned>(blocks * heads * a.batch)); }
 int64_t row_blocks(const WaArgs& a) { return (a.len + WA_ROWS - 1) / WA_ROWS; }
 
 template <typename T, int D>
 int fwd_launch(const WaArgs& a, hipStream_t st) {
   TraceScope trace("window_attn_fwd", st);
-  return launch_tiled(window_fwd_kernel<T, D>, tiles_lds<D, 2>(), linear_grid(a, row_blocks(a), a.heads), a, st, "window_attn_fwd");
+  return launch_tiled(window_fwd_kernel<T, D>, tiles_lds<D, fwd_tile<D>()>(), linear_grid(a, row_blocks(a), a.heads), a, st, "window_attn_fwd");
 }
 // How the blocks of dK and dV are laid out, and the floats they leave behind.
 struct DkvPlan {
@@ -644,7 +665,7 @@ template <typename T, int D>
 int bwd_launch(const WaArgs& a, hipStream_t st) {
   {
     TraceScope trace("window_attn_bwd_dq", st);
-    if (int rc = launch_tiled(window_bwd_dq_kernel<T, D>, tiles_lds<D, dq_stages<D>()>(), linear_grid(a, row_blocks(a), a.heads), a, st, "window_attn_bwd")) return rc;
+    if (int rc = launch_tiled(window_bwd_dq_kernel<T, D>, tiles_lds<D, FA_TILE>(), linear_grid(a, row_blocks(a), a.heads), a, st, "window_attn_bwd")) return rc;
   }
   {
     TraceScope trace("window_attn_bwd_dkv", st);
