@@ -31,7 +31,7 @@ OPT = os.environ.get("HOSTSIM_OPT", "-O0")
 LIB = os.path.join(BUILD, "libnmtg_hostsim_asan.so" if SANITIZE else "libnmtg_hostsim.so")
 
 KERNEL_SOURCES = ["api.hip", "layer_norm.hip", "softmax_dropout.hip", "dropout_add.hip", "xentropy.hip", "reduce.hip",
-                  "gemm.hip", "gemm_nt.hip", "gemm_nn.hip", "gemm_tn.hip", "mlp.hip", "attention.hip", "rel_position.hip", "multi_tensor.hip", "rotary.hip", "flash_attn.hip", "gemm_f32.hip", "glu.hip", "attn_decode.hip", "gemm_skinny.hip", "stream_probe.hip"]
+                  "gemm.hip", "gemm_nt.hip", "gemm_nn.hip", "gemm_tn.hip", "mlp.hip", "attention.hip", "rel_position.hip", "multi_tensor.hip", "rotary.hip", "flash_attn.hip", "gemm_f32.hip", "glu.hip", "attn_decode.hip", "gemm_skinny.hip", "stream_probe.hip", "window_attn.hip", "kv_cache.hip"]
 HEADERS = ["common.hip.h", "trace.hip.h", "reduce.hip.h", "gemm.hip.h", "gemm_ring.hip.h", "gemm_inst.hip.h", "flash_tile.hip.h"]
 OWN_SOURCES = ["hostsim.cpp", "stubs.cpp"]
 
@@ -43,6 +43,13 @@ ASM_REWRITES = [
     (r'asm volatile\("s_mov_b32 m0, %2\\n\\ts_nop 0\\n\\tglobal_load_lds_dwordx4 %0, %1"\s*:\s*:\s*"v"\(voff\), "s"\(sbase\), '
      r'"s"\(lds_addr\)\s*:\s*"memory", "m0"\);',
      "::hostsim::dma_issue(static_cast<const char*>(sbase) + voff, ::hostsim::lds_offset_of(lds_addr) + 16 * ::hostsim::lane_id(), 16);"),
+    # the same with 4 bytes a lane
+    (r'asm volatile\("s_mov_b32 m0, %2\\n\\ts_nop 0\\n\\tglobal_load_lds_dword %0, %1"\s*:\s*:\s*"v"\(voff\), "s"\(sbase\), '
+     r'"s"\(lds_addr\)\s*:\s*"memory", "m0"\);',
+     "::hostsim::dma_issue(static_cast<const char*>(sbase) + voff, ::hostsim::lds_offset_of(lds_addr) + 4 * ::hostsim::lane_id(), 4);"),
+    # an LDS address (the low 32 bits of a pointer into the dynamic-LDS block) as a pointer
+    (r'reinterpret_cast<const __attribute__\(\(address_space\(3\)\)\) V\*>\(at\)',
+     "(const __attribute__((address_space(3))) V*)(::hostsim::dynamic_lds + ::hostsim::lds_offset_of(at))"),
     # LDS reads done, then the workgroup barrier
     (r'asm volatile\("s_waitcnt lgkmcnt\(0\)\\n\\ts_barrier" ::: "memory"\);', "::hostsim::sync_block();"),
 ]

@@ -172,6 +172,66 @@ static inline uint32_t __builtin_amdgcn_perm(uint32_t src0, uint32_t src1, uint3
   return out;
 }
 
+// v_alignbit_b32: bits s .. s + 31 of the 64 bits {hi, lo}
+static inline uint32_t __builtin_amdgcn_alignbit(uint32_t hi, uint32_t lo, uint32_t s) {
+  return static_cast<uint32_t>(((static_cast<uint64_t>(hi) << 32) | lo) >> (s & 31u));
+}
+
+// v_cvt_scalef32_pk_*: two elements to and from 4-bit (E2M1) and 8-bit (E4M3) floats with a power-of-two scale, of which only
+// the exponent field counts (0 is 2^-127, 255 gives NaN). To nearest, ties to even; 4 bits saturate, 8 bits overflow to NaN.
+namespace hostsim {
+inline double block_scale(float scale) {
+  uint32_t u;
+  std::memcpy(&u, &scale, 4);
+  const int e = static_cast<int>((u >> 23) & 255u);
+  return e == 255 ? std::nan("") : std::ldexp(1.0, e - 127);
+}
+inline double small_value(int bits, int code) {        // code without its sign
+  const int m = bits == 4 ? 1 : 3, bias = bits == 4 ? 1 : 7, e = code >> m, f = code & ((1 << m) - 1);
+  return e == 0 ? std::ldexp(f, 1 - bias - m) : std::ldexp((1 << m) + f, e - bias - m);
+}
+inline uint32_t small_code(int bits, float v, float scale) {
+  const int top = bits == 4 ? 7 : 126;
+  const double y = std::fabs(static_cast<double>(v)) / block_scale(scale);
+  int code = top;
+  for (int c = 0; c < top; ++c) {
+    const double mid = (small_value(bits, c) + small_value(bits, c + 1)) / 2;
+    if (y < mid || (y == mid && c % 2 == 0)) { code = c; break; }
+  }
+  if (bits == 8 && !(y <= 464.0)) code = 127;
+  return static_cast<uint32_t>(code) | (std::signbit(v) ? (bits == 4 ? 8u : 128u) : 0u);
+}
+inline float small_float(int bits, uint32_t code, float scale) {
+  const uint32_t sign = bits == 4 ? 8u : 128u;
+  if (bits == 8 && (code & 127u) == 127u) return std::nanf("");
+  const double v = small_value(bits, static_cast<int>(code & (sign - 1))) * block_scale(scale);
+  return static_cast<float>((code & sign) != 0 ? -v : v);
+}
+template <typename V> inline uint32_t to_fp4(uint32_t old, V x, float scale, int sel) {
+  const uint32_t byte = small_code(4, static_cast<float>(x[0]), scale) | (small_code(4, static_cast<float>(x[1]), scale) << 4);
+  return (old & ~(0xffu << (8 * sel))) | (byte << (8 * sel));
+}
+template <typename S, typename V> inline S to_fp8(S old, V x, float scale, bool high) {
+  old[high ? 1 : 0] = static_cast<short>(small_code(8, static_cast<float>(x[0]), scale) | (small_code(8, static_cast<float>(x[1]), scale) << 8));
+  return old;
+}
+template <typename V, typename E> inline V from_fp4(uint32_t w, float scale, int sel) {
+  return V{static_cast<E>(small_float(4, (w >> (8 * sel)) & 15u, scale)), static_cast<E>(small_float(4, (w >> (8 * sel + 4)) & 15u, scale))};
+}
+template <typename V, typename E> inline V from_fp8(uint32_t w, float scale, bool high) {
+  return V{static_cast<E>(small_float(8, (w >> (high ? 16 : 0)) & 255u, scale)), static_cast<E>(small_float(8, (w >> (high ? 24 : 8)) & 255u, scale))};
+}
+}  // namespace hostsim
+typedef short hostsim_short2 __attribute__((ext_vector_type(2)));
+static inline uint32_t __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(uint32_t old, hostsim_bf16x2 x, float s, int sel) { return hostsim::to_fp4(old, x, s, sel); }
+static inline uint32_t __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(uint32_t old, hostsim_half2 x, float s, int sel) { return hostsim::to_fp4(old, x, s, sel); }
+static inline hostsim_short2 __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hostsim_short2 old, hostsim_bf16x2 x, float s, bool hi) { return hostsim::to_fp8(old, x, s, hi); }
+static inline hostsim_short2 __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(hostsim_short2 old, hostsim_half2 x, float s, bool hi) { return hostsim::to_fp8(old, x, s, hi); }
+static inline hostsim_bf16x2 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(uint32_t w, float s, int sel) { return hostsim::from_fp4<hostsim_bf16x2, __bf16>(w, s, sel); }
+static inline hostsim_half2 __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(uint32_t w, float s, int sel) { return hostsim::from_fp4<hostsim_half2, _Float16>(w, s, sel); }
+static inline hostsim_bf16x2 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(uint32_t w, float s, bool hi) { return hostsim::from_fp8<hostsim_bf16x2, __bf16>(w, s, hi); }
+static inline hostsim_half2 __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(uint32_t w, float s, bool hi) { return hostsim::from_fp8<hostsim_half2, _Float16>(w, s, hi); }
+
 // s_waitcnt: only the vmcnt field matters here (bits 3:0 and 15:14 of the gfx9 encoding)
 static inline void __builtin_amdgcn_s_waitcnt(int imm) { hostsim::dma_wait((imm & 15) | (((imm >> 14) & 3) << 4)); }
 
