@@ -82,11 +82,19 @@ __device__ __forceinline__ const __attribute__((address_space(3))) V* lds_ptr(ui
 template <int D>
 struct ImgReader {
   uint32_t rows, columns;
+  ImgReader() = default;
   // base: LDS address of the images, a multiple of 256
   __device__ __forceinline__ ImgReader(uint32_t base, int lane) {
     const int r = lane & 31, rt = 8 * (lane >> 5) + ((lane >> 2) & 3), ct = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
     rows = base + static_cast<uint32_t>(r * (2 * D) + ((lane >> 5) ^ img_swizzle<D>(r)) * 16);
     columns = base + static_cast<uint32_t>(rt * (2 * D) + (ct ^ img_swizzle<D>(rt)) * 16 + (lane & 1) * 8);
+  }
+  // the same `offset` bytes on (a multiple of 256)
+  __device__ __forceinline__ ImgReader at(int offset) const {
+    ImgReader r = *this;
+    r.rows += static_cast<uint32_t>(offset);
+    r.columns += static_cast<uint32_t>(offset);
+    return r;
   }
   __device__ __forceinline__ void per_tile() { asm volatile("" : "+v"(rows), "+v"(columns)); }
   // A operand: rows 32 i + (lane & 31), columns 16 s + 8 (lane >> 5) .. + 7 of the image at `img`
@@ -183,15 +191,24 @@ __device__ __forceinline__ bool some_hidden(const WaArgs& a, int n, int first, i
   return k0 + TILE - 1 > first || last >= n || (k0 <= last - a.window && k0 + TILE > a.sinks);
 }
 
-// Scores of one query against keys key0 + 8 (r / 4) + r % 4 (register r): those it does not see become `hidden`, the infinity
-// that the scale turns negative, whose probability is zero.
-__device__ __forceinline__ void hide_keys(acc16_t& s, const WaArgs& a, int n, int qrow, int key0, float hidden) {
-  // keys up to `from` are in front of the window
-  const int from = qrow - a.window - key0, to = (qrow < n ? qrow : -1) - key0, sinks = a.sinks - key0;
+// Scores of the queries first .. first + 31 (one a lane pair, qrow) against the 32 keys from k0 on, 8 (r / 4) + r % 4 + 4 half in
+// register r: those that a query does not see become `hidden`, the infinity that the scale turns negative, whose probability is zero.
+// Most tiles at an edge are at one of them, so that each edge is a pass of its own: a comparison and a select per score.
+__device__ __forceinline__ void hide_keys(acc16_t& s, const WaArgs& a, int n, int first, int qrow, int half, int k0, float hidden) {
+  asm volatile("" : "+v"(qrow), "+v"(half));                   // so that no bounds are kept in registers through the loops
+  const int key0 = k0 + 4 * half;
+  if (k0 + 31 > first || first + 31 >= n) {                    // the diagonal, or the end of the sequence
+    const int to = (qrow < n ? qrow : -1) - key0;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int key = 8 * (r / 4) + r % 4;
-    s[r] = (key > to) | ((key <= from) & (key >= sinks)) ? hidden : s[r];   // (selects: short-circuit tests became branches per element)
+    for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + r % 4 > to ? hidden : s[r];
+  }
+  if (k0 <= first + 31 - a.window && k0 + 31 >= a.sinks) {     // keys up to `from` are in front of the window
+    const int from = qrow - a.window - key0, sinks = a.sinks - key0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int key = 8 * (r / 4) + r % 4;
+      s[r] = (key <= from) & (key >= sinks) ? hidden : s[r];    // (a short-circuit test became a branch per element)
+    }
   }
 }
 
@@ -257,7 +274,7 @@ __global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) 
       for (int nn = 0; nn < TILE / 32; ++nn) mfma<T>::run(img.row_operand(kimg, nn, ss), qf[ss], s[nn]);
     if (some_hidden<TILE>(a, n, first, last, k0)) {
 #pragma unroll
-      for (int nn = 0; nn < TILE / 32; ++nn) hide_keys(s[nn], a, n, qrow, k0 + 32 * nn + 4 * half, hidden);
+      for (int nn = 0; nn < TILE / 32; ++nn) hide_keys(s[nn], a, n, first, qrow, half, k0 + 32 * nn, hidden);
     }
     // the tile's maximum from the extreme raw score
     float top = s[0][0];
@@ -325,9 +342,9 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_
   const TileLoader<T, D> ldk(a.k.st, wave, lane), ldv(a.v.st, wave, lane);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw)));
   const ImgReader<D> reader(lds0, lane);
-  auto start = [&](int i, int buffer) {
+  auto start = [&](int i) {
     const int row = tiles[i] * FA_TILE;
-    const uint32_t to = lds0 + static_cast<uint32_t>(buffer) * 2 * IMG;
+    const uint32_t to = lds0 + static_cast<uint32_t>(i & 1) * 2 * IMG;
     ldk.start(kb, a.k.st, row, n - 1, to);
     ldv.start(vb, a.v.st, row, n - 1, to + IMG);
   };
@@ -351,7 +368,7 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_
     // for the kernel of dK and dV: whole blocks of rows, so that it reads tiles without looking at lengths
     float* to = a.stats + static_cast<int64_t>(bh) * 2 * a.stat_rows + qrow;
     if (half == 0) to[0] = lse2;
-    else to[a.stat_rows] = delta;
+    else to[a.stat_rows] = -delta;
   }
   acc16_t dq[D / 32];
 #pragma unroll
@@ -359,32 +376,31 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
   registers_landed(qf);
-  if (count > 0) start(0, 0);
+  if (count > 0) start(0);
   const int first = qw, last = qw + 31;
   const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
-  const auto visit = [&](int i, auto buffer) __attribute__((always_inline)) {
+  for (int i = 0; i < count; ++i) {
     const int k0 = tiles[i] * FA_TILE;
     next_tile();
-    if (i + 1 < count) start(i + 1, 1 - buffer);
-    constexpr int kimg = decltype(buffer)::value * 2 * IMG, vimg = kimg + IMG;
-    ImgReader<D> img = reader;
-    img.per_tile();
-    if (nothing_seen(a, n, first, last, k0)) return;
-    const bool edge = some_hidden(a, n, first, last, k0);
-    // 32 keys at a time, so that scores, score gradients and their operands need half the registers
-#pragma unroll
-    for (int nn = 0; nn < 2; ++nn) {
+    if (i + 1 < count) start(i + 1);
+    // 32 keys at a time, so that scores, score gradients and their operands need half the registers; what is not seen is left out.
+    // At head dimension 128 the products of dP start from -D, which takes the subtraction out (2%); at 64 there are no registers for
+    // that (25 spilt, half as fast again).
+#pragma unroll 1
+    for (int kn = k0; kn < k0 + FA_TILE; kn += 32) {
+      if (nothing_seen<32>(a, n, first, last, kn)) continue;
+      const ImgReader<D> img = reader.at((i & 1) * (2 * IMG) + (kn - k0) * (2 * D));
       acc16_t s, dp;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+      for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = D == 128 ? -delta : 0.f; }
 #pragma unroll
       for (int ss = 0; ss < D / 16; ++ss) {
-        mfma<T>::run(img.row_operand(kimg, nn, ss), qf[ss], s);
-        mfma<T>::run(img.row_operand(vimg, nn, ss), gf[ss], dp);
+        mfma<T>::run(img.row_operand(0, 0, ss), qf[ss], s);
+        mfma<T>::run(img.row_operand(IMG, 0, ss), gf[ss], dp);
       }
-      if (edge) hide_keys(s, a, n, qrow, k0 + 32 * nn + 4 * half, hidden);
+      hide_keys(s, a, n, first, qrow, half, kn, hidden);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], a.scale_log2, -lse2)) * (dp[r] - delta);
+      for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], a.scale_log2, -lse2)) * (D == 128 ? dp[r] : dp[r] - delta);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         float dsv[8];
@@ -392,11 +408,10 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_
         for (int e = 0; e < 8; ++e) dsv[e] = s[8 * kk + e];
         const uint4 df = acc_to_operand<T>(dsv);
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) mfma<T>::run(img.column_operand(kimg, j, 2 * nn + kk), df, dq[j]);
+        for (int j = 0; j < D / 32; ++j) mfma<T>::run(img.column_operand(0, j, kk), df, dq[j]);
       }
     }
-  };
-  in_turn(0, count, visit);
+  }
   __syncthreads();
   store_rows_out<T, D>(dq, a.scale, lds_raw + wave * (32 * D * 2), out_head<T>(a.dq, b, h), a.dq.st, qw, a.len, lane);
 }
@@ -493,57 +508,62 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dkv
     ImgReader<D> img = reader;
     img.per_tile();
     const int klast = kw + 31;
-    const bool nothing = q0 + TILE - 1 < kw || kw >= n || (q0 - a.window >= klast && kw >= a.sinks);
-    if (!nothing) {
-      const bool edge = q0 < klast || klast >= n || (q0 + TILE - 1 - a.window >= kw && klast >= a.sinks);
-      // 32 queries at a time, so that scores, their gradients and their operands need half the registers
+    // 32 queries at a time, so that scores, their gradients and their operands need half the registers
 #pragma unroll
-      for (int nn = 0; nn < TILE / 32; ++nn) {
-        acc16_t s, dp;
+    for (int nn = 0; nn < TILE / 32; ++nn) {
+      const int qn = q0 + 32 * nn;
+      if (qn + 31 < kw || kw >= n || (qn - a.window >= klast && kw >= a.sinks)) continue;
+      acc16_t s, dp;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+      for (int g = 0; g < 4; ++g) {
+        const int ql = 32 * nn + 8 * g;
+        const f32x4_t dl = *lds_ptr<f32x4_t>(lds0 + 16 * half + static_cast<uint32_t>(stats + 4 * (TILE + ql)));
 #pragma unroll
-        for (int ss = 0; ss < D / 16; ++ss) {
-          uint4 key;
-          if constexpr (KEYS_IN_LDS) key = img.row_operand(2 * BUF, wave, ss);
-          else key = kf[ss];
-          mfma<T>::run(img.row_operand(qimg, nn, ss), key, s);
-          mfma<T>::run(img.row_operand(gimg, nn, ss), vf[ss], dp);
+        for (int e = 0; e < 4; ++e) { s[4 * g + e] = 0.f; dp[4 * g + e] = dl[e]; }
+      }
+#pragma unroll
+      for (int ss = 0; ss < D / 16; ++ss) {
+        uint4 key;
+        if constexpr (KEYS_IN_LDS) key = img.row_operand(2 * BUF, wave, ss);
+        else key = kf[ss];
+        mfma<T>::run(img.row_operand(qimg, nn, ss), key, s);
+        mfma<T>::run(img.row_operand(gimg, nn, ss), vf[ss], dp);
+      }
+      if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);   // exponentials among the products would need more registers than there are
+      // queries that do not see this lane's key: in front of it, or behind its window (a sink has none)
+      const int at = qn + 4 * half;
+      if (qn < klast || klast >= n) {
+        const int from = krow < n ? krow - at : n;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + r % 4 < from ? hidden : s[r];
+      }
+      if (qn + 31 - a.window >= kw && klast >= a.sinks) {
+        const int to = (krow < a.sinks ? n : min(krow + a.window, n)) - at;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + r % 4 >= to ? hidden : s[r];
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int ql = 32 * nn + 8 * g + 4 * half;            // first of four consecutive queries, within the tile
+        const f32x4_t lse2 = *lds_ptr<f32x4_t>(lds0 + 16 * half + static_cast<uint32_t>(stats + 4 * (ql - 4 * half)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          const float p = fast_exp2(__builtin_fmaf(s[r], a.scale_log2, -lse2[e]));
+          s[r] = p * dp[r];
+          dp[r] = p;
         }
-        if (edge) {
-          // queries that do not see this lane's key: in front of it, or behind its window (a sink has none)
-          const int at = q0 + 32 * nn + 4 * half;
-          const int from = krow < n ? krow - at : n, to = (krow < a.sinks ? n : min(krow + a.window, n)) - at;
+      }
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int qi = 8 * (r / 4) + r % 4;
-            s[r] = (qi < from) | (qi >= to) ? hidden : s[r];
-          }
-        }
+      for (int kk = 0; kk < 2; ++kk) {
+        float pv[8], dsv[8];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int ql = 32 * nn + 8 * g + 4 * half;            // first of four consecutive queries, within the tile
-          const f32x4_t lse2 = *lds_ptr<f32x4_t>(lds0 + 16 * half + static_cast<uint32_t>(stats + 4 * (ql - 4 * half)));
-          const f32x4_t dl = *lds_ptr<f32x4_t>(lds0 + 16 * half + static_cast<uint32_t>(stats + 4 * (TILE + ql - 4 * half)));
+        for (int e = 0; e < 8; ++e) { pv[e] = dp[8 * kk + e]; dsv[e] = s[8 * kk + e]; }
+        const uint4 pf = acc_to_operand<T>(pv), df = acc_to_operand<T>(dsv);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 4 * g + e;
-            const float p = fast_exp2(__builtin_fmaf(s[r], a.scale_log2, -lse2[e]));
-            s[r] = p * (dp[r] - dl[e]);
-            dp[r] = p;
-          }
-        }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          float pv[8], dsv[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) { pv[e] = dp[8 * kk + e]; dsv[e] = s[8 * kk + e]; }
-          const uint4 pf = acc_to_operand<T>(pv), df = acc_to_operand<T>(dsv);
-#pragma unroll
-          for (int j = 0; j < D / 32; ++j) {
-            mfma<T>::run(img.column_operand(gimg, j, 2 * nn + kk), pf, dv[j]);
-            mfma<T>::run(img.column_operand(qimg, j, 2 * nn + kk), df, dk[j]);
-          }
+        for (int j = 0; j < D / 32; ++j) {
+          mfma<T>::run(img.column_operand(gimg, j, 2 * nn + kk), pf, dv[j]);
+          mfma<T>::run(img.column_operand(qimg, j, 2 * nn + kk), df, dk[j]);
         }
       }
     }
