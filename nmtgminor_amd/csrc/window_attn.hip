@@ -570,14 +570,14 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dkv
   };
   in_turn(i0, i1, visit);
   wait_vmcnt<0>();                                              // of a share without a tile: the keys' transfers
-  const bool in_parts = sink_chunk || a.parts > 1 || k0 < a.sink_blocks * WA_ROWS;
-  if (in_parts) {
+  // What is still to be joined: all rows in parts, or those of the sinks, which the join then writes over.
+  if (sink_chunk || a.parts > 1 || k0 < a.sink_rows) {
     const int rows = sink_chunk ? a.sink_rows : a.part_rows;
     float* base = (sink_chunk ? a.sink_part : a.part) +
                   ((static_cast<int64_t>(share) * a.batch + b) * a.kv_heads + h) * rows * (2 * D);
     store_part<D>(dk, a.scale, base, 2 * D, kw, rows, lane);
     store_part<D>(dv, 1.f, base + D, 2 * D, kw, rows, lane);
-    return;
+    if (sink_chunk || a.parts > 1) return;
   }
   __syncthreads();
   uint8_t* patch = lds_raw + wave * (32 * D * 2);
@@ -672,7 +672,7 @@ struct DkvPlan {
     chunks = sink_blocks > 0 ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((behind + tiles - 1) / tiles, 128))) : 0;
     // two blocks for every compute unit, each with at least four tiles
     parts = static_cast<int>(std::max<int64_t>(1, std::min({(2 * num_cus() + blocks * batch * kv_heads - 1) / (blocks * batch * kv_heads), tiles * group / 4, int64_t(16)})));
-    sink_rows = static_cast<int>(std::min<int64_t>(len, static_cast<int64_t>(sink_blocks) * WA_ROWS));
+    sink_rows = sink_blocks > 0 ? static_cast<int>(std::min(sinks, len)) : 0;
     part_rows = parts > 1 ? static_cast<int>(len) : sink_rows;
     part_floats = batch * kv_heads * parts * part_rows * 2 * head_dim;
     sink_floats = batch * kv_heads * chunks * sink_rows * 2 * head_dim;
