@@ -493,23 +493,56 @@ __global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
   }
 }
 
-// The splits of every query row added up: one block of D threads per row.
+// The splits of every query row added up, one block per row: a thread per split for its weight, then every split's row by D / 4 threads,
+// 256 / (D / 4) splits at a time, added up in that order. Latency bounds it, so that nothing waits on a chain over the splits: 2 sequences
+// of 26506 positions, 103 splits each: 6.9 us with its events, 48.7 as a loop over them per element.
+constexpr int KV_SPLITS = 256;
 template <typename T, int D>
-__global__ __launch_bounds__(D) void kv_attn_join_kernel(KvAttn a, int64_t rows_all) {
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttn a, int64_t rows_all) {
+  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+  __shared__ float weight[KV_SPLITS], wave_top[4], wave_sum[4];
+  __shared__ float4 rows[256];
   const int64_t at = blockIdx.x;
-  const int d = static_cast<int>(threadIdx.x);
-  float top = KV_FLOOR;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[2 * (s * rows_all + at)]);
-  float sum = 0.f, val = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = fast_exp2(a.part_ml[2 * (s * rows_all + at)] - top);
-    sum += f * a.part_ml[2 * (s * rows_all + at) + 1];
-    val += f * a.part[(s * rows_all + at) * D + d];
+  const int t = static_cast<int>(threadIdx.x), wave = t >> 6;
+  float m = KV_FLOOR, l = 0.f;
+  if (t < a.splits) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (t * rows_all + at));
+    m = ml.x; l = ml.y;
   }
+  float top = m;
+  for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+  if ((t & 63) == 0) wave_top[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
+  const float f = fast_exp2(m - top);
+  weight[t] = f;
+  float sum = f * l;
+  for (int x = 32; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
+  if ((t & 63) == 0) wave_sum[wave] = sum;
+  __syncthreads();
+  const int c = t % LANES, g = t / LANES;
+  float4 val = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = g; s < a.splits; s += GROUPS) {
+    const float4 v = *reinterpret_cast<const float4*>(a.part + (s * rows_all + at) * D + 4 * c);
+    const float w = weight[s];
+    val.x += w * v.x; val.y += w * v.y; val.z += w * v.z; val.w += w * v.w;
+  }
+  rows[t] = val;
+  __syncthreads();
+  if (t >= LANES) return;
+  sum = wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
+  for (int i = 1; i < min(GROUPS, a.splits); ++i) {
+    const float4 v = rows[i * LANES + c];
+    val.x += v.x; val.y += v.y; val.z += v.z; val.w += v.w;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int qrow = static_cast<int>(at % a.rows);
   const int64_t bh = at / a.rows, b = bh / a.kv_heads, kvh = bh % a.kv_heads;
   T* op = static_cast<T*>(a.out) + static_cast<int64_t>(qrow / a.group) * a.o_st + b * a.o_sb + (kvh * a.group + qrow % a.group) * a.o_sh;
-  op[d] = elem<T>::from_float(sum == 0.f ? 0.f : val / sum);
+  const float out[4] = {val.x * inv, val.y * inv, val.z * inv, val.w * inv};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) op[4 * c + i] = elem<T>::from_float(out[i]);
 }
 
 int check_format(const char* what, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t capacity, int bits, int dtype) {
@@ -573,7 +606,7 @@ AttnPlan attn_plan(int64_t tq, int64_t batch, int64_t heads, int64_t kv_heads, i
   const int64_t tiles = (reach + KV_TILE - 1) / KV_TILE;
   if (tiles <= 64) return {8, 1, false};
   const int64_t splits = std::min((4 * num_cus() + blocks - 1) / std::max<int64_t>(blocks, 1), tiles / 8);
-  return {4, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, 256))), true};
+  return {4, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, KV_SPLITS))), true};
 }
 
 }  // namespace
@@ -695,11 +728,11 @@ extern "C" int nmtg_kv_cache_attn(const void* q, int64_t q_stride_t, int64_t q_s
     TraceScope trace("kv_cache_attn_join", st);
     const dim3 rows_grid(static_cast<unsigned>(rows_all));
     if (dtype == NMTG_F16) {
-      if (head_dim == 64) hipLaunchKernelGGL((kv_attn_join_kernel<f16_t, 64>), rows_grid, dim3(64), 0, st, a, rows_all);
-      else hipLaunchKernelGGL((kv_attn_join_kernel<f16_t, 128>), rows_grid, dim3(128), 0, st, a, rows_all);
+      if (head_dim == 64) hipLaunchKernelGGL((kv_attn_join_kernel<f16_t, 64>), rows_grid, dim3(256), 0, st, a, rows_all);
+      else hipLaunchKernelGGL((kv_attn_join_kernel<f16_t, 128>), rows_grid, dim3(256), 0, st, a, rows_all);
     } else {
-      if (head_dim == 64) hipLaunchKernelGGL((kv_attn_join_kernel<bf16_t, 64>), rows_grid, dim3(64), 0, st, a, rows_all);
-      else hipLaunchKernelGGL((kv_attn_join_kernel<bf16_t, 128>), rows_grid, dim3(128), 0, st, a, rows_all);
+      if (head_dim == 64) hipLaunchKernelGGL((kv_attn_join_kernel<bf16_t, 64>), rows_grid, dim3(256), 0, st, a, rows_all);
+      else hipLaunchKernelGGL((kv_attn_join_kernel<bf16_t, 128>), rows_grid, dim3(256), 0, st, a, rows_all);
     }
   }
   NMTG_CHECK_LAUNCH(what);

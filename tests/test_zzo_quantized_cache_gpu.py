@@ -201,6 +201,17 @@ def test_attend(dev, tq, b, h, hk, d, cap, lengths, window, sinks, dtype, bits):
     assert torch.equal(kv_cache_attend(q, *cache, n, cap, window, sinks), kv_cache_attend(q, *cache, n, cap, window, sinks))
 
 
+@pytest.mark.parametrize("d,lengths", [(64, [26000, 3]), (128, [40, 66000])])
+def test_attend_joins_many_parts(dev, d, lengths):
+    """Few rows over long reaches: a hundred parts and the most there are, many of them empty for the short sequence."""
+    cap = max(lengths)
+    cache, k, v = fill(2, 1, cap, d, 8, torch.float16, dev, 9)
+    q = torch.randn(1, 2, 3, d, generator=torch.Generator().manual_seed(8)).to(torch.float16).to(dev)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    want, mag = attend_reference(q, k, v, lengths, 0, 0, d ** -0.5)
+    check(kv_cache_attend(q, *cache, n, cap, 0, 0), want, mag, torch.float16)
+
+
 def test_attend_takes_strided_queries_other_scales_and_long_lengths(dev):
     cache, k, v = fill(2, 2, 100, 64, 8, torch.bfloat16, dev, 3)
     lin = torch.randn(1, 2, 8, 64, device=dev).to(torch.bfloat16)
