@@ -674,8 +674,11 @@ struct DkvPlan {
     // 580 with 16 tiles, 650 with 72). Where they are more: what a block has of its own.
     const int64_t behind = (len - std::min(len, window) + FA_TILE - 1) / FA_TILE * group, chunk = sinks <= 32 ? 8 : tiles * group;
     chunks = sink_blocks > 0 ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((behind + chunk - 1) / chunk, 64))) : 0;
-    // two blocks for every compute unit, each with at least four tiles
-    parts = static_cast<int>(std::max<int64_t>(1, std::min({(2 * num_cus() + blocks * batch * kv_heads - 1) / (blocks * batch * kv_heads), tiles * group / 4, int64_t(16)})));
+    // About two blocks for every compute unit, each with at least four tiles. But the sums of every part of every block pass through
+    // memory in 32 bits, while what a split saves is a block's own tiles: no more parts than 18 tiles per block / blocks (us of dK, dV and
+    // join, head dimension 128: 208 blocks of 12 tiles: 46 in one part, 64 in two; 104 of 24: 52 in three, 47 in four, 53 in five).
+    const int64_t all = std::max<int64_t>(blocks * batch * kv_heads, 1), pairs = tiles * group;
+    parts = static_cast<int>(std::max<int64_t>(1, std::min({(2 * num_cus() + all / 2) / all, pairs / 4, (18 * pairs + all / 2) / all, int64_t(16)})));
     sink_rows = sink_blocks > 0 ? static_cast<int>(std::min(sinks, len)) : 0;
     part_rows = parts > 1 ? static_cast<int>(len) : sink_rows;
     part_floats = batch * kv_heads * parts * part_rows * 2 * head_dim;
