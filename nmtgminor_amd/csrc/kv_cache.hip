@@ -214,6 +214,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRows a) {
 //   neighbouring elements and re-paired by position (one byte permutation per register) they are the operands of D / 16
 //   products.
 // The running maximum follows lazily (it moves when a score exceeds it by 2^8), the sums stay per lane until the end.
+// Memory bounds it, and latency where the cache is short: 856 MB of 32 sequences in 144 us (5.9 TB/s), 5 sequences of 61 positions in 4.4.
 struct KvAttn {
   const void* q;
   const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;

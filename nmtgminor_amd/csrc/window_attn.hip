@@ -8,15 +8,27 @@
 //               dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO   (dK, dV summed over the heads of a group)
 //
 // The tiling is that of the other tiled attention kernels (flash_tile.hip.h): scores as S^T = K Q^T on 32 x 32 x 16 products,
-// one query per lane pair and 32 keys of a tile of 64 in a lane's registers, so that the softmax's maximum and sum are scalars
-// of a lane; probabilities go from accumulators into operands with two lane exchanges per 16 keys. A block visits the tiles
-// that hold sinks, then the tiles from its first query's window to its last query. What is different here:
+// one query per lane pair and 32 keys in a lane's registers, so that the softmax's maximum and sum are scalars of a lane;
+// probabilities go from accumulators into operands with two lane exchanges per 16 keys. A block visits the tiles that hold
+// sinks, then the tiles from its first query's window to its last query. What is different here:
 //   - Tiles go from memory straight into LDS (no registers in between), one tile ahead.
-//   - A tile lies in LDS once and is read both by rows and transposed: chunk c (16 bytes) of row r at position
-//     c ^ (2 (r & 3) | (r >> 2 & 1)). Eight neighbouring rows put one chunk into eight different bank groups (reads by rows),
-//     four neighbouring rows put a pair of chunks into four (transposed reads).
+//   - A tile lies in LDS once and is read both by rows and transposed: the 16-byte chunks of row r change places by an
+//     exclusive-or with img_swizzle(r), under which both kinds of reads spread over all 64 banks (without conflicts; those
+//     counted, 1 to 5% of the LDS cycles, are the output patches').
 //   - A wavefront that sees nothing of a tile skips it; masks are computed only where a tile crosses an edge.
-// No atomics and nothing added up across blocks: results do not depend on scheduling.
+// Backward in two kernels of three and four products, seven where one kernel would do five: summing dQ over the blocks of keys, or dK
+// and dV over those of queries, takes atomics, whose order changes results, or a [blocks, len, head_dim] tensor in 32 bits.
+//
+// Rounding. Scores, the softmax's statistics, D and all sums are in 32 bits. P and dS are rounded to the tensors' type, which the
+// products take: about as much error as rounding the result adds, so that dQ is off by 1.5 times what sums in 32 bits rounded once
+// are. D is that of the rounded O which the forward returns: a second tensor with the rest of O would take 6% off dQ's error,
+// for some 5% of the time of forward and backward, by its traffic.
+//
+// What bounds them (MI355X). Head dimension 128: the products, with matrix cores busy 46 to 54% of the cycles and the vector units most of
+// the others; forward over 16384 positions, window 4096, 32 heads: 965 us, 1.0 PFLOP/s (a large library product: 1.43). Head
+// dimension 64: the vector instructions of the softmax, about 4 cycles of them to 2 of products: 8 x 2048 positions, window 512, 16
+// heads: 75 us forward, 87 dQ, 113 dK and dV.
+// No atomics, and what blocks leave to be added up is added in a fixed order: results do not depend on scheduling.
 #include "flash_tile.hip.h"
 #include <algorithm>
 
@@ -46,7 +58,7 @@ struct WaView { const void* p; int64_t st, sb, sh; };   // [len, batch, heads, h
 struct WaArgs {
   WaView q, k, v, o, d_o, dq, dk, dv;
   float* lse;                // [batch, heads, len]
-  float* stats;              // backward: [batch, heads][2][stat_rows], log-sum-exp in units of log2 and D, rows up to a whole block
+  float* stats;              // backward: [batch, heads][2][stat_rows], log-sum-exp in units of log2 and -D, rows up to a whole block
   int stat_rows;
   const int32_t* lengths;    // [batch] or null: every sequence fills `len`
   int len, batch, heads, kv_heads, group;
@@ -74,7 +86,7 @@ template <int D>
 __device__ __forceinline__ int img_swizzle(int r) { return D == 64 ? (4 * ((r >> 1) & 1) | ((r >> 2) & 3)) : (4 * (r & 3) | ((r >> 2) & 3)); }
 
 // The lane's LDS addresses, which differ between the pieces of an operand by an exclusive-or and a constant: two registers
-// instead of one per piece, which the compiler would keep through the loop (`per tile` hides from it that they do not change).
+// instead of one per piece, which the compiler would keep through the loop (per_tile() hides from it that they do not change).
 template <typename V>
 __device__ __forceinline__ const __attribute__((address_space(3))) V* lds_ptr(uint32_t at) {
   return reinterpret_cast<const __attribute__((address_space(3))) V*>(at);
@@ -82,7 +94,6 @@ __device__ __forceinline__ const __attribute__((address_space(3))) V* lds_ptr(ui
 template <int D>
 struct ImgReader {
   uint32_t rows, columns;
-  ImgReader() = default;
   // base: LDS address of the images, a multiple of 256
   __device__ __forceinline__ ImgReader(uint32_t base, int lane) {
     const int r = lane & 31, rt = 8 * (lane >> 5) + ((lane >> 2) & 3), ct = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
@@ -215,9 +226,10 @@ __device__ __forceinline__ void hide_keys(acc16_t& s, const WaArgs& a, int n, in
 // ------------------------------------------------------------------------------------------------------------- forward
 constexpr float WA_FLOOR = -5e29f;   // a running maximum before the first visible key: finite, and far above the -inf of hidden ones
 
-// Key tiles of 64, or of 32 for head_dim 128: with the scores of 32 keys a wavefront needs 168 registers there, and three of them
+// Key tiles of 64, or of 32 for head_dim 128: with the scores of 32 keys a wavefront needs at most 168 registers there, and three of them
 // share a SIMD (32 KB of LDS a block). What bounds the kernel is how much of the softmax runs under other wavefronts' products:
-// prompt of 16384 positions, window 4096, 32 heads of 128: 1088 us with two wavefronts and tiles of 64, 1023 with three.
+// prompt of 16384 positions, window 4096, 32 heads of 128: 1088 us with two wavefronts and tiles of 64, 965 with three. (For
+// head_dim 64 tiles of 32 keys take as long as tiles of 64.)
 template <int D> constexpr int fwd_tile() { return D == 64 ? 64 : 32; }
 
 template <typename T, int D>
@@ -326,6 +338,8 @@ __global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) 
 }
 
 // ------------------------------------------------------------------------------------ backward: dQ, and D = rowsum(dO O)
+// Queries in registers, tiles of 64 keys and values as in the forward. Head dimension 64: four wavefronts on a SIMD (128 registers, none
+// spilt), 128: two. 2 x 8192 positions, window 1024, 32 heads of 128: 450 us, 0.9 PFLOP/s of its three products.
 template <typename T, int D>
 __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_kernel(WaArgs a) {
   extern __shared__ __align__(256) uint8_t lds_raw[];
@@ -438,9 +452,9 @@ __device__ __forceinline__ void store_part(const acc16_t (&acc)[D / 32], float m
 // Query tiles of 64, or of 32 for head_dim 128: two wavefronts of that size on a SIMD leave 256 registers each, which the
 // accumulators of 32 keys half fill, so the keys of a block are read from LDS (32 KB, which the smaller tiles make room for)
 // and only the values stay in registers. With both in registers there was one wavefront on a SIMD, and nothing ran
-// under the waits of the other: 8192 positions, window 1024, 32 heads of 128: 1178 us against 784.
+// under the waits of the other: 1.5 times the time. 2 x 8192 positions, window 1024, 32 heads of 128: 550 us, 1.0 PFLOP/s of its products.
 template <int D> constexpr int dkv_tile() { return D == 64 ? 64 : 32; }
-template <int D> constexpr int dkv_buf() { return 2 * dkv_tile<D>() * D * 2 + 2 * dkv_tile<D>() * 4; }   // Q, dO, lse2, D
+template <int D> constexpr int dkv_buf() { return 2 * dkv_tile<D>() * D * 2 + 2 * dkv_tile<D>() * 4; }   // Q, dO, lse2, -D
 template <int D> constexpr int dkv_keys() { return D == 64 ? 0 : WA_ROWS * D * 2; }
 
 template <typename T, int D>
@@ -480,7 +494,7 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dkv
   const int i0 = static_cast<int>(static_cast<int64_t>(all) * share / static_cast<int>(shares)), i1 = static_cast<int>(static_cast<int64_t>(all) * (share + 1) / static_cast<int>(shares));
   const TileLoader<T, D, TILE> ldq(a.q.st, wave, lane), ldg(a.d_o.st, wave, lane);
   const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
-  // Beside a tile's rows, what the backward keeps of its queries: log-sum-exp, D. Tiles of 64: 64 floats a transfer, by two
+  // Beside a tile's rows, what the backward keeps of its queries: log-sum-exp, -D. Tiles of 64: 64 floats a transfer, by two
   // wavefronts each (the same values); of 32: both in one, by all four.
   const uint32_t stat_off = TILE == 64 ? static_cast<uint32_t>((wave & 1) * a.stat_rows + lane) * 4 : static_cast<uint32_t>((lane >> 5) * a.stat_rows + (lane & 31)) * 4;
   // (head, tile) of the next transfers and of the next products
