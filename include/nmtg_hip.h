@@ -734,8 +734,9 @@ int nmtg_multi_tensor_l2norm_scale(int n_tensors, const void* const* in, void* c
  * sums in fp32, probabilities and score gradients rounded to the 16-bit type for their products.
  * softmax_lse: fp32 [batch, heads, len], natural logarithm (-inf where nothing is visible), written
  * by the forward and read by the backward. workspace: nmtg_window_attn_bwd_workspace_bytes bytes,
- * 256-byte aligned. An inf or NaN at a position that some query of the same 64 sees may reach the
- * other queries of that tile (zero times it); positions behind a length are never read.
+ * 256-byte aligned. Positions behind a length are never read. An inf or NaN in a row of k or v may
+ * reach, as zero times it, queries that do not see the row but share an aligned 32 with one that sees
+ * some row of the aligned 64 around it; in a row of q or dout, the gradients of keys likewise.
  * ------------------------------------------------------------------------------------------ */
 int nmtg_window_attn_fwd(const void* q, const void* k, const void* v, void* out, float* softmax_lse,
                          const int32_t* lengths, const int64_t* strides, int64_t len, int64_t batch,

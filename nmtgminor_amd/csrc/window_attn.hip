@@ -683,11 +683,14 @@ struct DkvPlan {
     key_blocks = static_cast<int>(blocks);
     // some query stands behind the window of a block's first sinks
     sink_blocks = len > WA_ROWS - 1 + window ? static_cast<int>(std::min(blocks, (std::min(sinks, len) + WA_ROWS - 1) / WA_ROWS)) : 0;
-    // The queries behind, in chunks, up to 64 of a block. Where the sinks are one wavefront's keys, the other three only wait, and what a
-    // chunk leaves behind is small: eight tiles, so that the last chunks of a launch are short (8192 positions, window 1024: 570 us,
-    // 580 with 16 tiles, 650 with 72). Where they are more: what a block has of its own.
-    const int64_t behind = (len - std::min(len, window) + FA_TILE - 1) / FA_TILE * group, chunk = sinks <= 32 ? 8 : tiles * group;
-    chunks = sink_blocks > 0 ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((behind + chunk - 1) / chunk, 64))) : 0;
+    // The queries behind, in chunks of eight tiles: shorter than a block of its own, so that the last ones of a launch end it soon, and where
+    // the sinks are one wavefront's keys the other three only wait (2 x 8192 positions, window 1024, 4 sinks: 570 us, 580 with 16
+    // tiles, 650 with 72; 4096 positions of one key head, 33 sinks: 42, 53, 133). Every chunk leaves the sums of all sinks in 32 bits:
+    // with more than 256 of them twice as long (2048 sinks, 2 x 8192 positions: 210 us, 236 with eight), and no more than 64 chunks or
+    // 32768 rows, but 16 in any case (2048 sinks, 16384 positions: 710 us, 884 with four).
+    const int64_t behind = (len - std::min(len, window) + FA_TILE - 1) / FA_TILE * group, chunk = sinks <= 256 ? 8 : 16;
+    const int64_t most = std::min<int64_t>(64, std::max<int64_t>(16, 32768 / std::max<int64_t>(sinks, 1)));
+    chunks = sink_blocks > 0 ? static_cast<int>(std::max<int64_t>(1, std::min((behind + chunk - 1) / chunk, most))) : 0;
     // About two blocks for every compute unit, each with at least four tiles. But the sums of every part of every block pass through
     // memory in 32 bits, while what a split saves is a block's own tiles: no more parts than 18 tiles per block / blocks (us of dK, dV and
     // join, head dimension 128: 208 blocks of 12 tiles: 46 in one part, 64 in two; 104 of 24: 52 in three, 47 in four, 53 in five).

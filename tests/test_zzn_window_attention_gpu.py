@@ -101,6 +101,14 @@ def test_forward_and_gradients(dev, t, b, h, hk, d, window, sinks, ragged, dtype
         assert torch.equal(window_attn_func(q, k, v, window, sinks, lengths=lengths), out)
 
 
+@pytest.mark.parametrize("t,b,h,hk,d,window,sinks,ragged", [
+    (1500, 1, 4, 1, 64, 40, 2, False),               # a head's sinks in eleven chunks
+    (900, 2, 4, 1, 128, 30, 300, True),              # more sinks than a block's keys, in longer chunks
+])
+def test_sinks_in_many_chunks(dev, t, b, h, hk, d, window, sinks, ragged):
+    test_forward_and_gradients(dev, t, b, h, hk, d, window, sinks, ragged, torch.bfloat16)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.25, 1.0])
 def test_other_scales(dev, scale):
     q, k, v, dout = inputs(90, 1, 2, 2, 64, torch.bfloat16, dev, 3)
