@@ -43,11 +43,18 @@ __device__ __forceinline__ uint32_t xcd_item(uint32_t i, uint32_t total) {
   const uint32_t xcd = i & 7, share = total >> 3, more = total & 7;
   return xcd * share + min(xcd, more) + (i >> 3);
 }
-// Query block x of head h, sequence b: the heads of a group first, then the blocks of the sequence.
+// Query block x of head h, sequence b. First those with a whole window in front of them, the heads of a group together, then the blocks
+// of a sequence; at last the shorter ones, longest first, so that the launch ends evenly (forward, us, before and after: 16384 positions in
+// one window 1259 and 1053, 8 x 2048 positions with a window of 512 80 and 71).
 struct WaBlock { int x, h, b; };
-__device__ __forceinline__ WaBlock query_block(int blocks, int group, int kv_heads) {
-  const uint32_t id = xcd_item(blockIdx.x, gridDim.x), rest = id / group, kv = rest / blocks;
-  return {static_cast<int>(rest % blocks), static_cast<int>(kv % kv_heads * group + id % group), static_cast<int>(kv / kv_heads)};
+__device__ __forceinline__ WaBlock query_block(int blocks, int group, int kv_heads, int window) {
+  const uint32_t all = gridDim.x / blocks, part = min(blocks, (window + WA_ROWS - 1) / WA_ROWS), whole = all * (blocks - part);
+  if (blockIdx.x < whole) {
+    const uint32_t id = xcd_item(blockIdx.x, whole), rest = id / group, kv = rest / (blocks - part);
+    return {static_cast<int>(part + rest % (blocks - part)), static_cast<int>(kv % kv_heads * group + id % group), static_cast<int>(kv / kv_heads)};
+  }
+  const uint32_t id = blockIdx.x - whole, head = id % all, kv = head / group;
+  return {static_cast<int>(part - 1 - id / all), static_cast<int>(kv % kv_heads * group + head % group), static_cast<int>(kv / kv_heads)};
 }
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
@@ -236,7 +243,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) {
   extern __shared__ __align__(256) uint8_t lds_raw[];
   constexpr int TILE = fwd_tile<D>(), IMG = TILE * D * 2;
-  const WaBlock block = query_block((a.len + WA_ROWS - 1) / WA_ROWS, a.group, a.kv_heads);
+  const WaBlock block = query_block((a.len + WA_ROWS - 1) / WA_ROWS, a.group, a.kv_heads, a.window);
   const int b = block.b, h = block.h, q0 = block.x * WA_ROWS;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const int n = seq_len(a, b), bh = b * a.heads + h;
@@ -280,10 +287,16 @@ __global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) 
     for (int nn = 0; nn < TILE / 32; ++nn)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[nn][r] = 0.f;
+    uint4 kf[TILE / 32][D / 16];                                // all read before the first product, which otherwise waits for each in turn
 #pragma unroll
     for (int ss = 0; ss < D / 16; ++ss)
 #pragma unroll
-      for (int nn = 0; nn < TILE / 32; ++nn) mfma<T>::run(img.row_operand(kimg, nn, ss), qf[ss], s[nn]);
+      for (int nn = 0; nn < TILE / 32; ++nn) kf[nn][ss] = img.row_operand(kimg, nn, ss);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ss = 0; ss < D / 16; ++ss)
+#pragma unroll
+      for (int nn = 0; nn < TILE / 32; ++nn) mfma<T>::run(kf[nn][ss], qf[ss], s[nn]);
     if (some_hidden<TILE>(a, n, first, last, k0)) {
 #pragma unroll
       for (int nn = 0; nn < TILE / 32; ++nn) hide_keys(s[nn], a, n, first, qrow, half, k0 + 32 * nn, hidden);
@@ -344,7 +357,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_kernel(WaArgs a) {
   extern __shared__ __align__(256) uint8_t lds_raw[];
   constexpr int IMG = FA_TILE * D * 2;
-  const WaBlock block = query_block((a.len + WA_ROWS - 1) / WA_ROWS, a.group, a.kv_heads);
+  const WaBlock block = query_block((a.len + WA_ROWS - 1) / WA_ROWS, a.group, a.kv_heads, a.window);
   const int b = block.b, h = block.h, q0 = block.x * WA_ROWS;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const int n = seq_len(a, b), bh = b * a.heads + h;
@@ -408,9 +421,16 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_
 #pragma unroll
       for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = D == 128 ? -delta : 0.f; }
 #pragma unroll
-      for (int ss = 0; ss < D / 16; ++ss) {
-        mfma<T>::run(img.row_operand(0, 0, ss), qf[ss], s);
-        mfma<T>::run(img.row_operand(IMG, 0, ss), gf[ss], dp);
+      for (int ss = 0; ss < D / 16; ss += 2) {
+        uint4 kf[2], vf[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) { kf[x] = img.row_operand(0, 0, ss + x); vf[x] = img.row_operand(IMG, 0, ss + x); }
+        if constexpr (D == 128) __builtin_amdgcn_sched_barrier(0);   // four reads ahead: 4%; at head dimension 64 there are no registers for them
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          mfma<T>::run(kf[x], qf[ss + x], s);
+          mfma<T>::run(vf[x], gf[ss + x], dp);
+        }
       }
       hide_keys(s, a, n, first, qrow, half, kn, hidden);
 #pragma unroll
@@ -462,13 +482,24 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dkv
   extern __shared__ __align__(256) uint8_t lds_raw[];
   constexpr int TILE = dkv_tile<D>(), IMG = TILE * D * 2, BUF = dkv_buf<D>();
   constexpr bool KEYS_IN_LDS = dkv_keys<D>() > 0;
-  // the key blocks' parts first, then, shorter and so the ones to end with, the chunks of queries that see a block's keys as sinks only
-  const uint32_t own = static_cast<uint32_t>(a.key_blocks * a.parts), heads = static_cast<uint32_t>(a.kv_heads) * a.batch;
+  // First the parts of key blocks with a whole window of queries behind them, then those of the shorter blocks, longest first, at last
+  // the chunks of queries that see a block's keys as sinks only.
+  const uint32_t heads = static_cast<uint32_t>(a.kv_heads) * a.batch, shorter = min(a.key_blocks, (a.window + WA_ROWS - 1) / WA_ROWS);
+  const uint32_t whole = (a.key_blocks - shorter) * a.parts, own = a.key_blocks * a.parts;
   const bool sink_chunk = blockIdx.x >= own * heads;
-  const uint32_t id = sink_chunk ? xcd_item(blockIdx.x - own * heads, gridDim.x - own * heads) : xcd_item(blockIdx.x, own * heads);
-  const uint32_t per_head = sink_chunk ? static_cast<uint32_t>(a.sink_blocks * a.chunks) : own, shares = sink_chunk ? a.chunks : a.parts;
-  const int h = static_cast<int>(id / per_head % a.kv_heads), b = static_cast<int>(id / per_head / a.kv_heads);
-  const int k0 = static_cast<int>(id % per_head / shares) * WA_ROWS, share = static_cast<int>(id % per_head % shares);
+  uint32_t head, block, share, shares = a.parts;
+  if (sink_chunk) {
+    const uint32_t id = xcd_item(blockIdx.x - own * heads, gridDim.x - own * heads), per_head = a.sink_blocks * a.chunks;
+    shares = a.chunks;
+    head = id / per_head; block = id % per_head / shares; share = id % per_head % shares;
+  } else if (blockIdx.x < whole * heads) {
+    const uint32_t id = xcd_item(blockIdx.x, whole * heads);
+    head = id / whole; block = id % whole / shares; share = id % whole % shares;
+  } else {
+    const uint32_t id = blockIdx.x - whole * heads;
+    share = id % shares; head = id / shares % heads; block = a.key_blocks - shorter + id / shares / heads;
+  }
+  const int h = static_cast<int>(head % a.kv_heads), b = static_cast<int>(head / a.kv_heads), k0 = static_cast<int>(block) * WA_ROWS;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const int n = seq_len(a, b), kw = k0 + 32 * wave, krow = kw + (lane & 31);
   uint4 kf[KEYS_IN_LDS ? 1 : D / 16], vf[D / 16];
@@ -691,11 +722,15 @@ struct DkvPlan {
     const int64_t behind = (len - std::min(len, window) + FA_TILE - 1) / FA_TILE * group, chunk = sinks <= 256 ? 8 : 16;
     const int64_t most = std::min<int64_t>(64, std::max<int64_t>(16, 32768 / std::max<int64_t>(sinks, 1)));
     chunks = sink_blocks > 0 ? static_cast<int>(std::max<int64_t>(1, std::min((behind + chunk - 1) / chunk, most))) : 0;
-    // About two blocks for every compute unit, each with at least four tiles. But the sums of every part of every block pass through
-    // memory in 32 bits, while what a split saves is a block's own tiles: no more parts than 18 tiles per block / blocks (us of dK, dV and
-    // join, head dimension 128: 208 blocks of 12 tiles: 46 in one part, 64 in two; 104 of 24: 52 in three, 47 in four, 53 in five).
+    // About two blocks for every compute unit, each with at least four tiles; four where most blocks are shorter than a whole window's,
+    // so that the short ones even out the long (8192 positions in one window, 512 blocks of up to 516 tiles: 1480 us in one part, 1100
+    // in two), if they are long enough (128 blocks of up to 48 tiles: 61 us in four parts, 84 in seven). But the sums of every part of
+    // every block pass through memory in 32 bits, while what a split saves is a block's own tiles: no more parts than 18 tiles per block
+    // / blocks (us of dK, dV and join, head dimension 128: 208 blocks of 12 tiles: 46 in one part, 64 in two; 104 of 24: 52 in three,
+    // 47 in four, 53 in five).
     const int64_t all = std::max<int64_t>(blocks * batch * kv_heads, 1), pairs = tiles * group;
-    parts = static_cast<int>(std::max<int64_t>(1, std::min({(2 * num_cus() + all / 2) / all, pairs / 4, (18 * pairs + all / 2) / all, int64_t(16)})));
+    const int64_t fill = (2 * std::min(blocks, (window + WA_ROWS - 1) / WA_ROWS) > blocks && pairs >= 96 ? 4 : 2) * num_cus();
+    parts = static_cast<int>(std::max<int64_t>(1, std::min({(fill + all / 2) / all, pairs / 4, (18 * pairs + all / 2) / all, int64_t(16)})));
     sink_rows = sink_blocks > 0 ? static_cast<int>(std::min(sinks, len)) : 0;
     part_rows = parts > 1 ? static_cast<int>(len) : sink_rows;
     part_floats = batch * kv_heads * parts * part_rows * 2 * head_dim;
