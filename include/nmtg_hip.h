@@ -732,14 +732,17 @@ int nmtg_multi_tensor_l2norm_scale(int n_tensors, const void* const* in, void* c
  * 8; head_dim contiguous), in the order of the tensor arguments: q, k, v, out for the forward and
  * dout, q, k, v, out, dq, dk, dv for the backward. head_dim 64 or 128, fp16 or bf16, products and
  * sums in fp32, probabilities and score gradients rounded to the 16-bit type for their products.
+ * out_rest: what rounding took from out, in 8 bits and an order of its own: batch * heads *
+ * ceil(len / 32) * 32 * head_dim bytes, 16-byte aligned, written by the forward where it is not null
+ * and read by the backward; without it (null) the backward takes dout . out from the rounded out.
  * softmax_lse: fp32 [batch, heads, len], natural logarithm (-inf where nothing is visible), written
  * by the forward and read by the backward. workspace: nmtg_window_attn_bwd_workspace_bytes bytes,
  * 256-byte aligned. Positions behind a length are never read. An inf or NaN in a row of k or v may
  * reach, as zero times it, queries that do not see the row but share an aligned 32 with one that sees
  * some row of the aligned 64 around it; in a row of q or dout, the gradients of keys likewise.
  * ------------------------------------------------------------------------------------------ */
-int nmtg_window_attn_fwd(const void* q, const void* k, const void* v, void* out, float* softmax_lse,
-                         const int32_t* lengths, const int64_t* strides, int64_t len, int64_t batch,
+int nmtg_window_attn_fwd(const void* q, const void* k, const void* v, void* out, uint8_t* out_rest,
+                         float* softmax_lse, const int32_t* lengths, const int64_t* strides, int64_t len, int64_t batch,
                          int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window,
                          int64_t sinks, float softmax_scale, int dtype, void* stream);
 
@@ -748,10 +751,10 @@ int64_t nmtg_window_attn_bwd_workspace_bytes(int64_t len, int64_t batch, int64_t
                                              int64_t sinks);
 
 int nmtg_window_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
-                         const void* out, const float* softmax_lse, void* dq, void* dk, void* dv,
-                         const int32_t* lengths, const int64_t* strides, int64_t len, int64_t batch,
-                         int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window,
-                         int64_t sinks, float softmax_scale, int dtype, void* workspace,
+                         const void* out, const uint8_t* out_rest, const float* softmax_lse, void* dq,
+                         void* dk, void* dv, const int32_t* lengths, const int64_t* strides,
+                         int64_t len, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                         int64_t window, int64_t sinks, float softmax_scale, int dtype, void* workspace,
                          int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------

@@ -14,6 +14,7 @@ struct Window {
   int64_t window, sinks;
   double scale;
   Tensor lengths;
+  bool gradient = false;          // whether the backward will be run
 };
 
 // [len, batch, heads, head_dim] with a contiguous head_dim, 16-byte aligned, strides the kernels take; anything else is copied
@@ -27,15 +28,15 @@ void put_strides(int64_t* to, const Tensor& x) {
 }
 const int32_t* lengths_of(const Tensor& t) { return t.defined() ? t.data_ptr<int32_t>() : nullptr; }
 
-struct Forward { Tensor out, lse; };
+struct Forward { Tensor out, rest, lse; };
 Forward window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Window& w) {
   const int64_t t = q.size(0), b = q.size(1), h = q.size(2), d = q.size(3);
   Launch on(q);
-  Forward r{empty_like_sized(q, {t, b, h, d}), empty_as(q, {b, h, t}, at::kFloat)};
+  Forward r{empty_like_sized(q, {t, b, h, d}), w.gradient ? empty_as(q, {b, h, (t + 31) / 32 * 32, d}, at::kByte) : Tensor(), empty_as(q, {b, h, t}, at::kFloat)};
   int64_t strides[12];
   const Tensor* tensors[4] = {&q, &k, &v, &r.out};
   for (int i = 0; i < 4; ++i) put_strides(strides + 3 * i, *tensors[i]);
-  check(api.window_attn_fwd(ptr(q), ptr(k), ptr(v), ptr(r.out), r.lse.data_ptr<float>(), lengths_of(w.lengths), strides, t, b, h, k.size(2), d,
+  check(api.window_attn_fwd(ptr(q), ptr(k), ptr(v), ptr(r.out), w.gradient ? r.rest.data_ptr<uint8_t>() : nullptr, r.lse.data_ptr<float>(), lengths_of(w.lengths), strides, t, b, h, k.size(2), d,
                             w.window, w.sinks, static_cast<float>(w.scale), dtype_code(q), on.stream), "nmtg_window_attn_fwd");
   return r;
 }
@@ -48,7 +49,7 @@ void window_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tens
   const Tensor* tensors[8] = {&dout, &q, &k, &v, &f.out, &dq, &dk, &dv};
   for (int i = 0; i < 8; ++i) put_strides(strides + 3 * i, *tensors[i]);
   const Scratch ws(q, std::max<int64_t>(api.window_attn_bwd_workspace_bytes(t, b, h, hk, d, w.window, w.sinks), 16));
-  check(api.window_attn_bwd(ptr(dout), ptr(q), ptr(k), ptr(v), ptr(f.out), f.lse.data_ptr<float>(), ptr(dq), ptr(dk), ptr(dv),
+  check(api.window_attn_bwd(ptr(dout), ptr(q), ptr(k), ptr(v), ptr(f.out), f.rest.data_ptr<uint8_t>(), f.lse.data_ptr<float>(), ptr(dq), ptr(dk), ptr(dv),
                             lengths_of(w.lengths), strides, t, b, h, hk, d, w.window, w.sinks, static_cast<float>(w.scale), dtype_code(q), ws.get(),
                             ws.bytes, on.stream), "nmtg_window_attn_bwd");
 }
@@ -59,21 +60,21 @@ void keep(AutogradContext* ctx, const Window& w) {
   ctx->saved_data["s"] = w.scale;
 }
 Window kept(AutogradContext* ctx, const Tensor& lengths) {
-  return {ctx->saved_data["w"].toInt(), ctx->saved_data["n"].toInt(), ctx->saved_data["s"].toDouble(), lengths};
+  return {ctx->saved_data["w"].toInt(), ctx->saved_data["n"].toInt(), ctx->saved_data["s"].toDouble(), lengths, true};
 }
 
 struct WindowNode : Function<WindowNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Window* w) {
     Forward r = window_fwd(q, k, v, *w);
     keep(ctx, *w);
-    ctx->save_for_backward({q, k, v, r.out, r.lse, w->lengths});
+    ctx->save_for_backward({q, k, v, r.out, r.rest, r.lse, w->lengths});
     return r.out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     auto s = ctx->get_saved_variables();
     const Tensor &q = s[0], &k = s[1], &v = s[2];
     Tensor dq = empty_like_sized(q, q.sizes()), dk = empty_like_sized(k, k.sizes()), dv = empty_like_sized(v, v.sizes());
-    window_bwd(view_of(g[0]), q, k, v, {s[3], s[4]}, dq, dk, dv, kept(ctx, s[5]));
+    window_bwd(view_of(g[0]), q, k, v, {s[3], s[4], s[5]}, dq, dk, dv, kept(ctx, s[6]));
     return {dq, dk, dv, Tensor()};
   }
 };
@@ -94,7 +95,7 @@ struct WindowProjectionNode : Function<WindowProjectionNode> {
     keep(ctx, *w);
     ctx->saved_data["h"] = heads;
     ctx->saved_data["k"] = kv_heads;
-    ctx->save_for_backward({lin, r.out, r.lse, w->lengths});
+    ctx->save_for_backward({lin, r.out, r.rest, r.lse, w->lengths});
     return r.out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -102,7 +103,7 @@ struct WindowProjectionNode : Function<WindowProjectionNode> {
     const int64_t heads = ctx->saved_data["h"].toInt(), kv_heads = ctx->saved_data["k"].toInt();
     Tensor dlin = empty_like_sized(s[0], s[0].sizes());
     const Slots x = slots_of(s[0], heads, kv_heads), d = slots_of(dlin, heads, kv_heads);
-    window_bwd(view_of(g[0]), x.q, x.k, x.v, {s[1], s[2]}, d.q, d.k, d.v, kept(ctx, s[3]));
+    window_bwd(view_of(g[0]), x.q, x.k, x.v, {s[1], s[2], s[3]}, d.q, d.k, d.v, kept(ctx, s[4]));
     return {dlin, Tensor(), Tensor(), Tensor()};
   }
 };
@@ -110,7 +111,7 @@ struct WindowProjectionNode : Function<WindowProjectionNode> {
 Window window_args(const Tensor& q, int64_t batch, int64_t head_dim, int64_t window, int64_t sinks, optional<double> scale, const optional<Tensor>& lengths) {
   TORCH_CHECK(window >= 1, "window attention: a window of ", window, " positions (at least 1)");
   TORCH_CHECK(sinks >= 0, "window attention: ", sinks, " sinks");
-  Window w{window, sinks, scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(head_dim)), Tensor()};
+  Window w{window, sinks, scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(head_dim)), Tensor(), false};
   if (lengths.has_value() && lengths->defined()) {
     check_device(*lengths, q);
     TORCH_CHECK(lengths->dim() == 1 && lengths->size(0) == batch, "window attention: lengths must be [batch]");
@@ -168,11 +169,12 @@ void define_long_context(pybind11::module_& m) {
                 "window attention: k and v must have q's positions, batch and head dimension");
     TORCH_CHECK(k.size(2) > 0 && q.size(2) % k.size(2) == 0, "window attention: ", q.size(2), " query heads do not share ", k.size(2),
                 " key / value heads evenly");
-    const Window w = window_args(q, q.size(1), q.size(3), window, sinks, scale, lengths);
+    Window w = window_args(q, q.size(1), q.size(3), window, sinks, scale, lengths);
     if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad())) {
       TORCH_CHECK(!forward_mode() || !(has_tangent(q) || has_tangent(k) || has_tangent(v)), "window attention: jvp is not implemented");
       return window_fwd(view_of(q), view_of(k), view_of(v), w).out;
     }
+    w.gradient = true;
     return WindowNode::apply(view_of(q), view_of(k), view_of(v), &w);
   });
   m.def("window_attention_projection", [](const Tensor& lin, int64_t heads, int64_t kv_heads, int64_t window, int64_t sinks, optional<double> scale,
@@ -180,7 +182,8 @@ void define_long_context(pybind11::module_& m) {
     check_half(lin, "window attention");
     TORCH_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && lin.dim() == 3 && lin.size(2) % (8 * (heads + 2 * kv_heads)) == 0,
                 "window attention: a projection [T, B, (H + 2 H_kv) D] whose heads share key / value heads evenly");
-    const Window w = window_args(lin, lin.size(1), lin.size(2) / (heads + 2 * kv_heads), window, sinks, scale, lengths);
+    Window w = window_args(lin, lin.size(1), lin.size(2) / (heads + 2 * kv_heads), window, sinks, scale, lengths);
+    w.gradient = at::GradMode::is_enabled() && lin.requires_grad();
     return WindowProjectionNode::apply(contiguous(lin), heads, kv_heads, &w);
   });
   m.def("kv_cache_write", [](const Tensor& kc, const Tensor& ks, const Tensor& vc, const Tensor& vs, const Tensor& k, const Tensor& v, const optional<Tensor>& starts,

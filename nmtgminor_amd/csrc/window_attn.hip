@@ -20,9 +20,9 @@
 // and dV over those of queries, takes atomics, whose order changes results, or a [blocks, len, head_dim] tensor in 32 bits.
 //
 // Rounding. Scores, the softmax's statistics, D and all sums are in 32 bits. P and dS are rounded to the tensors' type, which the
-// products take: about as much error as rounding the result adds, so that dQ is off by 1.5 times what sums in 32 bits rounded once
-// are. D is that of the rounded O which the forward returns: a second tensor with the rest of O would take 6% off dQ's error,
-// for some 5% of the time of forward and backward, by its traffic.
+// products take: about as much error as rounding the result adds, so that gradients are off by 1.4 times what sums in 32 bits
+// rounded once are. D is that of O before its rounding: the forward of a training step leaves what the rounding took in 8 bits
+// per element (D of the rounded O alone: 1.5 times the error, in 98% of the time of forward and backward).
 //
 // What bounds them (MI355X). Head dimension 128: the products, with matrix cores busy 46 to 54% of the cycles and the vector units most of
 // the others; forward over 16384 positions, window 4096, 32 heads: 965 us, 1.0 PFLOP/s (a large library product: 1.43). Head
@@ -57,6 +57,9 @@ __device__ __forceinline__ WaBlock query_block(int blocks, int group, int kv_hea
   return {static_cast<int>(part - 1 - id / all), static_cast<int>(kv % kv_heads * group + head % group), static_cast<int>(kv / kv_heads)};
 }
 
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
@@ -64,6 +67,7 @@ struct WaView { const void* p; int64_t st, sb, sh; };   // [len, batch, heads, h
 
 struct WaArgs {
   WaView q, k, v, o, d_o, dq, dk, dv;
+  uint8_t* rest;             // what rounding took from o, or null: see rest_at()
   float* lse;                // [batch, heads, len]
   float* stats;              // backward: [batch, heads][2][stat_rows], log-sum-exp in units of log2 and -D, rows up to a whole block
   int stat_rows;
@@ -86,6 +90,33 @@ __device__ __forceinline__ T* out_head(const WaView& x, int b, int h) { return c
 
 __device__ __forceinline__ int seq_len(const WaArgs& a, int b) {
   return a.lengths != nullptr ? min(max(a.lengths[b], 0), a.len) : a.len;
+}
+
+// ---- what rounding took from O ----
+// In 8 bits (E4M3, a sixteenth of it at most is lost again) times a power of two that leaves room for |O| up to 7: 32 rows of a head by
+// column chunks of 8, [batch, heads, ceil(len / 32)][head_dim / 8][32][8] bytes, which the accumulators' lanes write and the queries'
+// lanes read in whole lines without going through LDS.
+template <int D>
+__device__ __forceinline__ uint8_t* rest_at(const WaArgs& a, int bh, int row0, int row) {
+  return a.rest + ((static_cast<int64_t>(bh) * ((a.len + 31) / 32) + row0 / 32) * (D / 8) * 32 + row) * 8;
+}
+template <typename T> constexpr float rest_scale() { return elem<T>::dtype == NMTG_BF16 ? 0x1p-14f : 0x1p-17f; }
+template <typename T>
+__device__ __forceinline__ uint32_t rest_word(uint32_t lo, uint32_t hi) {
+  s16x2_t w = {0, 0};
+  if constexpr (elem<T>::dtype == NMTG_BF16) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2_t, lo), rest_scale<T>(), false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2_t, hi), rest_scale<T>(), true);
+  } else {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2_t, lo), rest_scale<T>(), false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2_t, hi), rest_scale<T>(), true);
+  }
+  return __builtin_bit_cast(uint32_t, w);
+}
+template <typename T, bool HIGH>
+__device__ __forceinline__ uint32_t rest_pair(uint32_t word) {
+  if constexpr (elem<T>::dtype == NMTG_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, rest_scale<T>(), HIGH));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, rest_scale<T>(), HIGH));
 }
 
 // ---- the LDS image ----
@@ -250,15 +281,6 @@ __global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) 
   const int end = min(q0 + WA_ROWS, n), qw = q0 + 32 * wave, qrow = qw + (lane & 31);
   const T *kb = at_head<T>(a.k, b, h / a.group), *vb = at_head<T>(a.v, b, h / a.group);
 
-  uint4 qf[D / 16];
-  load_resident<T, D>(qf, at_head<T>(a.q, b, h), a.q.st, qrow, n, lane);
-  acc16_t o[D / 32];
-  float m = WA_FLOOR, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-  registers_landed(qf);
   const TileList<TILE> tiles(a, q0, end > q0 ? end : 0);
   const int count = end > q0 ? tiles.count : 0;
   const TileLoader<T, D, TILE> ldk(a.k.st, wave, lane), ldv(a.v.st, wave, lane);
@@ -270,7 +292,16 @@ __global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) 
     ldk.start(kb, a.k.st, row, n - 1, to);
     ldv.start(vb, a.v.st, row, n - 1, to + IMG);
   };
-  if (count > 0) start(0, 0);
+  if (count > 0) start(0, 0);                                    // before the queries: the two latencies are one
+  uint4 qf[D / 16];
+  load_resident<T, D>(qf, at_head<T>(a.q, b, h), a.q.st, qrow, n, lane);
+  acc16_t o[D / 32];
+  float m = WA_FLOOR, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+  registers_landed(qf);
   const int first = qw, last = qw + 31;                         // the wavefront's queries
   const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
   constexpr uint32_t ONES = elem<T>::dtype == NMTG_BF16 ? 0x3f803f80u : 0x3c003c00u;
@@ -347,6 +378,19 @@ __global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) 
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (half == 0 && qrow < a.len)
     a.lse[static_cast<int64_t>(bh) * a.len + qrow] = sum > 0.f ? (m + log2f(sum)) * (1.0f / FA_LOG2E) : sum == 0.f ? -INFINITY : sum;
+  if (a.rest != nullptr && qw < a.len) {
+    uint8_t* to = rest_at<D>(a, bh, qw, lane & 31) + 4 * half;
+#pragma unroll
+    for (int m = 0; m < D / 8; ++m) {
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float whole = o[m / 4][4 * (m % 4) + e] * inv;
+        x[e] = whole - elem<T>::to_float(elem<T>::from_float(whole));
+      }
+      *reinterpret_cast<uint32_t*>(to + 256 * m) = rest_word<T>(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+    }
+  }
   store_rows_out<T, D>(o, inv, lds_raw + wave * (32 * D * 2), out_head<T>(a.o, b, h), a.o.st, qw, a.len, lane);
 }
 
@@ -375,23 +419,37 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_
     ldk.start(kb, a.k.st, row, n - 1, to);
     ldv.start(vb, a.v.st, row, n - 1, to + IMG);
   };
+  if (count > 0) start(0);
   uint4 qf[D / 16], gf[D / 16];
   load_resident<T, D>(qf, at_head<T>(a.q, b, h), a.q.st, qrow, n, lane);
   load_resident<T, D>(gf, at_head<T>(a.d_o, b, h), a.d_o.st, qrow, n, lane);
   float delta = 0.f, lse2 = -FA_NEG;                            // rows behind the end: probability 0
   {
     uint4 of[D / 16];
+    uint2 rf[D / 16];
     load_resident<T, D>(of, at_head<T>(a.o, b, h), a.o.st, qrow, n, lane);
+    const bool more = a.rest != nullptr && qrow < n;
+    if (more) {
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) rf[s] = *reinterpret_cast<const uint2*>(rest_at<D>(a, bh, qw, lane & 31) + 256 * (2 * s + half));
+    }
+    if (qrow < n) {
+      const float v = a.lse[static_cast<int64_t>(bh) * a.len + qrow];
+      lse2 = v == -INFINITY ? -FA_NEG : v * FA_LOG2E;
+    }
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
       delta = dot2<T>(of[s].x, gf[s].x, dot2<T>(of[s].y, gf[s].y, delta));
       delta = dot2<T>(of[s].z, gf[s].z, dot2<T>(of[s].w, gf[s].w, delta));
     }
-    delta = pair_sum(delta);
-    if (qrow < n) {
-      const float v = a.lse[static_cast<int64_t>(bh) * a.len + qrow];
-      lse2 = v == -INFINITY ? -FA_NEG : v * FA_LOG2E;
+    if (more) {
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        delta = dot2<T>(rest_pair<T, false>(rf[s].x), gf[s].x, dot2<T>(rest_pair<T, true>(rf[s].x), gf[s].y, delta));
+        delta = dot2<T>(rest_pair<T, false>(rf[s].y), gf[s].z, dot2<T>(rest_pair<T, true>(rf[s].y), gf[s].w, delta));
+      }
     }
+    delta = pair_sum(delta);
     // for the kernel of dK and dV: whole blocks of rows, so that it reads tiles without looking at lengths
     float* to = a.stats + static_cast<int64_t>(bh) * 2 * a.stat_rows + qrow;
     if (half == 0) to[0] = lse2;
@@ -403,7 +461,6 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
   registers_landed(qf);
-  if (count > 0) start(0);
   const int first = qw, last = qw + 31;
   const float hidden = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
   for (int i = 0; i < count; ++i) {
@@ -502,15 +559,8 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dkv
   const int h = static_cast<int>(head % a.kv_heads), b = static_cast<int>(head / a.kv_heads), k0 = static_cast<int>(block) * WA_ROWS;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const int n = seq_len(a, b), kw = k0 + 32 * wave, krow = kw + (lane & 31);
-  uint4 kf[KEYS_IN_LDS ? 1 : D / 16], vf[D / 16];
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_raw)));
   const ImgReader<D> reader(lds0, lane);
-  if constexpr (KEYS_IN_LDS) {
-    if (k0 < n) TileLoader<T, D, WA_ROWS>(a.k.st, wave, lane).start(at_head<T>(a.k, b, h), a.k.st, k0, n - 1, lds0 + 2 * BUF);
-  } else {
-    load_resident<T, D>(kf, at_head<T>(a.k, b, h), a.k.st, krow, n, lane);
-  }
-  load_resident<T, D>(vf, at_head<T>(a.v, b, h), a.v.st, krow, n, lane);
   acc16_t dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
@@ -542,8 +592,15 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 3 : 2) void window_bwd_dkv
     ldg.start(at_head<T>(a.d_o, b, hq), a.d_o.st, q0, n - 1, to + IMG);
     dma4(stat_off, a.stats + (static_cast<int64_t>(b) * a.heads + hq) * 2 * a.stat_rows + q0, to + 2 * IMG + (TILE == 64 ? (wave & 1) * 256 : 0));
   };
-  wait_vmcnt<0>();      // the resident rows: waited for at their first use, they would be in every tile, behind its transfers
   if (i0 < i1) start(0);
+  uint4 kf[KEYS_IN_LDS ? 1 : D / 16], vf[D / 16];
+  if constexpr (KEYS_IN_LDS) {
+    if (k0 < n) TileLoader<T, D, WA_ROWS>(a.k.st, wave, lane).start(at_head<T>(a.k, b, h), a.k.st, k0, n - 1, lds0 + 2 * BUF);
+  } else {
+    load_resident<T, D>(kf, at_head<T>(a.k, b, h), a.k.st, krow, n, lane);
+  }
+  load_resident<T, D>(vf, at_head<T>(a.v, b, h), a.v.st, krow, n, lane);
+  wait_vmcnt<0>();      // the resident rows: waited for at their first use, they would be in every tile, behind its transfers
   const auto visit = [&](int i, auto buffer) __attribute__((always_inline)) {
     const int q0 = here.tile * TILE;
     advance(here);
@@ -765,18 +822,20 @@ int bwd_launch(const WaArgs& a, hipStream_t st) {
 
 using namespace nmtg;
 
-extern "C" int nmtg_window_attn_fwd(const void* q, const void* k, const void* v, void* out, float* softmax_lse, const int32_t* lengths,
-                                    const int64_t* strides, int64_t len, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+extern "C" int nmtg_window_attn_fwd(const void* q, const void* k, const void* v, void* out, uint8_t* out_rest, float* softmax_lse,
+                                    const int32_t* lengths, const int64_t* strides, int64_t len, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                     int64_t window, int64_t sinks, float softmax_scale, int dtype, void* stream) {
   const char* what = "window_attn_fwd";
   if (int rc = check_call(what, len, batch, heads, kv_heads, head_dim, window, sinks, softmax_scale, dtype)) return rc;
   if (len == 0 || batch == 0) return 0;
   NMTG_REQUIRE(q && k && v && out && softmax_lse && strides, "%s: null pointer argument", what);
+  NMTG_REQUIRE(aligned16(out_rest), "%s: out_rest must be 16-byte aligned", what);
   WaView views[4];
   const void* pointers[4] = {q, k, v, out};
   if (int rc = check_views(what, views, pointers, strides, 4)) return rc;
   WaArgs a = {};
   a.q = views[0]; a.k = views[1]; a.v = views[2]; a.o = views[3];
+  a.rest = out_rest;
   a.lse = softmax_lse; a.lengths = lengths; a.len = static_cast<int>(len); a.batch = static_cast<int>(batch); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
   a.group = static_cast<int>(heads / kv_heads); a.window = static_cast<int>(std::min(window, len + 1)); a.sinks = static_cast<int>(std::min(sinks, len)); a.scale = softmax_scale; a.scale_log2 = log2_scale(softmax_scale);
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -796,14 +855,15 @@ extern "C" int64_t nmtg_window_attn_bwd_workspace_bytes(int64_t len, int64_t bat
   return (stat_floats(len, batch, heads) + plan.part_floats + plan.sink_floats) * static_cast<int64_t>(sizeof(float));
 }
 
-extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* softmax_lse,
-                                    void* dq, void* dk, void* dv, const int32_t* lengths, const int64_t* strides, int64_t len,
+extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const uint8_t* out_rest,
+                                    const float* softmax_lse, void* dq, void* dk, void* dv, const int32_t* lengths, const int64_t* strides, int64_t len,
                                     int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window, int64_t sinks,
                                     float softmax_scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "window_attn_bwd";
   if (int rc = check_call(what, len, batch, heads, kv_heads, head_dim, window, sinks, softmax_scale, dtype)) return rc;
   if (len == 0 || batch == 0) return 0;
   NMTG_REQUIRE(dout && q && k && v && out && softmax_lse && dq && dk && dv && strides, "%s: null pointer argument", what);
+  NMTG_REQUIRE(aligned16(out_rest), "%s: out_rest must be 16-byte aligned", what);
   NMTG_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 &&
                    workspace_bytes >= nmtg_window_attn_bwd_workspace_bytes(len, batch, heads, kv_heads, head_dim, window, sinks),
                "%s: a 256-byte aligned workspace of nmtg_window_attn_bwd_workspace_bytes bytes required", what);
@@ -812,6 +872,7 @@ extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void*
   if (int rc = check_views(what, views, pointers, strides, 8)) return rc;
   WaArgs a = {};
   a.d_o = views[0]; a.q = views[1]; a.k = views[2]; a.v = views[3]; a.o = views[4]; a.dq = views[5]; a.dk = views[6]; a.dv = views[7];
+  a.rest = const_cast<uint8_t*>(out_rest);
   a.lse = const_cast<float*>(softmax_lse); a.stats = static_cast<float*>(workspace);
   a.stat_rows = stat_rows(len);
   const DkvPlan plan(len, batch, heads, kv_heads, head_dim, window, sinks);

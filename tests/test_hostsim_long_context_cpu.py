@@ -57,14 +57,19 @@ def strides(*tensors):
     return (ctypes.c_int64 * len(flat))(*flat)
 
 
+def rest_of(q):
+    t, b, h, d = q.shape
+    return torch.full((b * h * ((t + 31) // 32) * 32 * d,), 0x7f, dtype=torch.uint8)          # NaN where nothing is written
+
+
 def window(lib, q, k, v, dout, lengths, w, sinks, scale, dtype):
     t, b, h, d = q.shape
     sizes = (t, b, h, k.shape[2], d, w, sinks)
-    out, lse = torch.full_like(q, float("nan")), torch.full((b, h, t), float("nan"))
-    call(lib, "window_attn_fwd", q, k, v, out, lse, lengths, strides(q, k, v, out), *sizes, scale, _lib.dtype_code(dtype))
+    out, rest, lse = torch.full_like(q, float("nan")), rest_of(q), torch.full((b, h, t), float("nan"))
+    call(lib, "window_attn_fwd", q, k, v, out, rest, lse, lengths, strides(q, k, v, out), *sizes, scale, _lib.dtype_code(dtype))
     grads = [torch.full_like(x, float("nan")) for x in (q, k, v)]
     ws = bytes256(call(lib, "window_attn_bwd_workspace_bytes", *sizes))
-    call(lib, "window_attn_bwd", dout, q, k, v, out, lse, *grads, lengths, strides(dout, q, k, v, out, *grads), *sizes, scale, _lib.dtype_code(dtype),
+    call(lib, "window_attn_bwd", dout, q, k, v, out, rest, lse, *grads, lengths, strides(dout, q, k, v, out, *grads), *sizes, scale, _lib.dtype_code(dtype),
          ws, ws.numel())
     return [out, *grads]
 
@@ -108,12 +113,12 @@ def test_window_attention_of_slots(lib):
     q, k, v = lin.split((h, hk, hk), 2)
     dout = torch.randn(t, b, h, d).to(BF16)
     dense = window(lib, q.contiguous(), k.contiguous(), v.contiguous(), dout, None, 9, 2, 0.125, BF16)
-    out, lse = torch.empty(t, b, h, d, dtype=BF16), torch.empty(b, h, t)
+    out, rest, lse = torch.empty(t, b, h, d, dtype=BF16), rest_of(q), torch.empty(b, h, t)
     sizes = (t, b, h, hk, d, 9, 2)
-    call(lib, "window_attn_fwd", q, k, v, out, lse, None, strides(q, k, v, out), *sizes, 0.125, _lib.BF16)
+    call(lib, "window_attn_fwd", q, k, v, out, rest, lse, None, strides(q, k, v, out), *sizes, 0.125, _lib.BF16)
     ws = bytes256(call(lib, "window_attn_bwd_workspace_bytes", *sizes))
     grads = dlin.split((h, hk, hk), 2)
-    call(lib, "window_attn_bwd", dout, q, k, v, out, lse, *grads, None, strides(dout, q, k, v, out, *grads), *sizes, 0.125, _lib.BF16, ws, ws.numel())
+    call(lib, "window_attn_bwd", dout, q, k, v, out, rest, lse, *grads, None, strides(dout, q, k, v, out, *grads), *sizes, 0.125, _lib.BF16, ws, ws.numel())
     for x, y in zip((out, *grads), dense):
         assert torch.equal(x, y)
 
@@ -127,15 +132,15 @@ def test_window_attention_refuses(lib):
         c = {**good, **change}
         st = c.pop("strides", strides(q, k, v, out))
         p = c.pop("q", q)
-        return call(lib, "window_attn_fwd", p, k, v, out, lse, None, st, *c.values(), expect=c.pop("rc", -1))
+        return call(lib, "window_attn_fwd", p, k, v, out, None, lse, None, st, *c.values(), expect=c.pop("rc", -1))
     for change, text in ((dict(d=32), "head dimension 32"), (dict(h=3, hk=2), "evenly"), (dict(w=0), "window 0"), (dict(s=-1), "sinks -1"),
                          (dict(dtype=_lib.F32), "fp16 or bf16"), (dict(scale=float("nan")), "scale"), (dict(t=-1), "bad shape"),
                          (dict(b=70000), "65535"), (dict(q=None), "null pointer"), (dict(strides=(ctypes.c_int64 * 12)(*([4] * 12))), "multiples of 8")):
         assert text in run(**change)
     grads = [torch.empty_like(x) for x in (q, k, v)]
-    assert "workspace" in call(lib, "window_attn_bwd", dout, q, k, v, out, lse, *grads, None, strides(dout, q, k, v, out, *grads), 4, 1, 2, 1, 64, 3, 0, 0.125,
+    assert "workspace" in call(lib, "window_attn_bwd", dout, q, k, v, out, None, lse, *grads, None, strides(dout, q, k, v, out, *grads), 4, 1, 2, 1, 64, 3, 0, 0.125,
                                _lib.BF16, bytes256(64), 16, expect=-1)
-    call(lib, "window_attn_fwd", None, None, None, None, None, None, None, 0, 1, 2, 1, 64, 3, 0, 0.125, _lib.BF16)      # nothing to do
+    call(lib, "window_attn_fwd", None, None, None, None, None, None, None, None, 0, 1, 2, 1, 64, 3, 0, 0.125, _lib.BF16)      # nothing to do
 
 
 # ------------------------------------------------------------------------------------------------------ quantised cache
