@@ -24,10 +24,10 @@
 // rounded once are. D is that of O before its rounding: the forward of a training step leaves what the rounding took in 8 bits
 // per element (D of the rounded O alone: 1.5 times the error, in 98% of the time of forward and backward).
 //
-// What bounds them (MI355X). Head dimension 128: the products, with matrix cores busy 46 to 54% of the cycles and the vector units most of
-// the others; forward over 16384 positions, window 4096, 32 heads: 965 us, 1.0 PFLOP/s (a large library product: 1.43). Head
-// dimension 64: the vector instructions of the softmax, about 4 cycles of them to 2 of products: 8 x 2048 positions, window 512, 16
-// heads: 75 us forward, 87 dQ, 113 dK and dV.
+// What bounds them (MI355X). Head dimension 128: the matrix cores, busy 46 to 57% of the cycles, at the 1.9 to 2.1 GHz that the power limit
+// leaves: one kernel's time shrinks when another of the step waits more. Forward over 16384 positions, window 4096, 32 heads: 930 us,
+// 1.04 PFLOP/s (a large library product: 1.43). Head dimension 64: the vector instructions of the softmax, 42 to 69% of the cycles
+// beside 32 to 38% of products: 8 x 2048 positions, window 512, 16 heads: 73 us forward, 83 dQ, 114 dK and dV.
 // No atomics, and what blocks leave to be added up is added in a fixed order: results do not depend on scheduling.
 #include "flash_tile.hip.h"
 #include <algorithm>
@@ -266,7 +266,7 @@ constexpr float WA_FLOOR = -5e29f;   // a running maximum before the first visib
 
 // Key tiles of 64, or of 32 for head_dim 128: with the scores of 32 keys a wavefront needs at most 168 registers there, and three of them
 // share a SIMD (32 KB of LDS a block). What bounds the kernel is how much of the softmax runs under other wavefronts' products:
-// prompt of 16384 positions, window 4096, 32 heads of 128: 1088 us with two wavefronts and tiles of 64, 965 with three. (For
+// prompt of 16384 positions, window 4096, 32 heads of 128: 1088 us with two wavefronts and tiles of 64, 1023 with three, 930 as it is. (For
 // head_dim 64 tiles of 32 keys take as long as tiles of 64.)
 template <int D> constexpr int fwd_tile() { return D == 64 ? 64 : 32; }
 
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) 
 
 // ------------------------------------------------------------------------------------ backward: dQ, and D = rowsum(dO O)
 // Queries in registers, tiles of 64 keys and values as in the forward. Head dimension 64: four wavefronts on a SIMD (128 registers, none
-// spilt), 128: two. 2 x 8192 positions, window 1024, 32 heads of 128: 450 us, 0.9 PFLOP/s of its three products.
+// spilt), 128: two. 2 x 8192 positions, window 1024, 32 heads of 128: 440 us, 0.9 PFLOP/s of its three products.
 template <typename T, int D>
 __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_kernel(WaArgs a) {
   extern __shared__ __align__(256) uint8_t lds_raw[];
@@ -529,7 +529,7 @@ __device__ __forceinline__ void store_part(const acc16_t (&acc)[D / 32], float m
 // Query tiles of 64, or of 32 for head_dim 128: two wavefronts of that size on a SIMD leave 256 registers each, which the
 // accumulators of 32 keys half fill, so the keys of a block are read from LDS (32 KB, which the smaller tiles make room for)
 // and only the values stay in registers. With both in registers there was one wavefront on a SIMD, and nothing ran
-// under the waits of the other: 1.5 times the time. 2 x 8192 positions, window 1024, 32 heads of 128: 550 us, 1.0 PFLOP/s of its products.
+// under the waits of the other: 1.5 times the time. 2 x 8192 positions, window 1024, 32 heads of 128: 565 us, 1.0 PFLOP/s of its products.
 template <int D> constexpr int dkv_tile() { return D == 64 ? 64 : 32; }
 template <int D> constexpr int dkv_buf() { return 2 * dkv_tile<D>() * D * 2 + 2 * dkv_tile<D>() * 4; }   // Q, dO, lse2, -D
 template <int D> constexpr int dkv_keys() { return D == 64 ? 0 : WA_ROWS * D * 2; }

@@ -62,10 +62,10 @@ def rest_of(q):
     return torch.full((b * h * ((t + 31) // 32) * 32 * d,), 0x7f, dtype=torch.uint8)          # NaN where nothing is written
 
 
-def window(lib, q, k, v, dout, lengths, w, sinks, scale, dtype):
+def window(lib, q, k, v, dout, lengths, w, sinks, scale, dtype, keep_rest=True):
     t, b, h, d = q.shape
     sizes = (t, b, h, k.shape[2], d, w, sinks)
-    out, rest, lse = torch.full_like(q, float("nan")), rest_of(q), torch.full((b, h, t), float("nan"))
+    out, rest, lse = torch.full_like(q, float("nan")), rest_of(q) if keep_rest else None, torch.full((b, h, t), float("nan"))
     call(lib, "window_attn_fwd", q, k, v, out, rest, lse, lengths, strides(q, k, v, out), *sizes, scale, _lib.dtype_code(dtype))
     grads = [torch.full_like(x, float("nan")) for x in (q, k, v)]
     ws = bytes256(call(lib, "window_attn_bwd_workspace_bytes", *sizes))
@@ -104,6 +104,18 @@ def test_window_attention_whatever_the_wavefronts_order(lib, order, monkeypatch)
     q, k, v, dout = wa.inputs(200, 1, 2, 1, 64, BF16, "cpu", 8)
     want, mag = wa.reference(q, k, v, dout, None, 20, 3, -0.2)
     wa.check(window(lib, q, k, v, dout, None, 20, 3, -0.2, BF16), want, mag, BF16)
+
+
+def test_window_attention_without_the_rest(lib):
+    """The rest of the output left out: the same output, gradients with D of the rounded one (within the same bounds)."""
+    q, k, v, dout = wa.inputs(150, 1, 2, 1, 64, BF16, "cpu", 4)
+    want, mag = wa.reference(q, k, v, dout, None, 40, 3, 0.125)
+    got = window(lib, q, k, v, dout, None, 40, 3, 0.125, BF16, keep_rest=False)
+    wa.check(got, want, mag, BF16)
+    whole = window(lib, q, k, v, dout, None, 40, 3, 0.125, BF16)
+    assert torch.equal(got[0], whole[0]) and torch.equal(got[3], whole[3]) and not torch.equal(got[1], whole[1])
+    error = lambda x: (x[1].double() - want[1]).norm()                                          # noqa: E731
+    assert error(whole) < error(got)
 
 
 def test_window_attention_of_slots(lib):
