@@ -378,6 +378,16 @@ __global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) 
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (half == 0 && qrow < a.len)
     a.lse[static_cast<int64_t>(bh) * a.len + qrow] = sum > 0.f ? (m + log2f(sum)) * (1.0f / FA_LOG2E) : sum == 0.f ? -INFINITY : sum;
+  // O is rounded twice, for the result and for what that takes: both from one product in 32 bits. (Left to itself the compiler rounds the
+  // second from the unrounded product, and the rest of a mean that lies between two numbers is then that of the wrong one.)
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float whole = o[i][r] * inv;
+      asm volatile("" : "+v"(whole));
+      o[i][r] = whole;
+    }
   if (a.rest != nullptr && qw < a.len) {
     uint8_t* to = rest_at<D>(a, bh, qw, lane & 31) + 4 * half;
 #pragma unroll
@@ -385,13 +395,13 @@ __global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) 
       float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float whole = o[m / 4][4 * (m % 4) + e] * inv;
+        const float whole = o[m / 4][4 * (m % 4) + e];
         x[e] = whole - elem<T>::to_float(elem<T>::from_float(whole));
       }
       *reinterpret_cast<uint32_t*>(to + 256 * m) = rest_word<T>(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
     }
   }
-  store_rows_out<T, D>(o, inv, lds_raw + wave * (32 * D * 2), out_head<T>(a.o, b, h), a.o.st, qw, a.len, lane);
+  store_rows_out<T, D>(o, 1.f, lds_raw + wave * (32 * D * 2), out_head<T>(a.o, b, h), a.o.st, qw, a.len, lane);
 }
 
 // ------------------------------------------------------------------------------------ backward: dQ, and D = rowsum(dO O)

@@ -1,0 +1,63 @@
+"""Window attention and the quantised cache over the range of what they are given: D = dO . O of the output before its rounding, told
+apart from D of the rounded one.
+
+D. Keys that are all alike make every visible probability 1 / n, and sum_j dS_ij = sum_j P_ij (dP_ij - D_i) = 0: the true dQ is
+zero, and what the kernels leave is scale * key * (minus D's error + the sum of dS's roundings). Values of one large vector m plus small ones:
+the error of D of the rounded output is e_i = sum_d dO_id (round(O_id) - O_id), known exactly, about m u / 2 per element; dS's are
+those of the small part only, times 1 / sqrt(n). With |m| = 10 and a small part of 0.5 they are 4% of e (dQ) and 5% (dK, plus its own rounding,
+u of a value as small as they). The rest of the output is held in 8 bits, to a sixteenth of itself at worst: 3.6% in the mean square of
+a uniform error (2^-4 / sqrt(3)). Together below 10%; a quarter of what D of the rounded output would leave, in the 2-norm, is asked for.
+"""
+import pytest
+import torch
+
+import test_zzn_window_attention_gpu as wa
+from nmtgminor_amd.modules.window_attention import window_attn_func
+
+pytestmark = pytest.mark.gpu
+BOTH = pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+
+def alike(t, b, h, hk, d, factor, dtype, seed=21):
+    """Keys all alike, values of one large vector and small ones. -> q, k, v, dout on the CPU"""
+    gen = torch.Generator().manual_seed(seed)
+    rand = lambda *s: torch.randn(*s, generator=gen)                                        # noqa: E731
+    key = (4 * torch.sign(rand(d))).expand(t, b, hk, d)
+    v = (10 * (1 + 0.3 * rand(b, hk, d)).clamp(0.5, 1.5) * torch.sign(rand(b, hk, d)) + 0.5 * rand(t, b, hk, d)) * factor
+    return [x.to(dtype).contiguous() for x in (rand(t, b, h, d), key, v, rand(t, b, h, d))]
+
+
+def errors_of_rounded_d(q, k, v, dout, lengths, window, sinks, scale):
+    """What D of the rounded output adds to dQ and dK, in 64 bits"""
+    dtype = q.dtype
+    (out, *_), _ = wa.reference(q, k, v, dout, lengths, window, sinks, scale)
+    t, b, h, _ = q.shape
+    group = h // k.shape[2]
+    e = (dout.double() * (out.to(dtype).double() - out)).sum(-1)                            # [t, b, h]
+    dq, dk = torch.zeros_like(out), torch.zeros(k.shape, dtype=torch.float64)
+    for s in range(b):
+        sees = wa.visible(t if lengths is None else int(lengths[s]), t, window, sinks).double()
+        p = sees / sees.sum(1, keepdim=True).clamp_min(1.0)
+        for x in range(h):
+            ds = -p * e[:, s, x][:, None]
+            dq[:, s, x] = ds @ k[:, s, x // group].double() * scale
+            dk[:, s, x // group] += ds.t() @ q[:, s, x].double() * scale
+    return dq, dk
+
+
+def check_d(grads, q, k, v, dout, lengths, window, sinks, scale):
+    want, _ = wa.reference(q, k, v, dout, lengths, window, sinks, scale)
+    for name, got, true, lost in zip(("dq", "dk"), grads, want[1:3], errors_of_rounded_d(q, k, v, dout, lengths, window, sinks, scale)):
+        left = (got.detach().cpu().double() - true).norm() / lost.norm()
+        assert left <= 0.25, f"{name}: {left:.3f} of the error that the rounded output's D leaves"
+
+
+@BOTH
+@pytest.mark.parametrize("factor", [0.1])
+@pytest.mark.parametrize("t,b,h,hk,d,window,sinks,ragged", [(200, 1, 2, 1, 64, 48, 0, False), (300, 2, 2, 2, 128, 90, 3, True)])
+def test_d_is_that_of_the_output_before_its_rounding(dev, t, b, h, hk, d, window, sinks, ragged, factor, dtype):
+    data = alike(t, b, h, hk, d, factor, dtype)
+    lengths = torch.tensor([t, t - 61][:b], dtype=torch.int32) if ragged else None
+    leaves = [x.to(dev).requires_grad_() for x in data[:3]]
+    out = window_attn_func(*leaves, window, sinks, lengths=None if lengths is None else lengths.to(dev))
+    grads = torch.autograd.grad(out, leaves[:2], data[3].to(dev))
+    check_d(grads, *data, lengths, window, sinks, d ** -0.5)
