@@ -732,9 +732,10 @@ int nmtg_multi_tensor_l2norm_scale(int n_tensors, const void* const* in, void* c
  * 8; head_dim contiguous), in the order of the tensor arguments: q, k, v, out for the forward and
  * dout, q, k, v, out, dq, dk, dv for the backward. head_dim 64 or 128, fp16 or bf16, products and
  * sums in fp32, probabilities and score gradients rounded to the 16-bit type for their products.
- * out_rest: what rounding took from out, in 8 bits and an order of its own: batch * heads *
- * ceil(len / 32) * 32 * head_dim bytes, 16-byte aligned, written by the forward where it is not null
- * and read by the backward; without it (null) the backward takes dout . out from the rounded out.
+ * out_rest: what rounding took from out, in 8 bits, units of a power of two per row (finite for every
+ * finite out) and an order of its own: batch * heads * ceil(len / 32) * 32 * head_dim bytes, 16-byte
+ * aligned, written by the forward where it is not null and read by the backward, with out, as the
+ * forward left both; without it (null) the backward takes dout . out from the rounded out.
  * softmax_lse: fp32 [batch, heads, len], natural logarithm (-inf where nothing is visible), written
  * by the forward and read by the backward. workspace: nmtg_window_attn_bwd_workspace_bytes bytes,
  * 256-byte aligned. Positions behind a length are never read. An inf or NaN in a row of k or v may

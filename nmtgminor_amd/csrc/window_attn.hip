@@ -93,30 +93,54 @@ __device__ __forceinline__ int seq_len(const WaArgs& a, int b) {
 }
 
 // ---- what rounding took from O ----
-// In 8 bits (E4M3, a sixteenth of it at most is lost again) times a power of two that leaves room for |O| up to 7: 32 rows of a head by
-// column chunks of 8, [batch, heads, ceil(len / 32)][head_dim / 8][32][8] bytes, which the accumulators' lanes write and the queries'
-// lanes read in whole lines without going through LDS.
+// In 8 bits (E4M3, a sixteenth of it at most is lost again) and units of a power of two per row: 2^-8 (bf16, 2^-11 fp16: half a unit in
+// the last place) of the power of two in the row's largest |O| is 256 units, the most that any of its elements lost, so that the conversion,
+// which overflows to NaN above 464, cannot. The unit is taken from the rounded O, which the backward reads anyway. Elements below 2^-15 of the
+// row's largest lose their rest, of which D would not see anything. A row that is not finite has a D that is not, with a rest or without.
+// 32 rows of a head by column chunks of 8, [batch, heads, ceil(len / 32)][head_dim / 8][32][8] bytes, which the accumulators' lanes write
+// and the queries' lanes read in whole lines without going through LDS.
 template <int D>
 __device__ __forceinline__ uint8_t* rest_at(const WaArgs& a, int bh, int row0, int row) {
   return a.rest + ((static_cast<int64_t>(bh) * ((a.len + 31) / 32) + row0 / 32) * (D / 8) * 32 + row) * 8;
 }
-template <typename T> constexpr float rest_scale() { return elem<T>::dtype == NMTG_BF16 ? 0x1p-14f : 0x1p-17f; }
+// the unit of a row whose largest magnitude, rounded, is `largest`. Below fp16's normal range the last place stays where it is, and below
+// 2^-110 the unit of bf16 would leave that of 32 bits: the exponents stop there.
 template <typename T>
-__device__ __forceinline__ uint32_t rest_word(uint32_t lo, uint32_t hi) {
+__device__ __forceinline__ float rest_unit(uint32_t largest) {
+  constexpr uint32_t UNITS = elem<T>::dtype == NMTG_BF16 ? 16 : 19, LOWEST = elem<T>::dtype == NMTG_BF16 ? 17 : 127 - 14;
+  T x;
+  x.bits = static_cast<uint16_t>(largest);
+  return __uint_as_float((max(__float_as_uint(elem<T>::to_float(x)) >> 23, LOWEST) - UNITS) << 23);
+}
+__device__ __forceinline__ uint32_t rest_word(const float (&x)[4], float unit) {
   s16x2_t w = {0, 0};
-  if constexpr (elem<T>::dtype == NMTG_BF16) {
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2_t, lo), rest_scale<T>(), false);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2_t, hi), rest_scale<T>(), true);
-  } else {
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2_t, lo), rest_scale<T>(), false);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2_t, hi), rest_scale<T>(), true);
-  }
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x[0], x[1], unit, false);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x[2], x[3], unit, true);
   return __builtin_bit_cast(uint32_t, w);
 }
 template <typename T, bool HIGH>
-__device__ __forceinline__ uint32_t rest_pair(uint32_t word) {
-  if constexpr (elem<T>::dtype == NMTG_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, rest_scale<T>(), HIGH));
-  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, rest_scale<T>(), HIGH));
+__device__ __forceinline__ uint32_t rest_pair(uint32_t word, float unit) {
+  if constexpr (elem<T>::dtype == NMTG_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, unit, HIGH));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, unit, HIGH));
+}
+// rest . dO of a lane's half row, o the rounded O. fp16 holds the units' numbers, not the units: they come in at the end.
+template <typename T, int N>
+__device__ __forceinline__ float rest_dot(const uint4 (&o)[N], const uint2 (&rest)[N], const uint4 (&g)[N]) {
+  typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+  u16x2_t most = {0, 0};                                        // magnitudes of 16-bit floats compare as integers
+  const auto look = [&](uint32_t w) __attribute__((always_inline)) { most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, w & 0x7fff7fffu)); };
+#pragma unroll
+  for (int s = 0; s < N; ++s) { look(o[s].x); look(o[s].y); look(o[s].z); look(o[s].w); }
+  uint32_t mine = max(most[0], most[1]), other = mine;
+  swap_halves(mine, other);
+  const float unit = rest_unit<T>(max(mine, other)), held = elem<T>::dtype == NMTG_BF16 ? unit : 1.f;
+  float sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < N; ++s) {
+    sum = dot2<T>(rest_pair<T, false>(rest[s].x, held), g[s].x, dot2<T>(rest_pair<T, true>(rest[s].x, held), g[s].y, sum));
+    sum = dot2<T>(rest_pair<T, false>(rest[s].y, held), g[s].z, dot2<T>(rest_pair<T, true>(rest[s].y, held), g[s].w, sum));
+  }
+  return elem<T>::dtype == NMTG_BF16 ? sum : sum * unit;
 }
 
 // ---- the LDS image ----
@@ -390,6 +414,12 @@ __global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) 
     }
   if (a.rest != nullptr && qw < a.len) {
     uint8_t* to = rest_at<D>(a, bh, qw, lane & 31) + 4 * half;
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(o[i][r]));
+    const float unit = rest_unit<T>(elem<T>::from_float(pair_max(top)).bits);
 #pragma unroll
     for (int m = 0; m < D / 8; ++m) {
       float x[4];
@@ -398,7 +428,7 @@ __global__ __launch_bounds__(64 * WA_WAVES, 3) void window_fwd_kernel(WaArgs a) 
         const float whole = o[m / 4][4 * (m % 4) + e];
         x[e] = whole - elem<T>::to_float(elem<T>::from_float(whole));
       }
-      *reinterpret_cast<uint32_t*>(to + 256 * m) = rest_word<T>(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+      *reinterpret_cast<uint32_t*>(to + 256 * m) = rest_word(x, unit);
     }
   }
   store_rows_out<T, D>(o, 1.f, lds_raw + wave * (32 * D * 2), out_head<T>(a.o, b, h), a.o.st, qw, a.len, lane);
@@ -438,10 +468,9 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_
     uint4 of[D / 16];
     uint2 rf[D / 16];
     load_resident<T, D>(of, at_head<T>(a.o, b, h), a.o.st, qrow, n, lane);
-    const bool more = a.rest != nullptr && qrow < n;
-    if (more) {
+    if (a.rest != nullptr) {
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) rf[s] = *reinterpret_cast<const uint2*>(rest_at<D>(a, bh, qw, lane & 31) + 256 * (2 * s + half));
+      for (int s = 0; s < D / 16; ++s) rf[s] = qrow < n ? *reinterpret_cast<const uint2*>(rest_at<D>(a, bh, qw, lane & 31) + 256 * (2 * s + half)) : make_uint2(0, 0);
     }
     if (qrow < n) {
       const float v = a.lse[static_cast<int64_t>(bh) * a.len + qrow];
@@ -452,13 +481,7 @@ __global__ __launch_bounds__(64 * WA_WAVES, D == 64 ? 4 : 2) void window_bwd_dq_
       delta = dot2<T>(of[s].x, gf[s].x, dot2<T>(of[s].y, gf[s].y, delta));
       delta = dot2<T>(of[s].z, gf[s].z, dot2<T>(of[s].w, gf[s].w, delta));
     }
-    if (more) {
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        delta = dot2<T>(rest_pair<T, false>(rf[s].x), gf[s].x, dot2<T>(rest_pair<T, true>(rf[s].x), gf[s].y, delta));
-        delta = dot2<T>(rest_pair<T, false>(rf[s].y), gf[s].z, dot2<T>(rest_pair<T, true>(rf[s].y), gf[s].w, delta));
-      }
-    }
+    if (a.rest != nullptr) delta += rest_dot<T>(of, rf, gf);
     delta = pair_sum(delta);
     // for the kernel of dK and dV: whole blocks of rows, so that it reads tiles without looking at lengths
     float* to = a.stats + static_cast<int64_t>(bh) * 2 * a.stat_rows + qrow;

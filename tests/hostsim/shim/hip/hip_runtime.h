@@ -227,6 +227,10 @@ static inline uint32_t __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(uint32_t old, h
 static inline uint32_t __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(uint32_t old, hostsim_half2 x, float s, int sel) { return hostsim::to_fp4(old, x, s, sel); }
 static inline hostsim_short2 __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hostsim_short2 old, hostsim_bf16x2 x, float s, bool hi) { return hostsim::to_fp8(old, x, s, hi); }
 static inline hostsim_short2 __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(hostsim_short2 old, hostsim_half2 x, float s, bool hi) { return hostsim::to_fp8(old, x, s, hi); }
+static inline hostsim_short2 __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hostsim_short2 old, float a, float b, float s, bool hi) {
+  const float x[2] = {a, b};
+  return hostsim::to_fp8(old, x, s, hi);
+}
 static inline hostsim_bf16x2 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(uint32_t w, float s, int sel) { return hostsim::from_fp4<hostsim_bf16x2, __bf16>(w, s, sel); }
 static inline hostsim_half2 __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(uint32_t w, float s, int sel) { return hostsim::from_fp4<hostsim_half2, _Float16>(w, s, sel); }
 static inline hostsim_bf16x2 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(uint32_t w, float s, bool hi) { return hostsim::from_fp8<hostsim_bf16x2, __bf16>(w, s, hi); }

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import test_hostsim_long_context_cpu as sim
+import test_zzn_window_attention_gpu as wa
 import test_zzp_long_context_range_gpu as rng
 from test_hostsim_long_context_cpu import lib  # noqa: F401
 
@@ -11,7 +12,16 @@ BOTH = sim.BOTH
 
 
 @BOTH
-@pytest.mark.parametrize("factor", [0.1])
+@pytest.mark.parametrize("factor", [1e-3, 8.0, 64.0, 1000.0])
+@pytest.mark.parametrize("t,b,h,hk,d,window,sinks,ragged", rng.MAGNITUDES)
+def test_values_of_other_magnitudes(lib, t, b, h, hk, d, window, sinks, ragged, factor, dtype):  # noqa: F811
+    q, k, v, dout, lengths = rng.scaled_inputs(t, b, h, hk, d, ragged, factor, dtype, "cpu")
+    want, mag = wa.reference(*(torch.nan_to_num(x) for x in (q, k, v, dout)), lengths, window, sinks, d ** -0.5)
+    wa.check(sim.window(lib, q, k, v, dout, lengths, window, sinks, d ** -0.5, dtype), want, mag, dtype)
+
+
+@BOTH
+@pytest.mark.parametrize("factor", [1e-3, 1.0, 64.0, 1000.0])
 @pytest.mark.parametrize("t,b,h,hk,d,window,sinks,ragged", [(100, 1, 2, 1, 64, 48, 0, False), (140, 2, 1, 1, 128, 90, 3, True)])
 def test_d_is_that_of_the_output_before_its_rounding(lib, t, b, h, hk, d, window, sinks, ragged, factor, dtype):  # noqa: F811
     data = rng.alike(t, b, h, hk, d, factor, dtype)
@@ -20,3 +30,12 @@ def test_d_is_that_of_the_output_before_its_rounding(lib, t, b, h, hk, d, window
     rng.check_d(got[1:3], *data, lengths, window, sinks, d ** -0.5)
     with pytest.raises(AssertionError, match="dq"):            # the check tells the two apart
         rng.check_d(sim.window(lib, *data, lengths, window, sinks, d ** -0.5, dtype, keep_rest=False)[1:3], *data, lengths, window, sinks, d ** -0.5)
+
+
+def test_smallest_and_largest_outputs(lib):  # noqa: F811
+    """Outputs below the normal range of the type, in which every rounding is as large as any, and the largest of bf16."""
+    for dtype, factor in ((torch.float16, 2.0 ** -22), (torch.bfloat16, 2.0 ** -125), (torch.bfloat16, 2.0 ** 120)):
+        q, k, v, dout, _ = rng.scaled_inputs(70, 1, 1, 1, 64, False, factor, dtype, "cpu")
+        dout = dout * 2.0 ** -20 if factor > 1 else dout
+        got = sim.window(lib, q, k, v, dout, None, 20, 2, 0.125, dtype)
+        assert all(torch.isfinite(x).all() for x in got)

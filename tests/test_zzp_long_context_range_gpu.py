@@ -1,5 +1,7 @@
-"""Window attention and the quantised cache over the range of what they are given: D = dO . O of the output before its rounding, told
-apart from D of the rounded one.
+"""Window attention and the quantised cache over the range of what they are given: magnitudes far from one, and D = dO . O of the
+output before its rounding, told apart from D of the rounded one.
+
+Magnitudes: the bounds of test_zzn_window_attention_gpu, which scale with the terms they are sums of.
 
 D. Keys that are all alike make every visible probability 1 / n, and sum_j dS_ij = sum_j P_ij (dP_ij - D_i) = 0: the true dQ is
 zero, and what the kernels leave is scale * key * (minus D's error + the sum of dS's roundings). Values of one large vector m plus small ones:
@@ -12,10 +14,30 @@ import pytest
 import torch
 
 import test_zzn_window_attention_gpu as wa
+from nmtgminor_amd import _lib as L
 from nmtgminor_amd.modules.window_attention import window_attn_func
 
 pytestmark = pytest.mark.gpu
 BOTH = pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+
+MAGNITUDES = [
+    # t, b, h, hk, d, window, sinks, ragged
+    (150, 1, 2, 1, 64, 40, 3, False),
+    (200, 2, 2, 2, 128, 33, 70, True),
+]
+
+
+def scaled_inputs(t, b, h, hk, d, ragged, factor, dtype, dev):
+    """-> q, k, v * factor, dout, lengths; not a number behind the lengths"""
+    q, k, v, dout = wa.inputs(t, b, h, hk, d, torch.float32, "cpu", 11)
+    q, k, v, dout = (x.to(dtype).to(dev) for x in (q, k, v * factor, dout))
+    lengths = torch.tensor([(t, t // 2)[i % 2] for i in range(b)], dtype=torch.int32, device=dev) if ragged else None
+    if ragged:
+        for x in (q, k, v, dout):
+            for s in range(b):
+                x[int(lengths[s]):, s] = float("nan")
+    return q, k, v, dout, lengths
+
 
 def alike(t, b, h, hk, d, factor, dtype, seed=21):
     """Keys all alike, values of one large vector and small ones. -> q, k, v, dout on the CPU"""
@@ -52,7 +74,25 @@ def check_d(grads, q, k, v, dout, lengths, window, sinks, scale):
 
 
 @BOTH
-@pytest.mark.parametrize("factor", [0.1])
+@pytest.mark.parametrize("factor", [1e-3, 8.0, 64.0, 1000.0])
+@pytest.mark.parametrize("t,b,h,hk,d,window,sinks,ragged", MAGNITUDES)
+def test_values_of_other_magnitudes(dev, t, b, h, hk, d, window, sinks, ragged, factor, dtype):
+    q, k, v, dout, lengths = scaled_inputs(t, b, h, hk, d, ragged, factor, dtype, dev)
+    clean = [torch.nan_to_num(x) for x in (q, k, v, dout)]
+    want, mag = wa.reference(*clean, lengths, window, sinks, d ** -0.5)
+    for x in (q, k, v):
+        x.requires_grad_()
+    out = window_attn_func(q, k, v, window, sinks, lengths=lengths)
+    wa.check((out, *torch.autograd.grad(out, (q, k, v), dout)), want, mag, dtype)
+    # the same as slots of one projection
+    lin = torch.cat((q, k, v), 2).detach().flatten(2).requires_grad_()
+    out = L.host().window_attention_projection(lin, h, hk, window, sinks, None, lengths)
+    dlin, = torch.autograd.grad(out, lin, dout)
+    wa.check((out, *dlin.view(t, b, -1, d).split((h, hk, hk), 2)), want, mag, dtype)
+
+
+@BOTH
+@pytest.mark.parametrize("factor", [1e-3, 1.0, 64.0, 1000.0])
 @pytest.mark.parametrize("t,b,h,hk,d,window,sinks,ragged", [(200, 1, 2, 1, 64, 48, 0, False), (300, 2, 2, 2, 128, 90, 3, True)])
 def test_d_is_that_of_the_output_before_its_rounding(dev, t, b, h, hk, d, window, sinks, ragged, factor, dtype):
     data = alike(t, b, h, hk, d, factor, dtype)
@@ -61,3 +101,22 @@ def test_d_is_that_of_the_output_before_its_rounding(dev, t, b, h, hk, d, window
     out = window_attn_func(*leaves, window, sinks, lengths=None if lengths is None else lengths.to(dev))
     grads = torch.autograd.grad(out, leaves[:2], data[3].to(dev))
     check_d(grads, *data, lengths, window, sinks, d ** -0.5)
+
+
+@BOTH
+def test_rows_of_no_magnitude_and_of_none_that_is_finite(dev, dtype):
+    """An output of zeros has gradients like any other; one that is not finite spoils its own query's gradients, and no other head's."""
+    q, k, v, dout = wa.inputs(100, 1, 2, 2, 64, dtype, dev, 6)
+    for x in (q, k, v):
+        x.requires_grad_()
+    zero = torch.zeros_like(v).requires_grad_()
+    out = window_attn_func(q, k, zero, 30, 2)
+    assert not out.any()
+    grads = torch.autograd.grad(out, (q, k, zero), dout)
+    assert not grads[0].any() and not grads[1].any() and torch.isfinite(grads[2]).all()
+    poisoned = v.detach().clone()
+    poisoned[50, 0, 1, 3] = float("inf")
+    bad = torch.autograd.grad(window_attn_func(q, k, poisoned.requires_grad_(), 30, 2), (q, k, poisoned), dout)
+    good = torch.autograd.grad(window_attn_func(q, k, v, 30, 2), (q, k, v), dout)
+    assert all(torch.equal(x[:, :, 0], y[:, :, 0]) for x, y in zip(bad, good))
+    assert not torch.isfinite(bad[0][50, 0, 1]).all()
