@@ -59,6 +59,20 @@ __device__ __forceinline__ void held_word(uint32_t word, float scale, uint32_t* 
   }
 }
 
+// A block whose largest magnitude rounds up can be held as a power of two beyond the type's largest number (fp16: from 57344 on in 4 bits, 63488
+// in 8; a cache written in bf16 holds more than fp16 has anyway), which the conversion gives as inf. Scale bytes below the limit cannot.
+template <typename T, int BITS> constexpr uint32_t beyond_byte() {
+  return 127 + (elem<T>::dtype == NMTG_BF16 ? 128 : 16) - (BITS == 4 ? 2 : 8);      // 4 and 256 are the largest powers of two among the elements
+}
+// inf in a pair becomes the type's largest number, the nearest to what is held
+template <typename T>
+__device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
+  constexpr uint32_t INF = elem<T>::dtype == NMTG_BF16 ? 0x7f80u : 0x7c00u;
+  if ((w & 0x7fffu) == INF) w -= 1;
+  if ((w & 0x7fff0000u) == INF << 16) w -= 0x10000u;
+  return w;
+}
+
 // ------------------------------------------------------------------------------------------------------- write and read
 // A block takes a tile of 16-bit rows: 2^tshift neighbouring positions of as many (sequence, head) pairs as 128 (head_dim 64) or
 // 64 rows make. In the 16-bit tensors neighbouring pairs lie side by side, in the cache neighbouring positions do: with 8 or 16
@@ -319,9 +333,10 @@ struct KvTile {
   }
 };
 
-// Wavefronts per block: 4 or 8, see attn_plan().
+// Wavefronts per block: 4 or 8, see attn_plan(). Head dimension 64 in 4 bits keeps to the 128 registers of four wavefronts on a SIMD (32
+// sequences of 16384 to 32768 positions, 8 heads: 103 us, 136 with 129 registers and three).
 template <typename T, int D, int BITS, bool STREAM>
-__global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
+__global__ __launch_bounds__(512, D == 64 && BITS == 4 ? 4 : 2) void kv_attn_kernel(KvAttn a) {
   constexpr int NK = D / 32, NV = D / 16;
   using Tile = KvTile<D, BITS, STREAM>;
   extern __shared__ __align__(16) float lds_attn[];                 // [waves][KV_ROWS][2] maximum and sum, [waves][rows][D + 4]
@@ -365,9 +380,12 @@ __global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
     const int64_t position = position_of(i);
     to.load(kc, ksc, vc, vsc, position, a.capacity - position, lane);
   };
-  const auto visit = [&](int t, Tile& tile, Tile& next) __attribute__((always_inline)) {
+  uint64_t far_keys = 0;                                           // lanes that met a key that may be beyond the type's largest number
+  // exact: held values beyond the type's largest number become that number
+  const auto visit = [&](int t, Tile& tile, Tile& next, auto exact) __attribute__((always_inline)) {
     const int position = position_of(t);
     if (t + waves < t1) fetch(next, t + waves);
+    if constexpr (!exact) far_keys |= __builtin_amdgcn_ballot_w64(max(tile.ks[0], tile.ks[1]) >= beyond_byte<T, BITS>());
     float sc[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -376,6 +394,10 @@ __global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
       uint32_t kw[4 * NK];
 #pragma unroll
       for (int w = 0; w < Tile::KW; ++w) held_word<T, BITS>(tile.k[h][w], scale, kw + w * (BITS == 4 ? 4 : 2));
+      if constexpr (exact) {
+#pragma unroll
+        for (int w = 0; w < 4 * NK; ++w) kw[w] = finite_pair<T>(kw[w]);
+      }
 #pragma unroll
       for (int x = 0; x < NK; ++x) s = mfma_16x16x32<T>(make_uint4(kw[4 * x], kw[4 * x + 1], kw[4 * x + 2], kw[4 * x + 3]), qf[x], s);
 #pragma unroll
@@ -447,15 +469,38 @@ __global__ __launch_bounds__(512, 2) void kv_attn_kernel(KvAttn a) {
         vw[2 * j + 1][e / 2] = __builtin_amdgcn_perm(y[j], x[j], 0x07060302u);
       }
     }
+    if constexpr (exact) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) vw[j][w] = finite_pair<T>(vw[j][w]);
+    }
 #pragma unroll
     for (int j = 0; j < NV; ++j) o[j] = mfma_16x16x32<T>(make_uint4(vw[j][0], vw[j][1], vw[j][2], vw[j][3]), pf, o[j]);
   };
   // two sets of registers in turn, so that nothing is moved from one to the other
-  Tile even, odd;
-  if (t0 + wave < t1) fetch(even, t0 + wave);
-  for (int t = t0 + wave; t < t1; t += 2 * waves) {
-    visit(t, even, odd);
-    if (t + waves < t1) visit(t + waves, odd, even);
+  const auto pass = [&](auto exact) __attribute__((always_inline)) {
+    Tile even, odd;
+    if (t0 + wave < t1) fetch(even, t0 + wave);
+    for (int t = t0 + wave; t < t1; t += 2 * waves) {
+      visit(t, even, odd, exact);
+      if (t + waves < t1) visit(t + waves, odd, even, exact);
+    }
+  };
+  pass(std::false_type{});
+  // Where a key may have been inf, or a value was (whatever its probability, its product is inf or NaN and stays in the sums), this wavefront's
+  // tiles once more, exactly. (As a branch in every tile the question cost 2 to 7%.)
+  float spoilt = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) spoilt = __builtin_fmaf(o[j][i], 0.f, spoilt);
+  if ((far_keys | __builtin_amdgcn_ballot_w64(spoilt != spoilt)) != 0) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    m = KV_FLOOR;
+    l = 0.f;
+    pass(std::true_type{});
   }
 
   // the wavefronts' results: lane (r, g) holds elements (4 g + i) D / 16 + j of query row r in o[j][i]

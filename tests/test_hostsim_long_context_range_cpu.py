@@ -39,3 +39,20 @@ def test_smallest_and_largest_outputs(lib):  # noqa: F811
         dout = dout * 2.0 ** -20 if factor > 1 else dout
         got = sim.window(lib, q, k, v, dout, None, 20, 2, 0.125, dtype)
         assert all(torch.isfinite(x).all() for x in got)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype,d,lengths", [(torch.float16, 64, [70, 33]), (torch.float16, 128, [70, 2]), (torch.bfloat16, 128, [1, 1])])
+def test_finite_values_are_attended_to_as_finite(lib, dtype, d, lengths, bits):  # noqa: F811
+    cap = max(lengths)
+    k, v, seen, q, scale = rng.top_of_the_type(cap, 2, 2, d, bits, dtype)
+    cache = sim.qc.buffers(2, 2, cap, d, bits, "cpu")
+    sim.write(lib, cache, k, v, None, 0)
+    want, mag = sim.qc.attend_reference(q, *seen, lengths, 0, 0, scale)
+    rng.check_attend(sim.attend(lib, q, cache, torch.tensor(lengths, dtype=torch.int32), cap, 0, 0, scale), want, mag, dtype,
+                     lengths, torch.finfo(dtype).max)
+    # a block that is not finite is still NaN, and no other
+    v[0, 0, 0, 3] = float("inf")
+    sim.write(lib, cache, k, v, None, 0)
+    out = sim.attend(lib, q, cache, torch.tensor(lengths, dtype=torch.int32), cap, 0, 0, scale)
+    assert torch.isnan(out[0, 0, :2, :32]).all() and torch.isfinite(out[0, 0, :2, 32:]).all() and torch.isfinite(out[0, 0, 2:]).all()

@@ -14,6 +14,7 @@ import pytest
 import torch
 
 import test_zzn_window_attention_gpu as wa
+import test_zzo_quantized_cache_gpu as qc
 from nmtgminor_amd import _lib as L
 from nmtgminor_amd.modules.window_attention import window_attn_func
 
@@ -120,3 +121,44 @@ def test_rows_of_no_magnitude_and_of_none_that_is_finite(dev, dtype):
     good = torch.autograd.grad(window_attn_func(q, k, v, 30, 2), (q, k, v), dout)
     assert all(torch.equal(x[:, :, 0], y[:, :, 0]) for x, y in zip(bad, good))
     assert not torch.isfinite(bad[0][50, 0, 1]).all()
+
+
+# ------------------------------------------------------------------------------------------------------ quantised cache
+def check_attend(got, want, mag, dtype, lengths, largest):
+    """Probabilities rounded once (u each, their sum that of the rounded ones) times values exact in the type, rounded once: 2 u of the terms'
+    magnitudes and u of the result, 1e-5 of the magnitudes for sums and exponentials in 32 bits (u: 2^-8 for bf16, 2^-11 for fp16). Probabilities
+    below fp16's normal range, relative to a largest of at least 1, are off by up to 2^-25 each, times at most the largest value."""
+    got = got.cpu().double()
+    assert got.shape == want.shape and torch.isfinite(got).all()
+    small = 2.0 ** -25 * largest * torch.tensor(lengths, dtype=torch.float64)[None, :, None, None] if dtype == torch.float16 else 0.0
+    worst = ((got - want).abs() / ((2 * wa.U[dtype] + 1e-5) * mag + wa.U[dtype] * want.abs() + 1e-6 + small)).max().item()
+    assert worst <= 1.0, f"{worst:.3f} of the bound"
+
+
+def top_of_the_type(cap, b, hk, d, bits, dtype):
+    """Keys and values up to the type's largest. A block whose largest magnitude rounds up is held as a power of two beyond it, which the
+    attention takes as the type's largest. -> k, v, their values as the attention sees them, q, softmax scale"""
+    gen = torch.Generator().manual_seed(31)
+    top = torch.finfo(dtype).max
+    k, v = ((2 * torch.rand(cap, b, hk, d, generator=gen, dtype=torch.float64) - 1) * top for _ in range(2))
+    k[..., 5], v[..., 7] = top, -top
+    k[1::3, ..., :32] *= 2.0 ** -9                                # blocks of ordinary magnitude among them
+    k, v = k.to(dtype), v.to(dtype)
+    seen = [qc.held(x, bits)[0].clamp(-top, top) for x in (k, v)]
+    assert (qc.held(k, bits)[0].abs() > top).any() and (qc.held(v, bits)[0].abs() > top).any()
+    # scores of some units: sums of head_dim products of q and numbers up to the largest
+    q = (torch.randn(1, b, 2 * hk, d, generator=gen) * (2.0 ** -4 if dtype == torch.float16 else 2.0 ** -120)).to(dtype)
+    return k, v, seen, q, 2.0 ** -12 if dtype == torch.float16 else 2.0 ** -8
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype,d,lengths", [(torch.float16, 64, [70, 33]), (torch.float16, 128, [70, 2]), (torch.float16, 64, [2500, 40]),
+                                             (torch.bfloat16, 128, [1, 1])])          # (bf16: sums of two such values leave 32 bits)
+def test_finite_values_are_attended_to_as_finite(dev, dtype, d, lengths, bits):
+    cap = max(lengths)
+    k, v, seen, q, scale = top_of_the_type(cap, 2, 2, d, bits, dtype)
+    cache = qc.buffers(2, 2, cap, d, bits, dev)
+    qc.kv_cache_write(*cache, k.to(dev), v.to(dev), 0)
+    want, mag = qc.attend_reference(q, *seen, lengths, 0, 0, scale)
+    got = qc.kv_cache_attend(q.to(dev), *cache, torch.tensor(lengths, dtype=torch.int32, device=dev), cap, 0, 0, scale)
+    check_attend(got, want, mag, dtype, lengths, torch.finfo(dtype).max)
