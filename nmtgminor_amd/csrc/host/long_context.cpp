@@ -1,6 +1,7 @@
 // The operators of long-context decoders: attention with a sliding window and sinks as an autograd node, on three tensors or on the
 // heads of one projection, and the rows of the quantised key / value cache written, read back and attended to.
 #include "host.h"
+#include <limits>
 
 namespace nmtg_host {
 
@@ -25,6 +26,11 @@ Tensor view_of(const Tensor& x) {
 }
 void put_strides(int64_t* to, const Tensor& x) {
   for (int i = 0; i < 3; ++i) to[i] = x.stride(i);
+}
+// positions as the kernels take them; what 32 bits do not hold stays outside of every sequence and cache
+Tensor narrow32(const Tensor& t) {
+  const auto limits = std::numeric_limits<int32_t>();
+  return contiguous(t.scalar_type() == at::kLong ? t.clamp(limits.min(), limits.max()).to(at::kInt) : t);
 }
 const int32_t* lengths_of(const Tensor& t) { return t.defined() ? t.data_ptr<int32_t>() : nullptr; }
 
@@ -116,7 +122,7 @@ Window window_args(const Tensor& q, int64_t batch, int64_t head_dim, int64_t win
     check_device(*lengths, q);
     TORCH_CHECK(lengths->dim() == 1 && lengths->size(0) == batch, "window attention: lengths must be [batch]");
     TORCH_CHECK(lengths->scalar_type() == at::kInt || lengths->scalar_type() == at::kLong, "window attention: lengths must be integers");
-    w.lengths = contiguous(lengths->to(at::kInt));
+    w.lengths = narrow32(*lengths);
   }
   return w;
 }
@@ -149,7 +155,7 @@ Tensor int32_of(const Tensor& t, const Tensor& operand, int64_t batch, const cha
   check_device(t, operand);
   TORCH_CHECK(t.dim() == 1 && t.size(0) == batch && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong), "kv cache: ", what,
               " must be integers [batch]");
-  return contiguous(t.to(at::kInt));
+  return narrow32(t);
 }
 void no_gradient(const Tensor& t, const char* what) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what, " has no gradient: call it under torch.no_grad() or on detached tensors");

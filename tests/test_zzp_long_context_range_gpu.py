@@ -162,3 +162,25 @@ def test_finite_values_are_attended_to_as_finite(dev, dtype, d, lengths, bits):
     want, mag = qc.attend_reference(q, *seen, lengths, 0, 0, scale)
     got = qc.kv_cache_attend(q.to(dev), *cache, torch.tensor(lengths, dtype=torch.int32, device=dev), cap, 0, 0, scale)
     check_attend(got, want, mag, dtype, lengths, torch.finfo(dtype).max)
+
+
+def test_int64_positions_beyond_32_bits(dev):
+    """Starts that lie outside the cache are outside it however far, and a length is clamped, not wrapped."""
+    far = [1 << 32, -(1 << 32), (1 << 32) + 3, -(1 << 31) - 1, 2]
+    b, hk, d, cap = len(far), 1, 64, 8
+    k, v = (torch.randn(2, b, hk, d, device=dev).to(torch.bfloat16) for _ in range(2))
+    cache = qc.buffers(b, hk, cap, d, 8, dev, fill=7)
+    starts = torch.tensor(far, dtype=torch.int64, device=dev)
+    qc.kv_cache_write(*cache, k, v, starts)
+    for x in cache:
+        assert (x[:4] == 7).all() and (x[4, :, :2] == 7).all() and (x[4, :, 4:] == 7).all()
+    got = qc.kv_cache_read(*cache, starts, 2, torch.bfloat16)
+    assert not got[0][:, :4].any() and not got[1][:, :4].any() and got[0][:, 4].any()
+    qc.kv_cache_write(*cache, *(torch.randn(cap, b, hk, d, device=dev).to(torch.bfloat16) for _ in range(2)), 0)
+    q = torch.randn(1, b, 2, d, device=dev).to(torch.bfloat16)
+    lengths = torch.tensor([1 << 32, -(1 << 32), (1 << 32) + 3, -(1 << 31) - 1, 5], dtype=torch.int64, device=dev)
+    want = qc.kv_cache_attend(q, *cache, torch.tensor([cap, 0, cap, 0, 5], dtype=torch.int32, device=dev), cap)
+    assert torch.equal(qc.kv_cache_attend(q, *cache, lengths, cap), want)
+    x, y, z, _ = wa.inputs(20, b, 2, 1, 64, torch.bfloat16, dev)
+    want = window_attn_func(x, y, z, 5, 1, lengths=torch.tensor([20, 0, 20, 0, 5], dtype=torch.int32, device=dev))
+    assert torch.equal(window_attn_func(x, y, z, 5, 1, lengths=lengths), want)
