@@ -67,6 +67,12 @@ _host_module = None
 tracing = torch._C._get_tracing_state
 
 
+def refuse_tracing(what):
+    """For operators that only the host layer has."""
+    if tracing() is not None:
+        raise RuntimeError(f"{what} cannot be traced: torch.jit.trace would keep the result of the recording")
+
+
 def host():
     """The native host layer (csrc/host): operators that take tensors, prepare the call and enqueue the kernels without the
     interpreter in between. Used for tensors on the GPU; missing is an error there, as the library itself missing is."""

@@ -12,7 +12,7 @@ them. Here a block of 32 neighbouring elements of a row keeps one scale byte (a 
 
     QuantizedKVCache                                                        the four buffers with their lengths
 
-Inference only: nothing here has a gradient. Every call enqueues on the current stream and returns.
+Inference only: nothing here has a gradient, and torch.jit.trace is refused. Every call enqueues on the current stream and returns.
 """
 import torch
 
@@ -28,12 +28,14 @@ def kv_cache_write(k_codes, k_scales, v_codes, v_scales, k, v, start):
     """Quantises k and v [count, B, H_kv, D] (fp16 or bf16, any strides with a contiguous D that are multiples of 8) into
     the cache rows start .. start + count of every sequence. With a tensor of starts, rows outside the cache are dropped;
     with an int they are an error."""
+    L.refuse_tracing("kv_cache_write")
     L.host().kv_cache_write(k_codes, k_scales, v_codes, v_scales, k, v, *_start(start))
 
 
 def kv_cache_read(k_codes, k_scales, v_codes, v_scales, start, count, dtype=torch.bfloat16):
     """The values that cache rows start .. start + count stand for, k and v [count, B, H_kv, D]. With a tensor of starts,
     positions outside the cache read as zeros."""
+    L.refuse_tracing("kv_cache_read")
     return L.host().kv_cache_read(k_codes, k_scales, v_codes, v_scales, *_start(start), count, dtype)
 
 
@@ -41,6 +43,7 @@ def kv_cache_attend(q, k_codes, k_scales, v_codes, v_scales, lengths, longest, w
     """q [tq, B, H, D]: the newest tq positions of every sequence, which hold lengths[b] positions (int32 on the device,
     these included), at most `longest`. Position p sees positions up to p; with window > 0 the last `window` of them (itself
     included) and the first `sinks` positions only. H is a multiple of the cache's heads, softmax_scale defaults to D^-0.5."""
+    L.refuse_tracing("kv_cache_attend")
     return L.host().kv_cache_attend(q, k_codes, k_scales, v_codes, v_scales, lengths, longest, window, sinks, softmax_scale)
 
 

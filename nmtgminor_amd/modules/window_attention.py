@@ -7,7 +7,8 @@
 
 Work and memory grow with T * (window + sinks): there is no mask tensor and no [T, T] tensor. H is a multiple of H_kv (query
 heads share key / value heads). lengths (integers [B] on the device): positions behind a sequence's length see nothing, are
-seen by nobody, and have zero outputs and gradients. fp16 / bf16, head dimension 64 or 128, no dropout on the probabilities.
+seen by nobody, and have zero outputs and gradients. fp16 / bf16, head dimension 64 or 128, no dropout on the probabilities,
+torch.jit.trace is refused.
 """
 import math
 
@@ -22,6 +23,7 @@ from .quantized_cache import QuantizedKVCache
 
 
 def window_attn_func(q, k, v, window, sinks=0, softmax_scale=None, lengths=None):
+    L.refuse_tracing("window attention")
     if not torch.is_autocast_enabled():             # (the context manager costs half of a short call)
         return L.host().window_attention(q, k, v, window, sinks, softmax_scale, lengths)
     q, k, v = cast_if_autocast_enabled(q, k, v)
@@ -63,6 +65,7 @@ class WindowSelfMultiheadAttn(nn.Module):
     def forward(self, inputs, lengths=None, cache=None):
         """inputs [T, B, E] -> [T, B, E]. lengths [B]: as in window_attn_func; with a cache, how many of the T positions are a
         sequence's own (prompts of several lengths)."""
+        L.refuse_tracing("window attention")
         t, b, _ = inputs.shape
         lin = linear_function(inputs, self.in_proj_weight, self.in_proj_bias)
         if cache is None or cache.longest == 0:

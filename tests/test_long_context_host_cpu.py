@@ -1,0 +1,17 @@
+"""What window attention and the quantised cache decide before they touch a GPU."""
+import pytest
+import torch
+
+from nmtgminor_amd.modules import quantized_cache as qc
+from nmtgminor_amd.modules.window_attention import WindowSelfMultiheadAttn, window_attn_func
+
+
+def test_tracing_is_refused():
+    q = torch.zeros(3, 1, 2, 64, dtype=torch.bfloat16)
+    cache = qc.QuantizedKVCache(1, 2, 64, 8, device="cpu")
+    m = WindowSelfMultiheadAttn(128, 2, window=4).bfloat16().requires_grad_(False)
+    for call, arg in ((lambda y: window_attn_func(y, q, q, 4), q), (m, torch.zeros(3, 1, 128, dtype=torch.bfloat16)),
+                      (lambda y: cache.append(y, q) or y, q), (lambda y: cache.read()[0], q), (lambda y: cache.attend(y), q)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, (arg,), check_trace=False)
+    assert cache.longest == 0

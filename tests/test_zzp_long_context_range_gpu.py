@@ -184,3 +184,19 @@ def test_int64_positions_beyond_32_bits(dev):
     x, y, z, _ = wa.inputs(20, b, 2, 1, 64, torch.bfloat16, dev)
     want = window_attn_func(x, y, z, 5, 1, lengths=torch.tensor([20, 0, 20, 0, 5], dtype=torch.int32, device=dev))
     assert torch.equal(window_attn_func(x, y, z, 5, 1, lengths=lengths), want)
+
+
+# ----------------------------------------------------------------------------------------------------- what is refused
+def test_tracing_is_refused(dev):
+    """torch.jit.trace does not see the native layer's results and would keep those of the recording."""
+    cache = qc.QuantizedKVCache(1, 2, 64, 8, dtype=torch.float16, device=dev)
+    q, k, v, _ = wa.inputs(3, 1, 2, 2, 64, torch.float16, dev)
+    m = wa.WindowSelfMultiheadAttn(128, 2, window=4).to(dev).half().requires_grad_(False)
+    x = torch.randn(3, 1, 128, device=dev).half()
+    with torch.no_grad():
+        for call, arg in ((lambda y: window_attn_func(y, k, v, 4), q), (m, x), (lambda y: m(y, cache=cache), x),
+                          (lambda y: cache.append(y, v) or y, k), (lambda y: cache.read()[0] + y, q), (lambda y: cache.attend(y), q)):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                torch.jit.trace(call, (arg,), check_trace=False)
+        assert cache.longest == 0 and not cache.k_codes.any()
+        m(x)
