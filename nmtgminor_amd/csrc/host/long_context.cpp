@@ -159,6 +159,7 @@ Tensor int32_of(const Tensor& t, const Tensor& operand, int64_t batch, const cha
 }
 void no_gradient(const Tensor& t, const char* what) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what, " has no gradient: call it under torch.no_grad() or on detached tensors");
+  TORCH_CHECK(!(forward_mode() && has_tangent(t)), what, ": jvp is not implemented");
 }
 
 }  // namespace

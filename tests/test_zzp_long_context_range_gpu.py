@@ -200,3 +200,21 @@ def test_tracing_is_refused(dev):
                 torch.jit.trace(call, (arg,), check_trace=False)
         assert cache.longest == 0 and not cache.k_codes.any()
         m(x)
+
+
+def test_tangents_are_refused(dev):
+    """A forward-mode dual's tangent would be dropped without a word."""
+    from torch.autograd import forward_ad
+    cache = qc.QuantizedKVCache(1, 2, 64, 8, dtype=torch.float16, device=dev)
+    q, k, v, t = wa.inputs(3, 1, 2, 2, 64, torch.float16, dev)
+    lin = torch.cat((q, k, v), 2).flatten(2)
+    with torch.no_grad(), forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, t)
+        for call in (lambda: qc.kv_cache_write(*cache.tensors, dual, v, 0), lambda: qc.kv_cache_write(*cache.tensors, k, dual, 0),
+                     lambda: cache.append(k, dual), lambda: cache.attend(dual), lambda: window_attn_func(q, dual, v, 2),
+                     lambda: L.host().window_attention_projection(forward_ad.make_dual(lin, lin), 2, 2, 2, 0, None, None)):
+            with pytest.raises(RuntimeError, match="(?i)jvp"):
+                call()
+        assert cache.longest == 0 and not cache.k_codes.any()
+        cache.append(k, v)
+        cache.attend(q)
