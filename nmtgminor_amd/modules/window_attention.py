@@ -58,9 +58,15 @@ class WindowSelfMultiheadAttn(nn.Module):
         nn.init.constant_(self.in_proj_bias, 0.)
         nn.init.constant_(self.out_proj_bias, 0.)
 
-    def make_cache(self, batch, capacity):
+    def make_cache(self, batch, capacity, dtype=None):
+        """dtype: of the rows that will be appended and of what read() returns; by default the weights', and for weights in 32 bits
+        autocast's (bf16 outside of it)."""
         w = self.in_proj_weight
-        return QuantizedKVCache(batch, self.num_kv_heads, self.head_dim, capacity, self.cache_bits, w.dtype, w.device)
+        if dtype is None:
+            dtype = w.dtype
+            if dtype == torch.float32:
+                dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled() else torch.bfloat16
+        return QuantizedKVCache(batch, self.num_kv_heads, self.head_dim, capacity, self.cache_bits, dtype, w.device)
 
     def forward(self, inputs, lengths=None, cache=None):
         """inputs [T, B, E] -> [T, B, E]. lengths [B]: as in window_attn_func; with a cache, how many of the T positions are a

@@ -15,3 +15,18 @@ def test_tracing_is_refused():
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(call, (arg,), check_trace=False)
     assert cache.longest == 0
+
+
+def test_a_module_in_32_bits_has_a_cache():
+    """Of the type that its rows will have: autocast's, or bf16 outside of it; another by name."""
+    m = WindowSelfMultiheadAttn(128, 2, window=4, num_kv_heads=1)
+    assert m.make_cache(3, 8).dtype == torch.bfloat16
+    for dtype in (torch.float16, torch.bfloat16):
+        with torch.autocast("cuda", dtype=dtype):
+            cache = m.make_cache(3, 8)
+        assert cache.dtype == dtype and cache.k_codes.shape == (3, 1, 8, 32)
+        assert m.make_cache(3, 8, dtype=dtype).dtype == dtype
+        half = WindowSelfMultiheadAttn(128, 2, window=4).to(dtype)
+        assert half.make_cache(1, 4).dtype == dtype
+    with pytest.raises(ValueError, match="fp16 or bf16"):
+        m.make_cache(3, 8, dtype=torch.float32)

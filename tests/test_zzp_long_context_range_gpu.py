@@ -218,3 +218,22 @@ def test_tangents_are_refused(dev):
         assert cache.longest == 0 and not cache.k_codes.any()
         cache.append(k, v)
         cache.attend(q)
+
+
+# ---------------------------------------------------------------------------------------------------------- the module
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_module_in_32_bits_decodes_under_autocast(dev, dtype):
+    torch.manual_seed(4)
+    m = wa.WindowSelfMultiheadAttn(256, 4, window=12, sinks=2, num_kv_heads=2, cache_bits=8).to(dev).eval()
+    half = wa.WindowSelfMultiheadAttn(256, 4, window=12, sinks=2, num_kv_heads=2, cache_bits=8).to(dev).eval()
+    half.load_state_dict(m.state_dict())
+    half.to(dtype)
+    x = torch.randn(30, 2, 256, device=dev)
+    with torch.no_grad():
+        with torch.autocast("cuda", dtype=dtype):
+            cache = m.make_cache(2, 32)
+            got = [m(x[:25], cache=cache)] + [m(x[i:i + 1], cache=cache) for i in range(25, 30)]
+        other = half.make_cache(2, 32)
+        want = [half(x[:25].to(dtype), cache=other)] + [half(x[i:i + 1].to(dtype), cache=other) for i in range(25, 30)]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert cache.dtype == dtype and all(torch.equal(a, b) for a, b in zip(cache.read(), other.read()))
