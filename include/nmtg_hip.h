@@ -768,7 +768,7 @@ int nmtg_window_attn_bwd(const void* dout, const void* q, const void* k, const v
  * elements are E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6; the lower nibble is the lower index) or E4M3 (up to
  * 448), rounded to nearest, ties to even. A block with an inf or NaN has scale byte 255 and reads
  * back as NaN. head_dim 64 or 128; the 16-bit side is fp16 or bf16. Largest magnitudes near the end of
- * the type (fp16: from 57344 in 4 bits, 63488 in 8; bf16 from 1.75 2^127 and 1.9375 2^127) round up to a
+ * the type (fp16: above 57344 in 4 bits, from 63488 in 8; bf16 1.75 2^127, 1.9375 2^127) round up to a
  * power of two that the type does not hold: they read back as inf, what is held rounded to the type;
  * the attention takes the type's largest number, so that finite keys and values give finite results.
  *

@@ -18,12 +18,19 @@ def test_tracing_is_refused():
 
 
 def test_a_module_in_32_bits_has_a_cache():
-    """Of the type that its rows will have: autocast's, or bf16 outside of it; another by name."""
+    """Of the type that its rows will have: autocast's, or bf16 outside of it; another by name. (torch.autocast does nothing for a GPU that is
+    not there: its state is set by hand.)"""
     m = WindowSelfMultiheadAttn(128, 2, window=4, num_kv_heads=1)
     assert m.make_cache(3, 8).dtype == torch.bfloat16
     for dtype in (torch.float16, torch.bfloat16):
-        with torch.autocast("cuda", dtype=dtype):
+        before = torch.get_autocast_dtype("cuda")
+        torch.set_autocast_enabled("cuda", True)
+        torch.set_autocast_dtype("cuda", dtype)
+        try:
             cache = m.make_cache(3, 8)
+        finally:
+            torch.set_autocast_enabled("cuda", False)
+            torch.set_autocast_dtype("cuda", before)
         assert cache.dtype == dtype and cache.k_codes.shape == (3, 1, 8, 32)
         assert m.make_cache(3, 8, dtype=dtype).dtype == dtype
         half = WindowSelfMultiheadAttn(128, 2, window=4).to(dtype)
