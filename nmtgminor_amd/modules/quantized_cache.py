@@ -70,12 +70,14 @@ class QuantizedKVCache:
         return self.k_codes, self.k_scales, self.v_codes, self.v_scales
 
     def append(self, k, v, counts=None):
-        """Writes k, v [T, B, H_kv, D] behind what every sequence holds. counts (int32 [B] on the device): how many of the T
-        rows are a sequence's own; those behind are written and not counted, the next rows go over them."""
+        """Writes k, v [T, B, H_kv, D] behind what every sequence holds. counts (integers [B] on the device, clamped to [0, T]): how
+        many of the T rows are a sequence's own; those behind are written and not counted, the next rows go over them."""
         t = k.shape[0]
         if self.longest + t > self.capacity:
             raise RuntimeError(f"quantised cache: {self.longest} + {t} positions do not fit a capacity of {self.capacity}")
         kv_cache_write(*self.tensors, k, v, self.lengths)
+        if counts is not None and counts.dtype != torch.bool:
+            counts = counts.clamp(0, t)
         self.lengths += t if counts is None else counts.to(self.lengths)
         self.longest += t
 

@@ -37,3 +37,17 @@ def test_a_module_in_32_bits_has_a_cache():
         assert half.make_cache(1, 4).dtype == dtype
     with pytest.raises(ValueError, match="fp16 or bf16"):
         m.make_cache(3, 8, dtype=torch.float32)
+
+
+def test_appended_counts_are_those_of_rows_that_were_appended(monkeypatch):
+    """As in window_attn_func, whose lengths are clamped to the positions there are."""
+    monkeypatch.setattr(qc, "kv_cache_write", lambda *a: None)
+    rows = torch.zeros(5, 4, 2, 64, dtype=torch.bfloat16)
+    for kind in (torch.int32, torch.int64):
+        cache = qc.QuantizedKVCache(4, 2, 64, 16, device="cpu")
+        cache.append(rows, rows, torch.tensor([9, -2, 3, 5], dtype=kind))
+        assert cache.lengths.tolist() == [5, 0, 3, 5] and cache.lengths.dtype == torch.int32 and cache.longest == 5
+        cache.append(rows[:1], rows[:1], torch.tensor([True, False, False, True]))
+        assert cache.lengths.tolist() == [6, 0, 3, 6]
+    cache.append(rows, rows, torch.tensor([1 << 32, -(1 << 32), (1 << 32) + 1, 0]))
+    assert cache.lengths.tolist() == [11, 0, 8, 6]

@@ -237,3 +237,17 @@ def test_module_in_32_bits_decodes_under_autocast(dev, dtype):
         want = [half(x[:25].to(dtype), cache=other)] + [half(x[i:i + 1].to(dtype), cache=other) for i in range(25, 30)]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert cache.dtype == dtype and all(torch.equal(a, b) for a, b in zip(cache.read(), other.read()))
+
+
+def test_module_prompt_lengths_beyond_the_prompt(dev):
+    """Attention and cache agree on what a sequence holds."""
+    torch.manual_seed(5)
+    m = wa.WindowSelfMultiheadAttn(128, 2, window=6, sinks=1, cache_bits=8).to(dev).to(torch.bfloat16).eval()
+    x = torch.randn(12, 3, 128, device=dev).to(torch.bfloat16)
+    with torch.no_grad():
+        res = []
+        for lengths in ([10, 0, 10], [1 << 33, -5, 400]):
+            cache = m.make_cache(3, 16)
+            first = m(x[:10], torch.tensor(lengths, device=dev), cache=cache)
+            res.append((first, cache.lengths.clone(), m(x[10:11], cache=cache), m(x[11:], cache=cache)))
+    assert all(torch.equal(a, b) for a, b in zip(*res)) and res[0][1].tolist() == [10, 0, 10]
