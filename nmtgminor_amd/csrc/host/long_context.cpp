@@ -18,10 +18,11 @@ struct Window {
   bool gradient = false;          // whether the backward will be run
 };
 
-// [len, batch, heads, head_dim] with a contiguous head_dim, 16-byte aligned, strides the kernels take; anything else is copied
+// [len, batch, heads, head_dim] with a contiguous head_dim, 16-byte aligned, strides the kernels take (of a single position's there is
+// none); anything else is copied
 Tensor view_of(const Tensor& x) {
-  const bool ok = x.stride(3) == 1 && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 && x.stride(2) % 8 == 0 &&
-                  reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && x.stride(0) < (1 << 24);
+  const bool ok = x.stride(3) == 1 && (x.size(0) == 1 || x.stride(0) < (1 << 24)) && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 && x.stride(2) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
   return ok ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 void put_strides(int64_t* to, const Tensor& x) {

@@ -760,10 +760,10 @@ int check_call(const char* what, int64_t len, int64_t batch, int64_t heads, int6
   NMTG_REQUIRE((len / 128 + 1) * 32 * heads * batch <= 0x7fffffff, "%s: too many blocks in one launch", what);
   return 0;
 }
-// Views whose tile of 64 rows lies within 32-bit offsets of its first row
-int check_views(const char* what, WaView* views, const void* const* pointers, const int64_t* strides, int count) {
+// Views whose tile of up to 128 rows lies within 32-bit offsets of its first row. A single position has no stride.
+int check_views(const char* what, WaView* views, const void* const* pointers, const int64_t* strides, int count, int64_t len) {
   for (int i = 0; i < count; ++i) {
-    const int64_t* s = strides + 3 * i;
+    const int64_t s[3] = {len == 1 ? 0 : strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]};
     NMTG_REQUIRE(aligned16(pointers[i]) && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0 && s[0] >= 0 && s[1] >= 0 && s[2] >= 0 && s[0] < (1 << 24),
                  "%s: every tensor must be a 16-byte aligned [len, batch, heads, head_dim] view with a contiguous head_dim and strides that are "
                  "multiples of 8 elements (position stride below 2^24)", what);
@@ -865,7 +865,7 @@ extern "C" int nmtg_window_attn_fwd(const void* q, const void* k, const void* v,
   NMTG_REQUIRE(aligned16(out_rest), "%s: out_rest must be 16-byte aligned", what);
   WaView views[4];
   const void* pointers[4] = {q, k, v, out};
-  if (int rc = check_views(what, views, pointers, strides, 4)) return rc;
+  if (int rc = check_views(what, views, pointers, strides, 4, len)) return rc;
   WaArgs a = {};
   a.q = views[0]; a.k = views[1]; a.v = views[2]; a.o = views[3];
   a.rest = out_rest;
@@ -902,7 +902,7 @@ extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void*
                "%s: a 256-byte aligned workspace of nmtg_window_attn_bwd_workspace_bytes bytes required", what);
   WaView views[8];
   const void* pointers[8] = {dout, q, k, v, out, dq, dk, dv};
-  if (int rc = check_views(what, views, pointers, strides, 8)) return rc;
+  if (int rc = check_views(what, views, pointers, strides, 8, len)) return rc;
   WaArgs a = {};
   a.d_o = views[0]; a.q = views[1]; a.k = views[2]; a.v = views[3]; a.o = views[4]; a.dq = views[5]; a.dk = views[6]; a.dv = views[7];
   a.rest = const_cast<uint8_t*>(out_rest);

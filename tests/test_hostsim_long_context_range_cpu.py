@@ -56,3 +56,16 @@ def test_finite_values_are_attended_to_as_finite(lib, dtype, d, lengths, bits): 
     sim.write(lib, cache, k, v, None, 0)
     out = sim.attend(lib, q, cache, torch.tensor(lengths, dtype=torch.int32), cap, 0, 0, scale)
     assert torch.isnan(out[0, 0, :2, :32]).all() and torch.isfinite(out[0, 0, :2, 32:]).all() and torch.isfinite(out[0, 0, 2:]).all()
+
+
+def test_one_position_has_no_stride(lib):  # noqa: F811
+    q, k, v, dout = wa.inputs(1, 2, 2, 1, 64, torch.bfloat16, "cpu")
+    out, rest, lse = torch.empty_like(q), sim.rest_of(q), torch.empty(2, 2, 1)
+    grads = [torch.empty_like(x) for x in (q, k, v)]
+    views = lambda *ts: (sim.ctypes.c_int64 * (3 * len(ts)))(*(s for x in ts for s in ((1 << 24) + 3, *x.stride()[1:3])))     # noqa: E731
+    sizes = (1, 2, 2, 1, 64, 4, 1)
+    sim.call(lib, "window_attn_fwd", q, k, v, out, rest, lse, None, views(q, k, v, out), *sizes, 0.125, sim._lib.BF16)
+    ws = sim.bytes256(sim.call(lib, "window_attn_bwd_workspace_bytes", *sizes))
+    sim.call(lib, "window_attn_bwd", dout, q, k, v, out, rest, lse, *grads, None, views(dout, q, k, v, out, *grads), *sizes, 0.125, sim._lib.BF16, ws, ws.numel())
+    assert torch.equal(out, v.expand_as(q))
+    wa.check((out, *grads), *wa.reference(q, k, v, dout, None, 4, 1, 0.125), torch.bfloat16)

@@ -251,3 +251,22 @@ def test_module_prompt_lengths_beyond_the_prompt(dev):
             first = m(x[:10], torch.tensor(lengths, device=dev), cache=cache)
             res.append((first, cache.lengths.clone(), m(x[10:11], cache=cache), m(x[11:], cache=cache)))
     assert all(torch.equal(a, b) for a, b in zip(*res)) and res[0][1].tolist() == [10, 0, 10]
+
+
+def test_one_position_of_many_heads(dev):
+    """A single position has no stride to the next one: what that stride would be limits nothing."""
+    b, h, hk, d = 4096, 64, 64, 64
+    q, k, v, dout = (torch.randn(1, b, h, d, device=dev, dtype=torch.bfloat16) for _ in range(4))
+    assert q.stride(0) >= 1 << 24
+    for x in (q, k, v):
+        x.requires_grad_()
+    out = window_attn_func(q, k, v, 3, 1)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), dout)
+    assert torch.equal(out, v) and torch.equal(dv, dout)
+    # dS = dP - D is zero but for the order of the sums in 32 bits
+    terms = 2e-5 * (dout.double() * v.detach().double()).abs().sum(-1, keepdim=True) * d ** -0.5
+    assert (dq.double().abs() <= terms * k.detach().double().abs() + 1e-6).all() and (dk.double().abs() <= terms * q.detach().double().abs() + 1e-6).all()
+    lin = torch.cat((q, k, v), 2).detach().flatten(2)
+    assert torch.equal(L.host().window_attention_projection(lin, h, hk, 3, 1, None, None), v)
+    with pytest.raises(RuntimeError, match="position stride below"):
+        window_attn_func(*(x.detach().expand(2, b, h, d).contiguous() for x in (q, k, v)), 3, 1)
