@@ -591,6 +591,8 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttn a, int64_t row
   for (int i = 0; i < 4; ++i) op[4 * c + i] = elem<T>::from_float(out[i]);
 }
 
+constexpr int64_t KV_MOST_BLOCKS = 0xffffffffll / 256;                 // a launch holds less than 2^32 threads
+
 int check_format(const char* what, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t capacity, int bits, int dtype) {
   NMTG_REQUIRE(batch >= 0 && kv_heads >= 1 && capacity >= 0, "%s: bad shape batch=%lld kv_heads=%lld capacity=%lld", what, (long long)batch,
                (long long)kv_heads, (long long)capacity);
@@ -614,7 +616,7 @@ int row_tiles(const char* what, KvRows& a, const int32_t* starts, int64_t start,
   while ((2 << a.tshift) <= (head_dim == 64 ? 16 : 8) && (1 << a.tshift) < count) ++a.tshift;
   const int64_t pairs = batch * kv_heads, pairs_per = rows >> a.tshift, pair_tiles = (pairs + pairs_per - 1) / pairs_per;
   const int64_t tiles = ((count + (1 << a.tshift) - 1) >> a.tshift) * pair_tiles;
-  NMTG_REQUIRE(pairs < (1ll << 31) && tiles <= 0x7fffffff, "%s: too many rows in one call", what);
+  NMTG_REQUIRE(pairs < (1ll << 31) && tiles <= KV_MOST_BLOCKS, "%s: too many rows in one call", what);
   a.pair_tiles = static_cast<int>(pair_tiles);
   grid = dim3(static_cast<unsigned>(tiles), 2);
   return 0;
@@ -755,7 +757,7 @@ extern "C" int nmtg_kv_cache_attn(const void* q, int64_t q_stride_t, int64_t q_s
     const int64_t need = a.splits * rows_all * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
     NMTG_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= need,
                  "%s: a 16-byte aligned workspace of %lld bytes required (nmtg_kv_cache_attn_workspace_bytes)", what, (long long)need);
-    NMTG_REQUIRE(rows_all <= 0x7fffffff, "%s: too many query rows in one call", what);
+    NMTG_REQUIRE(rows_all <= KV_MOST_BLOCKS, "%s: too many query rows in one call", what);
     a.part = static_cast<float*>(workspace);
     a.part_ml = a.part + a.splits * rows_all * head_dim;
   }

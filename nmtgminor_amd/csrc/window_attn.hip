@@ -746,6 +746,8 @@ __global__ __launch_bounds__(256) void window_dkv_join_kernel(WaArgs a, int64_t 
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
+constexpr int64_t WA_MOST_BLOCKS = 0xffffffffll / (64 * WA_WAVES);     // a launch holds less than 2^32 threads
+
 int check_call(const char* what, int64_t len, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window, int64_t sinks,
                float scale, int dtype) {
   NMTG_REQUIRE(len >= 0 && batch >= 0 && heads >= 1 && kv_heads >= 1, "%s: bad shape len=%lld batch=%lld heads=%lld kv_heads=%lld", what,
@@ -757,7 +759,7 @@ int check_call(const char* what, int64_t len, int64_t batch, int64_t heads, int6
                (long long)window, (long long)sinks);
   NMTG_REQUIRE(scale >= -1e6f && scale <= 1e6f, "%s: scale %g", what, (double)scale);
   NMTG_REQUIRE(heads <= 65535 && batch <= 65535 && len <= (1 << 24), "%s: more than 65535 heads or sequences, or 2^24 positions", what);
-  NMTG_REQUIRE((len / 128 + 1) * 32 * heads * batch <= 0x7fffffff, "%s: too many blocks in one launch", what);
+  NMTG_REQUIRE((len + WA_ROWS - 1) / WA_ROWS * heads * batch <= WA_MOST_BLOCKS, "%s: too many blocks in one launch", what);
   return 0;
 }
 // Views whose tile of up to 128 rows lies within 32-bit offsets of its first row. A single position has no stride.
@@ -909,6 +911,8 @@ extern "C" int nmtg_window_attn_bwd(const void* dout, const void* q, const void*
   a.lse = const_cast<float*>(softmax_lse); a.stats = static_cast<float*>(workspace);
   a.stat_rows = stat_rows(len);
   const DkvPlan plan(len, batch, heads, kv_heads, head_dim, window, sinks);
+  NMTG_REQUIRE((static_cast<int64_t>(plan.key_blocks) * plan.parts + static_cast<int64_t>(plan.sink_blocks) * plan.chunks) * kv_heads * batch <= WA_MOST_BLOCKS,
+               "%s: too many blocks in one launch", what);
   a.part = a.stats + stat_floats(len, batch, heads);
   a.sink_part = a.part + plan.part_floats;
   a.key_blocks = plan.key_blocks; a.sink_blocks = plan.sink_blocks; a.parts = plan.parts; a.chunks = plan.chunks;

@@ -69,3 +69,21 @@ def test_one_position_has_no_stride(lib):  # noqa: F811
     sim.call(lib, "window_attn_bwd", dout, q, k, v, out, rest, lse, *grads, None, views(dout, q, k, v, out, *grads), *sizes, 0.125, sim._lib.BF16, ws, ws.numel())
     assert torch.equal(out, v.expand_as(q))
     wa.check((out, *grads), *wa.reference(q, k, v, dout, None, 4, 1, 0.125), torch.bfloat16)
+
+
+def test_launches_beyond_32_bits_are_refused(lib):  # noqa: F811
+    """A launch holds less than 2^32 threads: 2^24 blocks of 256. Refused before anything runs, the backward's later launches too."""
+    x = torch.zeros(64, dtype=torch.bfloat16)
+    st = lambda n: (sim.ctypes.c_int64 * (3 * n))(*([0, 64, 64] * n))                       # noqa: E731
+    lse = torch.zeros(1)
+    for sizes in ((1, 60000, 300, 300, 64, 4, 0), (1 << 20, 2, 60000, 60000, 64, 4, 0)):
+        assert "too many blocks" in sim.call(lib, "window_attn_fwd", x, x, x, x, None, lse, None, st(4), *sizes, 0.125, sim._lib.BF16, expect=-1)
+    # the forward fits, the chunks and parts of dK and dV do not
+    sizes = (8192, 128, 1024, 1024, 64, 1, 8192)
+    ws = sim.bytes256(256)
+    huge = sim.call(lib, "window_attn_bwd_workspace_bytes", *sizes)
+    assert "too many blocks" in sim.call(lib, "window_attn_bwd", x, x, x, x, x, None, lse, x, x, x, None, st(8), *sizes, 0.125, sim._lib.BF16, ws, huge, expect=-1)
+    # rows of a broadcast key written to 2^31 - 1 positions
+    codes, scales = torch.zeros(64, dtype=torch.uint8), torch.zeros(2, dtype=torch.uint8)
+    n = (1 << 30) - 1
+    assert "too many rows" in sim.call(lib, "kv_cache_write", x, 0, 0, 0, x, 0, 0, 0, codes, scales, codes, scales, None, 0, n, 4, 1, 64, n, 8, sim._lib.BF16, expect=-1)
