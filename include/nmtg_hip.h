@@ -729,9 +729,10 @@ int nmtg_multi_tensor_l2norm_scale(int n_tensors, const void* const* in, void* c
  * q, out, dout, dq [len, batch, heads, head_dim]; k, v, dk, dv [len, batch, kv_heads, head_dim],
  * heads a multiple of kv_heads: query head h reads key / value head h / (heads / kv_heads).
  * strides: HOST array of three int64 per tensor (position, sequence, head; in elements, multiples of
- * 8, the position's below 2^24 and not looked at where len is 1; head_dim contiguous), in the order of the tensor arguments: q, k, v, out for the forward and
- * dout, q, k, v, out, dq, dk, dv for the backward. head_dim 64 or 128, fp16 or bf16, products and
- * sums in fp32, probabilities and score gradients rounded to the 16-bit type for their products.
+ * 8, the position's below 2^24 and not looked at where len is 1; head_dim contiguous), in the order of
+ * the tensor arguments: q, k, v, out for the forward and dout, q, k, v, out, dq, dk, dv for the backward.
+ * head_dim 64 or 128, fp16 or bf16, products and sums in fp32, probabilities and score gradients rounded
+ * to the 16-bit type for their products.
  * out_rest: what rounding took from out, in 8 bits, units of a power of two per row (finite for every
  * finite out) and an order of its own: batch * heads * ceil(len / 32) * 32 * head_dim bytes, 16-byte
  * aligned, written by the forward where it is not null and read by the backward, with out, as the
