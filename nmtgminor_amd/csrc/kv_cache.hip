@@ -302,8 +302,10 @@ struct KvTile {
       for (int e = 0; e < 8; ++e) {
         const uint32_t row = min(static_cast<uint32_t>(16 * (e / 4) + 4 * g + (e & 3)), last);
         load_v(e, vp, row, r);
-        if constexpr (SB == 4) vs[e] = *reinterpret_cast<const uint32_t*>(vsp + row * SB);
-        else vs[e] = *reinterpret_cast<const uint16_t*>(vsp + row * SB);
+        typedef uint32_t word __attribute__((aligned(1)));
+        typedef uint16_t half __attribute__((aligned(1)));
+        if constexpr (SB == 4) vs[e] = *reinterpret_cast<const word*>(vsp + row * SB);
+        else vs[e] = *reinterpret_cast<const half*>(vsp + row * SB);
       }
     }
   }

@@ -270,3 +270,21 @@ def test_one_position_of_many_heads(dev):
     assert torch.equal(L.host().window_attention_projection(lin, h, hk, 3, 1, None, None), v)
     with pytest.raises(RuntimeError, match="position stride below"):
         window_attn_func(*(x.detach().expand(2, b, h, d).contiguous() for x in (q, k, v)), 3, 1)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d,lengths", [(64, [70, 33]), (128, [95, 64])])
+def test_scales_at_any_address(dev, d, lengths, bits):
+    """Scale bytes are a dense tensor of bytes, which may begin anywhere."""
+    b, hk, cap = 2, 2, max(lengths)
+    k, v = (torch.randn(cap, b, hk, d, device=dev).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(1, b, 4, d, device=dev).to(torch.bfloat16)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    dense = qc.buffers(b, hk, cap, d, bits, dev)
+    qc.kv_cache_write(*dense, k, v, 0)
+    want = qc.kv_cache_attend(q, *dense, n, cap)
+    for offset in (1, 3):
+        moved = [torch.zeros(x.numel() + 16, dtype=torch.uint8, device=dev)[offset if i % 2 else 0:][:x.numel()].view(x.shape) for i, x in enumerate(dense)]
+        qc.kv_cache_write(*moved, k, v, 0)
+        assert all(torch.equal(x, y) for x, y in zip(moved, dense)) and torch.equal(qc.kv_cache_attend(q, *moved, n, cap), want)
+        assert all(torch.equal(x, y) for x, y in zip(qc.kv_cache_read(*moved, 0, cap), qc.kv_cache_read(*dense, 0, cap)))
