@@ -739,7 +739,8 @@ int nmtg_multi_tensor_l2norm_scale(int n_tensors, const void* const* in, void* c
  * forward left both; without it (null) the backward takes dout . out from the rounded out.
  * softmax_lse: fp32 [batch, heads, len], natural logarithm (-inf where nothing is visible), written
  * by the forward and read by the backward. workspace: nmtg_window_attn_bwd_workspace_bytes bytes,
- * 256-byte aligned. Positions behind a length are never read. An inf or NaN in a row of k or v may
+ * 256-byte aligned. Exponents are differences of fp32 products, off by up to 2^-23 of a score: scores
+ * are expected below 10^4 or so in magnitude. Positions behind a length are never read. An inf or NaN in a row of k or v may
  * reach, as zero times it, queries that do not see the row but share an aligned 32 with one that sees
  * some row of the aligned 64 around it; in a row of q or dout, the gradients of keys likewise.
  * ------------------------------------------------------------------------------------------ */
@@ -783,7 +784,9 @@ int nmtg_window_attn_bwd(const void* dout, const void* q, const void* k, const v
  *   clamped to [0, capacity]) and sees positions up to its own, with window > 0 those of its window
  *   and the first `sinks` only. A query that sees nothing gets zeros. longest: an upper bound of
  *   lengths known to the host, which sizes the launch and the workspace; results do not depend on it
- *   beyond the order of sums. q, out [tq, batch, heads, head_dim] by three strides. workspace:
+ *   beyond the order of sums. Scores as for window attention. An inf or NaN among the values reaches the
+ *   queries that see it and, with tq > 1, may reach other new positions of its sequence, as zero times it.
+ *   q, out [tq, batch, heads, head_dim] by three strides. workspace:
  *   nmtg_kv_cache_attn_workspace_bytes bytes, 16-byte aligned (none where that is 0).
  * ------------------------------------------------------------------------------------------ */
 int nmtg_kv_cache_write(const void* k, int64_t k_stride_t, int64_t k_stride_b, int64_t k_stride_h,

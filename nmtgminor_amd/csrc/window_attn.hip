@@ -22,12 +22,18 @@
 // Rounding. Scores, the softmax's statistics, D and all sums are in 32 bits. P and dS are rounded to the tensors' type, which the
 // products take: about as much error as rounding the result adds, so that gradients are off by 1.4 times what sums in 32 bits
 // rounded once are. D is that of O before its rounding: the forward of a training step leaves what the rounding took in 8 bits
-// per element (D of the rounded O alone: 1.5 times the error, in 98% of the time of forward and backward).
+// per element, a byte each that is kept until then. That takes 2.0 to 2.2% of the time of forward and backward; without it gradients of values
+// of unit variance are off by 1.5 times instead of 1.45, and those of values with a large common part by up to thirty times as much.
+// Exponents are differences of products in 32 bits, the backward's also of the kept logarithm: off by 2^-23 of a score, so that scores beyond
+// 10^4 or so in magnitude cost more than the roundings above.
 //
-// What bounds them (MI355X). Head dimension 128: the matrix cores, busy 46 to 57% of the cycles, at the 1.9 to 2.1 GHz that the power limit
-// leaves: one kernel's time shrinks when another of the step waits more. Forward over 16384 positions, window 4096, 32 heads: 930 us,
-// 1.04 PFLOP/s (a large library product: 1.43). Head dimension 64: the vector instructions of the softmax, 42 to 69% of the cycles
-// beside 32 to 38% of products: 8 x 2048 positions, window 512, 16 heads: 73 us forward, 83 dQ, 114 dK and dV.
+// What bounds them (MI355X; shares of the cycles in which a compute unit is busy). Head dimension 128: the matrix cores, busy 46 to 57%, at the
+// 1.9 to 2.1 GHz that the power limit leaves: one kernel's time shrinks when another of the step waits more. Forward over 16384 positions,
+// window 4096, 32 heads: 925 us, 1.04 PFLOP/s (a large library product: 1.43). Head dimension 64, 8 x 2048 positions, window 512, 16
+// heads, a pass of 228 us: forward and dQ the vector instructions, 70 and 61% beside 32 and 37% of products (6.7 and 7.9 per score
+// that is computed, masks and the blocks' beginnings and ends among them; a score is half the products of head dimension 128). dK and dV
+// wait: 46% of the wavefronts' cycles, with the vector units at 42%, the matrix cores at 35 and the LDS at 29. Operands are read in front of
+// their products: four reads ahead take 16 registers, of which three wavefronts on a SIMD leave 6. 61, 73 and 99 us where counters ran.
 // No atomics, and what blocks leave to be added up is added in a fixed order: results do not depend on scheduling.
 #include "flash_tile.hip.h"
 #include <algorithm>
@@ -290,7 +296,7 @@ constexpr float WA_FLOOR = -5e29f;   // a running maximum before the first visib
 
 // Key tiles of 64, or of 32 for head_dim 128: with the scores of 32 keys a wavefront needs at most 168 registers there, and three of them
 // share a SIMD (32 KB of LDS a block). What bounds the kernel is how much of the softmax runs under other wavefronts' products:
-// prompt of 16384 positions, window 4096, 32 heads of 128: 1088 us with two wavefronts and tiles of 64, 1023 with three, 930 as it is. (For
+// prompt of 16384 positions, window 4096, 32 heads of 128: 1088 us with two wavefronts and tiles of 64, 1023 with three, 925 as it is. (For
 // head_dim 64 tiles of 32 keys take as long as tiles of 64.)
 template <int D> constexpr int fwd_tile() { return D == 64 ? 64 : 32; }
 
