@@ -87,6 +87,10 @@ class WindowSelfMultiheadAttn(nn.Module):
             raise RuntimeError("window attention: qk_norm needs pos_emb, the tables (cos, sin) of positions")
         lin = linear_function(inputs, self.in_proj_weight, self.in_proj_bias)
         sizes = (self.num_heads, self.num_kv_heads, self.num_kv_heads)
+        # (before the norms: their node would keep the cache's lengths, which append changes)
+        if cache is not None and torch.is_grad_enabled() and (
+                lin.requires_grad or self.qk_norm and (self.q_norm_weight.requires_grad or self.k_norm_weight.requires_grad)):
+            raise RuntimeError("window attention: decoding from a quantised cache has no gradient, call it under torch.no_grad()")
         if self.qk_norm:
             q, k, v = lin.view(t, b, -1, self.head_dim).split(sizes, dim=2)
             with no_autocast():
@@ -105,8 +109,6 @@ class WindowSelfMultiheadAttn(nn.Module):
             first = cache.longest == 0
             if not first and lengths is not None:
                 raise RuntimeError("window attention: lengths go with the prompt, a decoding step has the same positions for every sequence")
-            if torch.is_grad_enabled() and lin.requires_grad:
-                raise RuntimeError("window attention: decoding from a quantised cache has no gradient, call it under torch.no_grad()")
             cache.append(k, v, lengths)
             if not first:
                 context = cache.attend(q, self.window, self.sinks)
