@@ -863,8 +863,9 @@ int nmtg_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void* 
  *   change nothing and have zero outputs and gradients. scale: 1e-6 <= |scale| <= 1e6.
  * Whole sequences run in chunks on the matrix cores. A product with the state takes it rounded to the
  * tensors' type (fp16: relative to the largest element of a slice of 32 columns); what S itself is updated
- * with is carried to 22 bits (fp16: of the largest of 32 positions and columns) or 24 (bf16, where a state or its gradient is asked
- * for; 16 otherwise: the last bit of an output may depend on what is asked for). bf16: S below 2^110. An inf or NaN among k or v reaches every position from its
+ * with is carried to 22 bits (fp16: of the largest of 32 positions and columns, or of 2^-127 of the largest S in them) or 24 (bf16, where a state or its gradient is asked
+ * for; 16 otherwise: the last bit of an output may depend on what is asked for). S is finite where it is in 32 bits (bf16: below 2^110), and
+ * dstate_in where dstate_out / scale is. An inf or NaN among k or v reaches every position from its
  * own on, as it must, and may reach up to 31 positions before it, as zero times it.
  * Backward: states: the workspace of the forward of the same inputs, as that left it (null where it has
  *   none). dq, dk, dv from dout and, where given, dstate_out (the gradient of state_out); dstate_in

@@ -146,11 +146,12 @@ struct LaLoader {
 };
 
 // 2^k with k so that `largest`, if it is at least 2^LOWEST, times it is at least 2^14 and below 2^15, and its inverse: where fp16 holds
-// all its bits, and two of its numbers 22. room: as many powers of two less
+// all its bits, and two of its numbers 22. room: as many powers of two less; up is 2^(14 - least) at most
 struct Pow2 { float up, down; };
+__device__ __forceinline__ int exponent_of(float x) { return static_cast<int>(__float_as_uint(x) >> 23) - 127; }      // x >= 0
 template <int LOWEST>
-__device__ __forceinline__ Pow2 to_half_range(float largest, int room = 0) {
-  const int e = max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, LOWEST) + room;
+__device__ __forceinline__ Pow2 to_half_range(float largest, int room = 0, int least = LOWEST) {
+  const int e = max(max(exponent_of(largest), LOWEST) + room, least);
   return {__uint_as_float(static_cast<uint32_t>(141 - e) << 23), __uint_as_float(static_cast<uint32_t>(113 + e) << 23)};
 }
 
@@ -255,7 +256,8 @@ __global__ __launch_bounds__(2 * D, 2) void linear_walk_kernel(LaArgs a) {
   const float front = __builtin_amdgcn_exp2f(static_cast<float>(li + e) * l2) * a.scale;
   // The registers hold the state times 2^owed unit.up: decays are owed to it until they come to 2^-LA_OWED (the weights of what is added
   // grow instead), which is less work, and no factor of a chunk multiplies its own rounding over the chunks. unit: fp16's
-  // numbers, which lambda^.. z is split into, have their bits where the chunk's largest z is.
+  // numbers, which lambda^.. z is split into, have their bits where the chunk's largest z is, and the state in the registers, whatever it was given
+  // as, stays below 2^126 (where segments begin with zero, 2^24 positions of fp16's values make 2^94 at most).
   float owed = 0.f;
   Pow2 unit = {1.f, 1.f};
   const bool lean = !HALF && LA_CHUNK * -l2 <= LA_OWED;
@@ -287,7 +289,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_walk_kernel(LaArgs a) {
     uint4 zf[2];                                                // z: column `col`, 16 rows each
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) zf[kk] = reader.column_operand(img + ZIMG, wave, kk);
-    float out[16];
+    float out[16], highest = 0.f;                               // highest: of the state in the registers (fp16)
     if constexpr (OUT) {
       uint4 xf[D / 16], yf[D / 16];
 #pragma unroll
@@ -315,6 +317,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_walk_kernel(LaArgs a) {
           top = wave_max(top);
         }
         range = to_half_range<-112>(top);
+        highest = top;
       }
 #pragma unroll
       for (int ss = 0; ss < D / 16; ++ss) {
@@ -390,7 +393,8 @@ __global__ __launch_bounds__(2 * D, 2) void linear_walk_kernel(LaArgs a) {
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
           for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(zv[kk][j]));
-        const Pow2 next = to_half_range<-24>(fminf(wave_max(top), 65504.f), static_cast<int>(ceilf(owed)));
+        const int least = OUT ? exponent_of(highest * pay) - exponent_of(unit.up) - 111 : -24;
+        const Pow2 next = to_half_range<-24>(fminf(wave_max(top), 65504.f), static_cast<int>(ceilf(owed)), least);
         pay *= unit.down * next.up;
         unit = next;
       }

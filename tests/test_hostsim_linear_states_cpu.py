@@ -1,0 +1,36 @@
+"""States of linear attention at the ends of their range, executed on the CPU: the kernels' own source through tests/hostsim, called by the
+C ABI, against the definition in 64 bits."""
+import pytest
+import torch
+
+import test_zzr_linear_attention_gpu as la
+from test_hostsim_linear_attention_cpu import linear
+from test_hostsim_long_context_cpu import hostsim_build, lib      # noqa: F401 (a fixture among them)
+
+pytestmark = pytest.mark.skipif(not hostsim_build.available(), reason="no clang++ to build the CPU simulator")
+F16 = torch.float16
+
+
+@pytest.mark.parametrize("t,d", [(40, 64), (100, 128)])
+@pytest.mark.parametrize("size", [1e24, 1e28, 3e37])
+def test_large_states_meet_small_rows_in_fp16(lib, t, d, size):     # noqa: F811
+    """A state of a finite size stays finite whatever the rows behind it are: zeros, or some that grow again."""
+    (q, k, v, dout), (s0, dlast) = la.inputs(t, 1, 6, d, F16, "cpu", 21)
+    s0, dlast = s0.clamp(-3, 3) * size, dlast.clamp(-3, 3) * size
+    ld = la.decays(6)
+    for rows in (torch.zeros(t), (torch.arange(t) >= 33).float(), (torch.arange(t) < 7).float() * 2.0 ** -20):
+        vv, gg = (x * rows.to(F16)[:, None, None, None] for x in (v, dout))
+        got = linear(lib, q, k, vv, gg, ld, None, 1.0, F16, s0, dlast, True)
+        want, mag = la.reference(q, k, vv, gg, ld, None, 1.0, s0, dlast)
+        la.check({n: got[n] for n in ("last", "dstate")}, want, mag)
+
+
+@pytest.mark.parametrize("size", [1e10, 1e30])
+def test_large_columns_leave_small_ones_their_bits_in_fp16(lib, size):     # noqa: F811
+    (q, k, v, dout), (s0, dlast) = la.inputs(70, 1, 6, 64, F16, "cpu", 22)
+    for x in (s0, dlast):
+        x[..., 3] *= size
+    ld = la.decays(6)
+    got = linear(lib, q, k, v, dout, ld, None, 1.0, F16, s0, dlast, True)
+    want, mag = la.reference(q, k, v, dout, ld, None, 1.0, s0, dlast)
+    la.check({n: got[n] for n in ("last", "dstate")}, want, mag)
