@@ -109,6 +109,7 @@ struct NormNode : Function<NormNode> {
 Tensor table_of(const Tensor& t, const Tensor& q) {
   check_device(t, q);
   TORCH_CHECK(!t.requires_grad(), "qk_norm_rotary: the tables of positions have no gradient");
+  no_tangents("qk_norm_rotary", {&t});
   TORCH_CHECK(t.dim() >= 2 && t.numel() == t.size(0) * q.size(3) && t.size(-1) == q.size(3), "qk_norm_rotary: tables must be [positions, head_dim] or [positions, 1, head_dim], got ",
               t.sizes());
   TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == q.scalar_type(), "qk_norm_rotary: tables must be fp32 or of the rows' type");

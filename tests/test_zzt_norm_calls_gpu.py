@@ -1,0 +1,33 @@
+"""Calls of the norms with rotation, of linear attention's step and of the modules around them that their documentation allows or refuses."""
+import pytest
+import torch
+
+from nmtgminor_amd.modules.linear_attention import LinearSelfMultiheadAttn, linear_attn_step
+from nmtgminor_amd.modules.qk_norm import qk_norm_rotary_func
+from nmtgminor_amd.modules.window_attention import WindowSelfMultiheadAttn
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def tables(rows, d, dev, dtype=torch.float32):
+    angles = torch.arange(rows, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, d, 2, dtype=torch.float64) / d)
+    angles = torch.cat((angles, angles), 1)
+    return angles.cos().to(dtype).to(dev), angles.sin().to(dtype).to(dev)
+
+
+def rows(t, b, h, d, dtype, dev, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.randn(t, b, h, d, generator=gen).to(dtype).to(dev) for _ in range(3)]
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_of_the_tables_are_refused(dev, which, grad):
+    q, k, _ = rows(3, 1, 2, 64, F16, dev)
+    q.requires_grad_(grad)
+    pos = list(tables(4, 64, dev))
+    with torch.autograd.forward_ad.dual_level():
+        pos[which] = torch.autograd.forward_ad.make_dual(pos[which], torch.ones_like(pos[which]))
+        with pytest.raises(RuntimeError, match="jvp"):
+            qk_norm_rotary_func(q, k, None, None, *pos)
