@@ -108,7 +108,7 @@ struct NormNode : Function<NormNode> {
 // [rows, head_dim] from the reference's [rows, 1, head_dim] or that itself
 Tensor table_of(const Tensor& t, const Tensor& q) {
   check_device(t, q);
-  TORCH_CHECK(!t.requires_grad(), "qk_norm_rotary: the tables of positions have no gradient");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), "qk_norm_rotary: the tables of positions have no gradient");
   no_tangents("qk_norm_rotary", {&t});
   TORCH_CHECK(t.dim() >= 2 && t.numel() == t.size(0) * q.size(3) && t.size(-1) == q.size(3), "qk_norm_rotary: tables must be [positions, head_dim] or [positions, 1, head_dim], got ",
               t.sizes());

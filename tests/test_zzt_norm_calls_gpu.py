@@ -31,3 +31,15 @@ def test_tangents_of_the_tables_are_refused(dev, which, grad):
         pos[which] = torch.autograd.forward_ad.make_dual(pos[which], torch.ones_like(pos[which]))
         with pytest.raises(RuntimeError, match="jvp"):
             qk_norm_rotary_func(q, k, None, None, *pos)
+
+
+def test_tables_that_learn_elsewhere(dev):
+    """Where nothing is recorded they are tables like others."""
+    q, k, _ = rows(3, 1, 2, 64, F16, dev)
+    pos = tables(4, 64, dev)
+    want = qk_norm_rotary_func(q, k, None, None, *pos)
+    learned = [x.clone().requires_grad_() for x in pos]
+    with torch.no_grad():
+        assert all(torch.equal(x, y) for x, y in zip(qk_norm_rotary_func(q, k, None, None, *learned), want))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        qk_norm_rotary_func(q, k, None, None, *learned)
