@@ -38,6 +38,8 @@ def linear_attn_step(q, k, v, log_decay, state, state_out=None, scale=None, leng
     """The recurrence itself, position by position, in fp32 (one position, or a few). state is written in place, or left alone with
     another tensor state_out to write; both contiguous. lengths: how many of the T positions are a sequence's own."""
     L.refuse_tracing("linear attention")
+    if torch.is_autocast_enabled():
+        q, k, v = cast_if_autocast_enabled(q, k, v)
     return L.host().linear_attention_step(q, k, v, log_decay, state, state_out, scale, lengths)
 
 

@@ -43,3 +43,12 @@ def test_tables_that_learn_elsewhere(dev):
         assert all(torch.equal(x, y) for x, y in zip(qk_norm_rotary_func(q, k, None, None, *learned), want))
     with pytest.raises(RuntimeError, match="no gradient"):
         qk_norm_rotary_func(q, k, None, None, *learned)
+
+
+def test_step_under_autocast(dev):
+    q, k, v = rows(2, 3, 2, 64, torch.float32, dev)
+    decay, states = torch.tensor([-0.1, -0.01], device=dev), [torch.ones(3, 2, 64, 64, device=dev) for _ in range(2)]
+    want = linear_attn_step(q.bfloat16(), k.bfloat16(), v.bfloat16(), decay, states[0])
+    with torch.autocast("cuda", dtype=BF16):
+        got = linear_attn_step(q, k, v, decay, states[1])
+    assert got.dtype == BF16 and torch.equal(got, want) and torch.equal(*states) and states[1].dtype == torch.float32
