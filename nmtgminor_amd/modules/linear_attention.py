@@ -112,11 +112,11 @@ class LinearSelfMultiheadAttn(nn.Module):
         decay = self.log_decay
         if state is not None and torch.is_grad_enabled() and lin.requires_grad:
             raise RuntimeError("linear attention: decoding from a state has no gradient, call it under torch.no_grad()")
+        q, k, v = lin.view(t, b, 3 * self.num_heads, self.head_dim).split(self.num_heads, dim=2)
+        if self.qk_norm:
+            positions = None if state is None else state.lengths
+            q, k = qk_norm_rotary_func(q, k, self.q_norm_weight, self.k_norm_weight, *pos_emb, positions=positions)
         with no_autocast():
-            q, k, v = lin.view(t, b, 3 * self.num_heads, self.head_dim).split(self.num_heads, dim=2)
-            if self.qk_norm:
-                positions = None if state is None else state.lengths
-                q, k = qk_norm_rotary_func(q, k, self.q_norm_weight, self.k_norm_weight, *pos_emb, positions=positions)
             if state is None:
                 context = linear_attn_func(q, k, v, decay, lengths=lengths)
             else:

@@ -14,7 +14,7 @@ from ._autocast import cast_if_autocast_enabled, no_autocast
 
 def qk_norm_rotary_func(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6):
     """q and k may be slots of one projection (any strides with a contiguous D that are multiples of 8). Weights [D], fp32 or of the
-    rows' type, or None for both. cos, sin: [positions, D] or [positions, 1, D], fp32 or of the rows' type. positions: None (row t of
+    rows' type, or None for both (under autocast weights and tables of 16 bits take its type with the rows). cos, sin: [positions, D] or [positions, 1, D], fp32 or of the rows' type. positions: None (row t of
     the tables for position t), an int (of the first row), integers [B] on the device (of every sequence's first row: a decoder's
     lengths) or [T, B] (of every row). An int that leads out of the tables is an error, positions on the device are clamped to them."""
     L.refuse_tracing("qk_norm_rotary")
@@ -24,5 +24,7 @@ def qk_norm_rotary_func(q, k, q_weight, k_weight, cos, sin, positions=None, eps=
     if not torch.is_autocast_enabled():
         return L.host().qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, start, eps)
     q, k = cast_if_autocast_enabled(q, k)
+    # (those in 32 bits stay so)
+    q_weight, k_weight, cos, sin = (x.to(q.dtype) if x is not None and x.dtype in (torch.float16, torch.bfloat16) else x for x in (q_weight, k_weight, cos, sin))
     with no_autocast():
         return L.host().qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, start, eps)

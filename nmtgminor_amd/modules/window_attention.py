@@ -93,8 +93,7 @@ class WindowSelfMultiheadAttn(nn.Module):
             raise RuntimeError("window attention: decoding from a quantised cache has no gradient, call it under torch.no_grad()")
         if self.qk_norm:
             q, k, v = lin.view(t, b, -1, self.head_dim).split(sizes, dim=2)
-            with no_autocast():
-                q, k = qk_norm_rotary_func(q, k, self.q_norm_weight, self.k_norm_weight, *pos_emb, positions=None if cache is None else cache.lengths)
+            q, k = qk_norm_rotary_func(q, k, self.q_norm_weight, self.k_norm_weight, *pos_emb, positions=None if cache is None else cache.lengths)
         if cache is None or cache.longest == 0:
             with no_autocast():
                 if self.qk_norm:

@@ -52,3 +52,23 @@ def test_step_under_autocast(dev):
     with torch.autocast("cuda", dtype=BF16):
         got = linear_attn_step(q, k, v, decay, states[1])
     assert got.dtype == BF16 and torch.equal(got, want) and torch.equal(*states) and states[1].dtype == torch.float32
+
+
+def test_weights_and_tables_of_another_type_under_autocast(dev):
+    """Weights and tables in 32 bits stay what they are, others take autocast's type as the rows do."""
+    q, k, g = rows(5, 2, 2, 64, F16, dev)
+    w = [torch.linspace(0.5, 1.5, 64, device=dev).half().requires_grad_() for _ in range(2)]
+    pos = tables(8, 64, dev, F16)
+    same = [x.detach().bfloat16().requires_grad_() for x in w]
+    want = qk_norm_rotary_func(q.bfloat16(), k.bfloat16(), *same, *(x.bfloat16() for x in pos))
+    with torch.autocast("cuda", dtype=BF16):
+        got = qk_norm_rotary_func(q, k, *w, *pos)
+    assert all(x.dtype == BF16 and torch.equal(x, y) for x, y in zip(got, want))
+    one, two = (torch.autograd.grad(x, y, (g.bfloat16(), g.bfloat16())) for x, y in ((got, w), (want, same)))
+    assert all(x.dtype == F16 and torch.equal(x, y.half()) for x, y in zip(one, two))
+    x = torch.randn(6, 2, 128, device=dev).half()
+    for m in (LinearSelfMultiheadAttn(128, 2), WindowSelfMultiheadAttn(128, 2, window=4, qk_norm=True)):
+        m = m.to(dev).half()
+        with torch.autocast("cuda", dtype=BF16):
+            out = m(x, pos_emb=pos)
+        assert out.dtype == BF16 and torch.isfinite(out).all()
