@@ -11,12 +11,14 @@ using torch::autograd::variable_list;
 
 namespace {
 
-// [len, batch, heads, head_dim] with a contiguous head_dim, 16-byte aligned, strides the kernels take; anything else is copied
-Tensor view_of(const Tensor& x) {
-  const bool ok = x.stride(3) == 1 && (x.size(0) == 1 || x.stride(0) < (1 << 24)) && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 && x.stride(2) % 8 == 0 &&
+// [len, batch, heads, head_dim] with a contiguous head_dim, 16-byte aligned, strides the kernels take (linear attention's positions are
+// less than 2^24 elements apart); anything else is copied
+Tensor view_of(const Tensor& x, int64_t below = 1 << 24) {
+  const bool ok = x.stride(3) == 1 && (x.size(0) == 1 || x.stride(0) < below) && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 && x.stride(2) % 8 == 0 &&
                   reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
   return ok ? x : x.clone(at::MemoryFormat::Contiguous);
 }
+Tensor norm_view(const Tensor& x) { return view_of(x, std::numeric_limits<int64_t>::max()); }
 template <size_t N>
 void put_strides(int64_t (&to)[N], std::initializer_list<const Tensor*> tensors) {
   size_t i = 0;
@@ -88,7 +90,7 @@ struct NormNode : Function<NormNode> {
     const Tensor &q = s[0], &k = s[1], &wq = s[2], &wk = s[3];
     NormArgs a{s[4], s[5], s[6], ctx->saved_data["start"].toInt(), ctx->saved_data["eps"].toDouble()};
     Launch on(q);
-    const Tensor gq = view_of(g[0]), gk = view_of(g[1]);
+    const Tensor gq = norm_view(g[0]), gk = norm_view(g[1]);
     Tensor dq = empty_like_sized(q, q.sizes()), dk = empty_like_sized(k, k.sizes()), dwq, dwk;
     if (wq.defined()) {
       dwq = empty_like_sized(wq, wq.sizes());
@@ -234,10 +236,10 @@ void define_linear_attention(pybind11::module_& m) {
     }
     if (!wants_grad({&q, &k, &wq, &wk})) {
       no_tangents(what, {&q, &k, &wq, &wk});
-      auto out = norm_fwd(view_of(q), view_of(k), wq.defined() ? dense(wq) : wq, wk.defined() ? dense(wk) : wk, a);
+      auto out = norm_fwd(norm_view(q), norm_view(k), wq.defined() ? dense(wq) : wq, wk.defined() ? dense(wk) : wk, a);
       return std::make_tuple(out.first, out.second);
     }
-    const variable_list out = NormNode::apply(view_of(q), view_of(k), some(wq), some(wk), &a);
+    const variable_list out = NormNode::apply(norm_view(q), norm_view(k), some(wq), some(wk), &a);
     return std::make_tuple(out[0], out[1]);
   });
   m.def("linear_attention", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, optional<double> scale, const optional<Tensor>& lengths,

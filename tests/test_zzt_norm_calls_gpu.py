@@ -72,3 +72,21 @@ def test_weights_and_tables_of_another_type_under_autocast(dev):
         with torch.autocast("cuda", dtype=BF16):
             out = m(x, pos_emb=pos)
         assert out.dtype == BF16 and torch.isfinite(out).all()
+
+
+def test_rows_far_apart_are_read_where_they_are(dev):
+    t, b, h, d, far = 2, 64, 64, 64, 1 << 24
+    q, k, g = rows(t, b, h, d, BF16, dev, 3)
+    room = torch.empty(t * far, dtype=BF16, device=dev)
+    apart = [room.as_strided(x.shape, (far, h * d, d, 1), b * h * d * i).copy_(x) for i, x in enumerate((q, k, g))]
+    pos = tables(t, d, dev)
+    want = qk_norm_rotary_func(q, k, None, None, *pos)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = qk_norm_rotary_func(*apart[:2], None, None, *pos)
+    assert torch.cuda.max_memory_allocated() - before < 3 * q.numel() * 2          # the two results, no copies of the rows
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    near, leaves = q.requires_grad_(), apart[0].detach().requires_grad_()
+    one, two = (torch.autograd.grad(qk_norm_rotary_func(x, k, None, None, *pos)[0], x, y)[0] for x, y in ((near, g), (leaves, apart[2])))
+    assert torch.equal(one, two)
