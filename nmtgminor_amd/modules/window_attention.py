@@ -92,7 +92,7 @@ class WindowSelfMultiheadAttn(nn.Module):
                 lin.requires_grad or self.qk_norm and (self.q_norm_weight.requires_grad or self.k_norm_weight.requires_grad)):
             raise RuntimeError("window attention: decoding from a quantised cache has no gradient, call it under torch.no_grad()")
         if self.qk_norm:
-            q, k, v = lin.view(t, b, -1, self.head_dim).split(sizes, dim=2)
+            q, k, v = lin.view(t, b, sum(sizes), self.head_dim).split(sizes, dim=2)
             q, k = qk_norm_rotary_func(q, k, self.q_norm_weight, self.k_norm_weight, *pos_emb, positions=None if cache is None else cache.lengths)
         if cache is None or cache.longest == 0:
             with no_autocast():
@@ -104,7 +104,7 @@ class WindowSelfMultiheadAttn(nn.Module):
             if self.qk_norm:
                 q, k, v = q.detach(), k.detach(), v.detach()
             else:
-                q, k, v = lin.detach().view(t, b, -1, self.head_dim).split(sizes, dim=2)
+                q, k, v = lin.detach().view(t, b, sum(sizes), self.head_dim).split(sizes, dim=2)
             first = cache.longest == 0
             if not first and lengths is not None:
                 raise RuntimeError("window attention: lengths go with the prompt, a decoding step has the same positions for every sequence")

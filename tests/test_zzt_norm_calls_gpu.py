@@ -90,3 +90,14 @@ def test_rows_far_apart_are_read_where_they_are(dev):
     near, leaves = q.requires_grad_(), apart[0].detach().requires_grad_()
     one, two = (torch.autograd.grad(qk_norm_rotary_func(x, k, None, None, *pos)[0], x, y)[0] for x, y in ((near, g), (leaves, apart[2])))
     assert torch.equal(one, two)
+
+
+@pytest.mark.parametrize("norm", [True, False])
+def test_modules_without_positions(dev, norm):
+    pos = tables(8, 64, dev) if norm else None
+    for m in (LinearSelfMultiheadAttn(128, 2, qk_norm=norm), WindowSelfMultiheadAttn(128, 2, window=4, qk_norm=norm)):
+        m = m.to(dev).bfloat16()
+        for t, b in ((0, 2), (3, 0)):
+            x = torch.randn(t, b, 128, device=dev).bfloat16().requires_grad_()
+            out = m(x, pos_emb=pos)
+            assert out.shape == x.shape and torch.autograd.grad(out.sum(), x)[0].shape == x.shape
