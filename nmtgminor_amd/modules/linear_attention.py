@@ -103,7 +103,8 @@ class LinearSelfMultiheadAttn(nn.Module):
 
     def forward(self, inputs, lengths=None, state=None, pos_emb=None):
         """inputs [T, B, E] -> [T, B, E]. lengths [B]: how many of the T positions are a sequence's own. pos_emb: (cos, sin) tables of
-        positions (with qk_norm); with a state, positions go on from its lengths."""
+        positions (with qk_norm); with a state, positions go on from its lengths, and one behind the tables' last row takes that row
+        (more positions in one call than the tables have are an error): the tables have to reach as far as decoding goes."""
         L.refuse_tracing("linear attention")
         t, b, _ = inputs.shape
         if self.qk_norm and pos_emb is None:
@@ -114,6 +115,8 @@ class LinearSelfMultiheadAttn(nn.Module):
             raise RuntimeError("linear attention: decoding from a state has no gradient, call it under torch.no_grad()")
         q, k, v = lin.view(t, b, 3 * self.num_heads, self.head_dim).split(self.num_heads, dim=2)
         if self.qk_norm:
+            if state is not None and lengths is None and t > pos_emb[0].shape[0]:
+                raise RuntimeError(f"linear attention: positions 0 to {t - 1} of tables of {pos_emb[0].shape[0]} rows")
             positions = None if state is None else state.lengths
             q, k = qk_norm_rotary_func(q, k, self.q_norm_weight, self.k_norm_weight, *pos_emb, positions=positions)
         with no_autocast():

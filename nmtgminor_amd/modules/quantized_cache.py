@@ -48,8 +48,8 @@ def kv_cache_attend(q, k_codes, k_scales, v_codes, v_scales, lengths, longest, w
 
 
 class QuantizedKVCache:
-    """Buffers for `capacity` positions of `batch` sequences and what they hold: `lengths` (int32 [batch] on the device) and
-    `longest` (an upper bound of them that the host knows without asking the device)."""
+    """Buffers for `capacity` positions of `batch` sequences and what they hold: `lengths` (int32 [batch] on the device),
+    `longest` and `shortest` (an upper and a lower bound of them that the host knows without asking the device)."""
 
     def __init__(self, batch, kv_heads, head_dim, capacity, bits=4, dtype=torch.bfloat16, device="cuda"):
         if bits not in (4, 8):
@@ -63,7 +63,11 @@ class QuantizedKVCache:
         self.k_codes, self.v_codes = (torch.zeros(shape + (head_dim * bits // 8,), dtype=torch.uint8, device=device) for _ in range(2))
         self.k_scales, self.v_scales = (torch.zeros(shape + (head_dim // 32,), dtype=torch.uint8, device=device) for _ in range(2))
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
-        self.longest = 0
+        self.longest = self._appended = 0
+
+    @property
+    def shortest(self):
+        return min(self._appended, self.longest)                # (a longest that is set back counts for both)
 
     @property
     def tensors(self):
@@ -79,6 +83,7 @@ class QuantizedKVCache:
         if counts is not None and counts.dtype != torch.bool:
             counts = counts.clamp(0, t)
         self.lengths += t if counts is None else counts.to(self.lengths)
+        self._appended = self.shortest + (t if counts is None else 0)
         self.longest += t
 
     def read(self, start=0, count=None):

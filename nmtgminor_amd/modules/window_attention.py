@@ -80,7 +80,8 @@ class WindowSelfMultiheadAttn(nn.Module):
     def forward(self, inputs, lengths=None, cache=None, pos_emb=None):
         """inputs [T, B, E] -> [T, B, E]. lengths [B]: as in window_attn_func; with a cache, how many of the T positions are a
         sequence's own (prompts of several lengths). pos_emb: (cos, sin) tables of positions (with qk_norm); with a cache, positions
-        go on from its lengths."""
+        go on from its lengths, and one behind the tables' last row takes that row: an error where the host knows that all sequences come
+        to it (cache.shortest)."""
         L.refuse_tracing("window attention")
         t, b, _ = inputs.shape
         if self.qk_norm and pos_emb is None:
@@ -92,6 +93,9 @@ class WindowSelfMultiheadAttn(nn.Module):
                 lin.requires_grad or self.qk_norm and (self.q_norm_weight.requires_grad or self.k_norm_weight.requires_grad)):
             raise RuntimeError("window attention: decoding from a quantised cache has no gradient, call it under torch.no_grad()")
         if self.qk_norm:
+            start = 0 if cache is None else cache.shortest
+            if cache is not None and lengths is None and start + t > pos_emb[0].shape[0]:
+                raise RuntimeError(f"window attention: positions {start} to {start + t - 1} of tables of {pos_emb[0].shape[0]} rows")
             q, k, v = lin.view(t, b, sum(sizes), self.head_dim).split(sizes, dim=2)
             q, k = qk_norm_rotary_func(q, k, self.q_norm_weight, self.k_norm_weight, *pos_emb, positions=None if cache is None else cache.lengths)
         if cache is None or cache.longest == 0:
