@@ -1,14 +1,15 @@
-"""States of linear attention at the ends of their range, executed on the CPU: the kernels' own source through tests/hostsim, called by the
+"""Linear attention at the ends of their range and precision, executed on the CPU: the kernels' own source through tests/hostsim, called by the
 C ABI, against the definition in 64 bits."""
 import pytest
 import torch
 
 import test_zzr_linear_attention_gpu as la
+import test_zzs_linear_states_gpu as ends
 from test_hostsim_linear_attention_cpu import linear
 from test_hostsim_long_context_cpu import hostsim_build, lib      # noqa: F401 (a fixture among them)
 
 pytestmark = pytest.mark.skipif(not hostsim_build.available(), reason="no clang++ to build the CPU simulator")
-F16 = torch.float16
+F16, BF16 = torch.float16, torch.bfloat16
 
 
 @pytest.mark.parametrize("t,d", [(40, 64), (100, 128)])
@@ -34,3 +35,21 @@ def test_large_columns_leave_small_ones_their_bits_in_fp16(lib, size):     # noq
     got = linear(lib, q, k, v, dout, ld, None, 1.0, F16, s0, dlast, True)
     want, mag = la.reference(q, k, v, dout, ld, None, 1.0, s0, dlast)
     la.check({n: got[n] for n in ("last", "dstate")}, want, mag)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("states", [0.0, 1.0])
+@pytest.mark.parametrize("t,d", [(5, 64), (200, 64), (130, 128), (1100, 64)])
+def test_states_have_their_bits(lib, t, d, states, dtype):     # noqa: F811
+    rows, (s0, dlast), ld = ends.few_rows(t, 3, d, dtype, "cpu", states)
+    got = linear(lib, *rows, ld, None, 0.3, dtype, s0, dlast, True)
+    want, mag = la.reference(*rows, ld, None, 0.3, s0, dlast)
+    ends.check_bits({n: got[n] for n in ("last", "dstate")}, want, mag)
+
+
+@pytest.mark.parametrize("dtype,size", [(BF16, 1e12), (BF16, 1e-12), (F16, 200.0), (F16, 1e-3)])
+def test_magnitudes(lib, dtype, size):     # noqa: F811
+    rows, scale, ld = ends.magnitudes(dtype, size, "cpu")
+    got = linear(lib, *rows, ld, None, scale, dtype, states=True)
+    want, mag = la.reference(*rows, ld, None, scale)
+    ends.check_by_type({n: x for n, x in got.items() if x.dtype != F16 or want[n].abs().max() < 6e4}, want, mag)
