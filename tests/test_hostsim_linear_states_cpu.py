@@ -1,11 +1,12 @@
-"""Linear attention at the ends of their range and precision, executed on the CPU: the kernels' own source through tests/hostsim, called by the
+"""Linear attention and the norms with rotation at the ends of their range and precision, executed on the CPU: the kernels' own source through tests/hostsim, called by the
 C ABI, against the definition in 64 bits."""
 import pytest
 import torch
 
 import test_zzr_linear_attention_gpu as la
 import test_zzs_linear_states_gpu as ends
-from test_hostsim_linear_attention_cpu import linear
+import test_zzt_norm_calls_gpu as calls
+from test_hostsim_linear_attention_cpu import linear, norm
 from test_hostsim_long_context_cpu import hostsim_build, lib      # noqa: F401 (a fixture among them)
 
 pytestmark = pytest.mark.skipif(not hostsim_build.available(), reason="no clang++ to build the CPU simulator")
@@ -53,3 +54,13 @@ def test_magnitudes(lib, dtype, size):     # noqa: F811
     got = linear(lib, *rows, ld, None, scale, dtype, states=True)
     want, mag = la.reference(*rows, ld, None, scale)
     ends.check_by_type({n: x for n, x in got.items() if x.dtype != F16 or want[n].abs().max() < 6e4}, want, mag)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_magnitudes_of_norms(lib, dtype):     # noqa: F811
+    x, pos = calls.magnitudes(dtype, "cpu"), calls.tables(8, 64, "cpu")
+    g = torch.ones_like(x)
+    out, grads, _ = norm(lib, x, x, g, g, [None, None], *pos, None, dtype)
+    want, mag = calls.reference(x, None, g, *pos, calls.rows_of(len(x), 1, None), 1e-6)
+    calls.check_by_type("out", out[0], want[0], mag[0])
+    calls.check_by_type("dx", grads[0], want[1], mag[1])

@@ -5,6 +5,7 @@ import torch
 from nmtgminor_amd.modules.linear_attention import LinearSelfMultiheadAttn, linear_attn_step
 from nmtgminor_amd.modules.qk_norm import qk_norm_rotary_func
 from nmtgminor_amd.modules.window_attention import WindowSelfMultiheadAttn
+from test_zzq_qk_norm_gpu import U, reference, rows_of
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
@@ -101,3 +102,32 @@ def test_modules_without_positions(dev, norm):
             x = torch.randn(t, b, 128, device=dev).bfloat16().requires_grad_()
             out = m(x, pos_emb=pos)
             assert out.shape == x.shape and torch.autograd.grad(out.sum(), x)[0].shape == x.shape
+
+
+SIZES = {BF16: (3e38, 1e30, 1e19, 1.0, 1e-20, 0.0), F16: (6e4, 1.0, 6e-5, 1e-7, 0.0)}
+
+
+def magnitudes(dtype, dev):
+    base = torch.randn(len(SIZES[dtype]), 1, 2, 64, generator=torch.Generator().manual_seed(2)).clamp(-1, 1)
+    return (base * torch.tensor(SIZES[dtype]).view(-1, 1, 1, 1)).to(dtype).to(dev)
+
+
+def check_by_type(name, got, want, mag):
+    """As test_zzq_qk_norm_gpu.check, with an absolute part that goes by the type: fp16 rounds its smallest values to 2^-25, bf16's
+    smallest normal number is 2^-126."""
+    u, slack = U[got.dtype], {F16: 2.0 ** -25, BF16: 2.0 ** -126}[got.dtype]
+    got = got.detach().cpu().double()
+    worst = ((got - want).abs() / (u * want.abs() + 1e-5 * mag + slack)).max().item()
+    assert torch.isfinite(got).all() and worst <= 1.0, f"{name}: {worst:.3f} of the bound"
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_magnitudes(dev, dtype):
+    """Rows of the largest and smallest numbers, every result to its own size."""
+    x, pos = magnitudes(dtype, dev).requires_grad_(), tables(8, 64, dev)
+    g = torch.ones_like(x)
+    out = qk_norm_rotary_func(x, x.detach(), None, None, *pos)[0]
+    dx, = torch.autograd.grad(out, x, g)
+    want, mag = reference(x, None, g, *pos, rows_of(len(x), 1, None), 1e-6)
+    check_by_type("out", out, want[0], mag[0])
+    check_by_type("dx", dx, want[1], mag[1])
