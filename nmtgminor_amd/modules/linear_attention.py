@@ -36,7 +36,8 @@ def linear_attn_func(q, k, v, log_decay, scale=None, lengths=None, state=None, r
 
 def linear_attn_step(q, k, v, log_decay, state, state_out=None, scale=None, lengths=None):
     """The recurrence itself, position by position, in fp32 (one position, or a few). state is written in place, or left alone with
-    another tensor state_out to write; both contiguous. lengths: how many of the T positions are a sequence's own."""
+    another tensor state_out to write; both contiguous. lengths: how many of the T positions are a sequence's own. Under autocast the
+    rows take its type, the state stays in fp32."""
     L.refuse_tracing("linear attention")
     if torch.is_autocast_enabled():
         q, k, v = cast_if_autocast_enabled(q, k, v)
@@ -62,7 +63,10 @@ class LinearSelfMultiheadAttn(nn.Module):
     from 2 to 2048 positions. Training and whole sequences: forward(inputs [T, B, E], lengths). Decoding: make_state(), then
     forward(inputs, lengths, state=state) for the prompt and for every step behind it."""
 
-    STEP = 8        # positions up to which decoding runs the recurrence: it reads the state once whatever their number
+    # Positions up to which decoding runs the recurrence, which is in 32 bits throughout, where chunks round the state for their products. us on the
+    # device, recurrence and chunk: 5 x 8 heads of 64 3.0 and 5.6 for one position, 4.3 and 5.6 for four, 6.2 and 5.6 for eight, 9.8 and 5.6
+    # for 16; 128 x 32 heads of 128 86 and 92, 99 and 97, 121 and 99, 176 and 109.
+    STEP = 8
 
     def __init__(self, embed_dim, num_heads, qk_norm=True, log_decay=None):
         super().__init__()
